@@ -221,10 +221,14 @@ def run(state: dict):
 
 # ---- plain forms -----------------------------------------------------------------------------------------------------------------
 
+def _over_127(x):
+    return x / torch.full_like(x, 127.0)      # a quotient: dividing by a Python number multiplies by its rounded reciprocal
+
+
 def _plain_linear(x, q_weight, scale, zero, bias, input_scale):
     if input_scale is not None:
         x = (x.float() / input_scale).to(x.dtype)
-    step = x.float().abs().amax(dim=1, keepdim=True).clamp(min=1e-6) / 127.0
+    step = _over_127(x.float().abs().amax(dim=1, keepdim=True).clamp(min=1e-6))
     codes = torch.round(x.float() / step)
     w = q_weight.float() if zero is None else q_weight.float() - zero[:, None]
     y = codes @ w.t() * step * scale
@@ -259,7 +263,7 @@ def _quantized(x):
     piece = max(1, (1 << 28) // max(1, math.prod(x.shape[1:])))
     for a in range(0, x.shape[0], piece):
         f = x[a:a + piece].float()
-        s = f.abs().amax(dim=(2, 3)) / 127.0
+        s = _over_127(f.abs().amax(dim=(2, 3)))
         codes[a:a + piece] = torch.where(s[..., None, None] > 0, torch.round(f / s[..., None, None]), 0.0).to(torch.int8)
         scale[a:a + piece] = s
     return codes, scale
