@@ -295,6 +295,76 @@ int pare_rope(const void* x, int64_t stride_b, int64_t stride_h, int64_t stride_
               int B, int H, int T, int D, int dtype, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Paged KV cache in 8 bits: a pool of blocks of block_size tokens (16, 32 or 64) shared by R requests (R <= 4096).  No counterpart
+ * in the reference, whose cache is one dense batch (pare/kv_cache.py:163-288); the schedule has the property of its residual
+ * window: a token's code does not depend on how the tokens were cut into calls.  One layer holds
+ *   k_codes, v_codes  [num_blocks][H][block_size][D] int8, D = 64 or 128
+ *   k_scale, v_scale  [num_blocks][H] float32: value = code * scale; scale = max |x| / 127 over the block's tokens and
+ *                     channels of the head, code = round_half_even(x / scale); a block of zeros has scale 0, one that holds
+ *                     an infinity or NaN a scale that is not finite (its values read as NaN)
+ *   tail_k, tail_v    [R][H][block_size][D] F16 / BF16: tokens of a request's open block (length % block_size of them), quantized
+ *                     when the block fills up
+ * and the requests share
+ *   seq_lens [R], block_table [R][ld_table] (max_blocks columns used; entry j holds tokens j * block_size ..),
+ *   free_blocks [free_capacity], a stack of free block ids, *free_count of them.
+ *
+ * pare_paged_plan: the tables of a STEP in which request r gets new_lens[r] more tokens (0: none), laid out one request after the
+ * other over T rows (rows behind the last token belong to nobody).  Request r takes ceil(new length / block_size) -
+ * ceil(old length / block_size) blocks from the top of the stack, in request order, entered into block_table.  Nothing else of
+ * the caller's is written; the step holds (pare_paged_step_offset(field): byte offset in `step`)
+ *   field 0  status        int32: 0, or why the step was refused as a whole (PARE_PAGED_* flags; then no row belongs to anybody)
+ *   field 1  query_start   int32 [R + 1]: first row of each request
+ *   field 2  seq_lens      int32 [R + 1]: lengths after the step, then the number of free blocks after it
+ *   field 3  context_start int64 [R + 1]: prefix sum of the lengths after the step of the requests with new tokens
+ *   field 4  slots         int64 [T]: block id * block_size + offset, -1 for rows that belong to nobody
+ *   field 5  token_request int32 [T], -1 likewise
+ *   field 6  positions     int32 [T], -1 likewise
+ * and work lists that only the calls below read.  Planning again from the same lengths gives the same step; to go on, copy
+ * seq_lens and the number of free blocks back.  `step` is 16-byte aligned, pare_paged_step_bytes() (0: sizes not supported), and
+ * need not be initialised.  Integers only, no float anywhere: exact. */
+enum {
+  PARE_PAGED_NEGATIVE = 1,   /* a length or number of new tokens is negative */
+  PARE_PAGED_ROWS = 2,       /* more new tokens than rows */
+  PARE_PAGED_TABLE = 4,      /* a request would not fit its row of block_table */
+  PARE_PAGED_BLOCKS = 8      /* not enough free blocks (or free_count out of range) */
+};
+size_t pare_paged_step_bytes(int R, int T, int block_size);
+int64_t pare_paged_step_offset(int field, int R, int T, int block_size);
+int pare_paged_plan(const int32_t* seq_lens, const int32_t* new_lens, int R, int32_t* block_table, int64_t ld_table, int max_blocks,
+                    const int32_t* free_blocks, int free_capacity, const int32_t* free_count, int block_size, int T,
+                    void* step, size_t step_bytes, void* stream);
+
+/* Blocks of every request with release[r] != 0 back onto the stack (request order, oldest block first); its length becomes 0. */
+int pare_paged_release(const int32_t* release, int32_t* seq_lens, int R, const int32_t* block_table, int64_t ld_table, int max_blocks,
+                       int32_t* free_blocks, int free_capacity, int32_t* free_count, int block_size, void* stream);
+
+/* The step's new keys and values [T][H][D] (element strides, multiples of 8; channels contiguous; 16-byte aligned) into one layer.
+ * Ids that are not in the pool are not written to. */
+int pare_paged_append(const void* k, const void* v, int dtype, int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t,
+                      int64_t v_stride_h, const void* step, int R, int T, int block_size,
+                      int8_t* k_codes, int8_t* v_codes, float* k_scale, float* v_scale, void* tail_k, void* tail_v,
+                      int num_blocks, int H, int D, void* stream);
+
+/* Keys and values, after the step, of every request with new tokens in it: out_k / out_v [total][H][D] dense, request r's from row
+ * context_start[r] on; rows behind the last are zeros, rows beyond `total` are left out.  Ids not in the pool read as NaN. */
+int pare_paged_dense(const void* step, int R, int T, int block_size, const int32_t* block_table, int64_t ld_table, int max_blocks,
+                     const int8_t* k_codes, const int8_t* v_codes, const float* k_scale, const float* v_scale,
+                     const void* tail_k, const void* tail_v, int num_blocks, int H, int D,
+                     void* out_k, void* out_v, int dtype, int64_t total, void* stream);
+
+/* Attention of the step's tokens over the layer, after the step's append: token t of request r attends to the positions up to its
+ * own.  q, out [T][Hq][D] (element strides; q's multiples of 8, 16-byte aligned), query head hq reads KV head hq / (Hq / H), any
+ * ratio; T <= 4096.  Rows that belong to nobody are left as they were.  Ids not in the pool read as NaN.  The workspace
+ * (16-byte aligned, pare_paged_attn_workspace_bytes()) need not be initialised and holds nothing between calls. */
+size_t pare_paged_attn_workspace_bytes(int D);
+int pare_paged_attn(const void* q, int dtype, int64_t q_stride_t, int64_t q_stride_h, const void* step, int R, int T, int block_size,
+                    const int32_t* block_table, int64_t ld_table, int max_blocks,
+                    const int8_t* k_codes, const int8_t* v_codes, const float* k_scale, const float* v_scale,
+                    const void* tail_k, const void* tail_v, int num_blocks, int Hq, int H, int D,
+                    void* out, int64_t out_stride_t, int64_t out_stride_h, float softmax_scale,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * W4A16 decode linear without any caller-provided workspace.  No counterpart in the reference;
  * it exists for callers that cannot allocate device memory (code running inside another
  * runtime's callback or memory pool where cudaMalloc is forbidden or would synchronise, or code

@@ -3,7 +3,7 @@
 Same names as the reference's top-level package (``pare/__init__.py:7-18``) for everything on
 the run-time path: ``QuantConfig``, ``QuantDtype``, ``QuantizedLinear`` (via
 ``pare_b200.layers``), ``save_quantized`` / ``load_quantized``, ``KVCacheConfig`` /
-``QuantizedKVCache``.  ``quantize`` covers round-to-nearest only: the calibration-based
+``QuantizedKVCache``.  ``PagedKVConfig`` / ``PagedKVCache`` (a paged 8-bit cache for requests of their own lengths) come on top.  ``quantize`` covers round-to-nearest only: the calibration-based
 solvers (GPTQ, AWQ, SmoothQuant) are offline tools that end in the same ``QuantizedLinear``
 buffers and are not part of this package.
 """
@@ -21,10 +21,12 @@ from pare_b200.core.dtype import QuantDtype
 from pare_b200.kv_cache import KVCacheConfig, QuantizedKVCache
 from pare_b200.layers.linear import QuantizedLinear
 from pare_b200.model.io import load_quantized, save_quantized
+from pare_b200.paged_cache import PagedKVCache, PagedKVConfig
 
 __all__ = [
     "QuantConfig", "QuantDtype", "QuantizedLinear", "quantize",
-    "save_quantized", "load_quantized", "KVCacheConfig", "QuantizedKVCache", "__version__",
+    "save_quantized", "load_quantized", "KVCacheConfig", "QuantizedKVCache", "PagedKVConfig", "PagedKVCache",
+    "__version__",
 ]
 
 

@@ -1,0 +1,46 @@
+// Shared by the kernels of the paged 8-bit KV cache (paged_cache.cu, paged_attn.cu): the layout of a step's tables.
+#pragma once
+
+#include "common.cuh"
+
+namespace pare {
+namespace paged {
+
+constexpr int kMaxRequests = 4096;
+constexpr int kMaxQueryTokens = 4096;      // tokens of a step that attention is planned for
+constexpr int kMaxTokens = 1 << 22;
+constexpr int kUnit = 16;                  // tokens per unit of attention work
+constexpr int kItemInts = 8;               // request, block id, first row, offset in the block, tokens, block index, length before, length after
+
+inline bool block_size_ok(int bs) { return bs == 16 || bs == 32 || bs == 64; }
+
+// Blocks that T new tokens of at most R requests touch: one per token at most; a request with n tokens touches ceil((n - 1) / bs) + 1.
+inline int max_items(int R, int T, int bs) {
+  const int64_t a = (int64_t)T / bs + 2ll * (R < T ? R : T);
+  return (int)(a < T ? a : T);
+}
+
+// A step: one buffer of 32-bit words, every array on a 16-byte boundary.
+struct StepLayout {
+  int64_t status, query_start, seq_lens, context_start, token_request, positions, slots, unit_start, items, words;
+  int n_items;
+  bool units;
+  __host__ StepLayout(int R, int T, int bs) {
+    auto up = [](int64_t w) { return (w + 3) / 4 * 4; };
+    n_items = max_items(R, T, bs);
+    units = T <= kMaxQueryTokens;
+    status = 0;
+    query_start = 4;
+    seq_lens = query_start + up(R + 1);            // [R] lengths, then the number of free blocks
+    context_start = seq_lens + up(R + 1);          // [R + 1] 64-bit
+    slots = context_start + up(2 * ((int64_t)R + 1));   // [T] 64-bit
+    token_request = slots + up(2 * (int64_t)T);
+    positions = token_request + up(T);
+    unit_start = positions + up(T);
+    items = unit_start + up(units ? T + 1 : 0);
+    words = items + (int64_t)n_items * kItemInts;
+  }
+};
+
+}  // namespace paged
+}  // namespace pare

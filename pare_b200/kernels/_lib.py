@@ -74,6 +74,17 @@ SIGNATURES: dict[str, tuple] = {
                                                    _i, _i, _i, _i, _vp, _sz, _i, _i, C.POINTER(C.c_void_p), _sz, _vp]),
     "pare_workspace_status": (_i, [_vp, _vp]),
     "pare_selftest_bounded_wait": (_i, [_vp, C.c_uint, _vp]),
+    "pare_paged_step_bytes": (_sz, [_i, _i, _i]),
+    "pare_paged_step_offset": (_i64, [_i, _i, _i, _i]),
+    "pare_paged_plan": (_i, [_vp, _vp, _i, _vp, _i64, _i, _vp, _i, _vp, _i, _i, _vp, _sz, _vp]),
+    "pare_paged_release": (_i, [_vp, _vp, _i, _vp, _i64, _i, _vp, _i, _vp, _i, _vp]),
+    "pare_paged_append": (_i, [_vp, _vp, _i, _i64, _i64, _i64, _i64, _vp, _i, _i, _i,
+                               _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
+    "pare_paged_dense": (_i, [_vp, _i, _i, _i, _vp, _i64, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i,
+                              _vp, _vp, _i, _i64, _vp]),
+    "pare_paged_attn_workspace_bytes": (_sz, [_i]),
+    "pare_paged_attn": (_i, [_vp, _i, _i64, _i64, _vp, _i, _i, _i, _vp, _i64, _i, _vp, _vp, _vp, _vp, _vp, _vp,
+                             _i, _i, _i, _i, _vp, _i64, _i64, C.c_float, _vp, _sz, _vp]),
     "pare_w4a16_static_status": (_i, [_vp]),
     "pare_w4a16_static_scratch_bytes": (_sz, []),
     "pare_w4a16_forward_static": (_i, [_vp, _i, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64,
