@@ -295,6 +295,25 @@ int pare_rope(const void* x, int64_t stride_b, int64_t stride_h, int64_t stride_
               int B, int H, int T, int D, int dtype, void* stream);
 
 /* ------------------------------------------------------------------------
+ * W8A8 linear: Y[M,N] = X . W^T in 8-bit integers with a scale per token and per output channel.  The reference's quantize_inputs
+ * branch (pare/layers/linear.py:121-138) rounds the activations to 127 steps per token and multiplies in floats; here the steps
+ * themselves are multiplied:
+ *   x~ = x, or dtype(x / input_scale);  step = max(max_k |x~|, 1e-6) / 127;  c = round_half_even(x~ / step) in [-127, 127]
+ *   y = dtype((sum_k c q - zero sum_k c) * step * scale + bias)
+ *   x            [M, ldx]  F16 or BF16
+ *   weight       [N, ldw]  int8, ldw >= K a multiple of 16, 16-byte aligned
+ *   scale, zero  [N] float32 (zero may be NULL = 0)
+ *   input_scale  optional [K] float32, divides the activations first (the quotient rounded to their dtype)
+ *   bias         optional [N] x_dtype;   y [M, ldy] x_dtype
+ * The integer sums are exact (K <= 65536; zero-points up to 128 in magnitude are taken off in integers, others in float32).  Rows
+ * with an infinity or NaN give NaN.  The workspace (16-byte aligned, pare_w8a8_workspace_bytes(), 0: sizes not supported) need
+ * not be initialised and holds nothing between calls.  A bounded wait that runs out shows as NaN in the outputs it concerns. */
+size_t pare_w8a8_workspace_bytes(int M, int N, int K);
+int pare_w8a8_forward(const void* x, int x_dtype, int64_t ldx, const int8_t* weight, int64_t ldw, const float* scale,
+                      const float* zero, const float* input_scale, const void* bias, void* y, int64_t ldy,
+                      int M, int N, int K, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * Paged KV cache in 8 bits: a pool of blocks of block_size tokens (16, 32 or 64) shared by R requests (R <= 4096).  No counterpart
  * in the reference, whose cache is one dense batch (pare/kv_cache.py:163-288); the schedule has the property of its residual
  * window: a token's code does not depend on how the tokens were cut into calls.  One layer holds

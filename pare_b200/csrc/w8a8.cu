@@ -1,0 +1,537 @@
+// W8A8 linear, sm_100a: tokens quantized to int8 with a scale each, int8 weights with a scale (and zero-point) per output channel,
+// integer products on tcgen05.mma kind::i8, everything else in the epilogue.  What the reference has as an eager
+// fake-quantization (quantize_inputs, SmoothQuant W8A8: pare/layers/linear.py:121-138) in real integers:
+//   x~ = x, or dtype(x / input_scale)      step_m = max(max_k |x~_mk|, 1e-6) / 127      c_mk = round_half_even(x~_mk / step_m)
+//   y_mn = dtype((sum_k c_mk q_nk - z_n sum_k c_mk) * step_m s_n + b_n)
+// The sums are exact 32-bit integers, so neither tiles nor splits of K nor their order change a bit of the result.
+//
+// Two launches: the tokens' codes (one thread block per row), then the product.  The second starts while the first runs and fills
+// its ring with weights, which the first does not write; it waits before it touches anything else.
+//
+// The product: as in w4a16_gemm.cu the 128 rows of a weight tile sit on the MMA's M axis (the TMEM lanes), activation rows on its N
+// axis, one persistent thread block per SM, each with one contiguous run of (weight tile, activation tile, 128-column unit); tiles
+// that span runs are added up by whoever arrives last.  Both operands come by TMA (128-byte rows, 128B swizzle) and are multiplied
+// where they land; the accumulator is double-buffered in tensor memory so a tile's epilogue overlaps the next tile's products.
+//   warp 0     TMA of both operands      warp 1  tcgen05.mma      warp 2  tensor memory      warps 4-7  epilogue
+// All waits are bounded; when one runs out the thread block stops waiting and loading, lets its copies and products in flight
+// end, and its outputs become NaN.
+#include "tcgen05.cuh"
+
+namespace pare {
+namespace {
+
+using namespace tc;
+
+constexpr int kRows = 128;               // weight rows per tile (UMMA M)
+constexpr int kUnitK = 128;              // columns per unit: one 128-byte swizzle row, four MMAs
+constexpr int kWBytes = kRows * kUnitK;
+constexpr int kMaxStages = 12;
+constexpr int kThreads = 256;
+constexpr uint32_t kTmemCols = 512;      // two accumulators of up to 256 columns
+constexpr int kMaxSmem = 224 * 1024;    // beside 2 KB of static shared memory
+constexpr int kRingBytes = kMaxSmem - 1024 - 512;
+constexpr int kMaxK = 65536;             // 65536 * 127 * (128 + 128) < 2^31
+
+// ---- tokens -> codes ----------------------------------------------------------------------------------------------------------------
+constexpr int kQuantThreads = 256;
+
+struct QuantParams {
+  const void* x;
+  int64_t ldx;
+  const float* input_scale;
+  int8_t* codes;
+  int64_t ldc;
+  float* step;
+  int* sums;
+  int* zeroed;      // words the product's thread blocks count in
+  int n_zeroed, K;
+};
+
+template <typename T>
+__device__ __forceinline__ T smoothed(T v, const float* input_scale, int k) {
+  return input_scale ? from_float<T>(__fdiv_rn(to_float<T>(v), __ldg(input_scale + k))) : v;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t magnitude(T v) {   // orders like |v|, infinities and NaN above all numbers
+  return *reinterpret_cast<const uint16_t*>(&v) & 0x7fffu;
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kQuantThreads) w8a8_quantize_kernel(const QuantParams p) {
+  pdl_launch_dependents();
+  constexpr int kW = kQuantThreads / 32;
+  __shared__ uint32_t s_top[kW];
+  __shared__ int s_sum[kW];
+  const int m = blockIdx.x, tid = threadIdx.x;
+  const T* row = reinterpret_cast<const T*>(p.x) + m * p.ldx;
+  int8_t* out = p.codes + m * p.ldc;
+  for (int i = m * kQuantThreads + tid; i < p.n_zeroed; i += gridDim.x * kQuantThreads) p.zeroed[i] = 0;
+  uint32_t top = 0;
+  if (VEC) {
+    for (int k = tid * 8; k < p.K; k += kQuantThreads * 8) {
+      const uint4 w = *reinterpret_cast<const uint4*>(row + k);
+      const T* v = reinterpret_cast<const T*>(&w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = max(top, magnitude(smoothed<T>(v[j], p.input_scale, k + j)));
+    }
+  } else {
+    for (int k = tid; k < p.K; k += kQuantThreads) top = max(top, magnitude(smoothed<T>(row[k], p.input_scale, k)));
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((tid & 31) == 0) s_top[tid >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kW; ++w) top = max(top, s_top[w]);
+  const uint16_t bits = (uint16_t)top;
+  const float amax = to_float<T>(*reinterpret_cast<const T*>(&bits));
+  // a row with an infinity or NaN has a step that is not finite, so its outputs are NaN
+  const float step = __fdiv_rn(amax < 1e-6f ? 1e-6f : amax, 127.f);
+  const bool finite = step < INFINITY;
+  const float inv = finite ? __fdiv_rn(1.f, step) : 0.f;
+  int sum = 0;
+  // round(x / step): the product with 1 / step decides except next to a border between two codes (within 1e-4; its own error is
+  // below 2e-5), where the quotient does
+  auto code = [&](T v) {
+    const float x = to_float<T>(v), t = x * inv;
+    float c = rintf(t);
+    if (fabsf(t - c) > 0.4999f) c = rintf(__fdiv_rn(x, step));
+    const int q = finite ? (int)fminf(fmaxf(c, -127.f), 127.f) : 0;
+    sum += q;
+    return q;
+  };
+  if (VEC) {
+    for (int k = tid * 8; k < p.K; k += kQuantThreads * 8) {
+      const uint4 w = *reinterpret_cast<const uint4*>(row + k);
+      const T* v = reinterpret_cast<const T*>(&w);
+      uint32_t o[2] = {0, 0};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j >> 2] |= ((uint32_t)code(smoothed<T>(v[j], p.input_scale, k + j)) & 0xffu) << (8 * (j & 3));
+      *reinterpret_cast<uint2*>(out + k) = make_uint2(o[0], o[1]);
+    }
+  } else {
+    for (int k = tid; k < p.K; k += kQuantThreads) out[k] = (int8_t)code(smoothed<T>(row[k], p.input_scale, k));
+  }
+  sum = __reduce_add_sync(0xffffffffu, sum);
+  if ((tid & 31) == 0) s_sum[tid >> 5] = sum;
+  __syncthreads();
+  if (tid == 0) {
+    int all = 0;
+#pragma unroll
+    for (int w = 0; w < kW; ++w) all += s_sum[w];
+    p.step[m] = finite ? step : __int_as_float(0x7fffffff);
+    p.sums[m] = all;
+  }
+}
+
+// ---- product --------------------------------------------------------------------------------------------------------------------------
+struct W8Params {
+  const float* step;     // [M]
+  const int* sums;       // [M]
+  const float* scale;    // [N]
+  const float* zero;     // [N] or NULL
+  const void* bias;
+  void* y;
+  int64_t ldy;
+  int M, N;
+  int mt;                // activation rows per tile (UMMA N), a multiple of 16
+  int mtiles;
+  int ku;                // units per tile
+  int total_units, run_units, stages;
+  int* partial;          // [thread block][2][mt / 4][128][4]: a run's first tile (begun by another) and its last (not finished)
+  int* counters;         // [thread block]: arrivals at the tile that it begins and others continue; behind them a word for failures
+};
+
+// both operands in shared memory, 8-bit integers
+__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate, uint32_t elected) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(da), "l"(db), "r"(idesc), "r"(accumulate), "r"(elected)
+      : "memory");
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1) w8a8_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
+                                                                const W8Params p) {
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ int s_failed, s_flag;
+  __shared__ float s_step[256];
+  __shared__ int s_sums[256];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int stages = p.stages, ku = p.ku;
+  const uint32_t x_bytes = (uint32_t)p.mt * kUnitK, w_ring = s_u32(smem), x_ring = w_ring + stages * kWBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + stages * (kWBytes + x_bytes));
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kMaxStages + 5);
+  const uint32_t full = s_u32(bars), empty = full + kMaxStages * 8, acc_full = empty + kMaxStages * 8, acc_empty = acc_full + 16,
+                 mma_done = acc_empty + 16;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int u0 = blockIdx.x * p.run_units, u1 = min(u0 + p.run_units, p.total_units);
+  bool dead = false;
+  int* status = &s_failed;
+
+  if (threadIdx.x == 0) {
+    s_failed = 0;
+    for (int i = 0; i < kMaxStages; ++i) {
+      bar_init(full + i * 8, 1);
+      bar_init(empty + i * 8, 1);
+    }
+    bar_init(mma_done, 1);
+    for (int i = 0; i < 2; ++i) {
+      bar_init(acc_full + i * 8, 1);
+      bar_init(acc_empty + i * 8, 4);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 2) {  // one thread block per SM (its shared memory sees to that): it takes all of tensor memory
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_u32(tmem_slot)), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+
+  if (warp == 0) {
+    // ================= operands =================
+    if (lane == 0) {
+      const int n = u1 - u0;
+      auto load_w = [&](int i, int s) {
+        const int t = (u0 + i) / ku, k = u0 + i - t * ku;
+        bar_expect(full + s * 8, kWBytes + x_bytes);
+        tma_tile(w_ring + s * kWBytes, &tm_w, k * kUnitK, t / p.mtiles * kRows, full + s * 8);
+      };
+      auto load_x = [&](int i, int s) {
+        const int t = (u0 + i) / ku, k = u0 + i - t * ku;
+        tma_tile(x_ring + s * x_bytes, &tm_x, k * kUnitK, t % p.mtiles * p.mt, full + s * 8);
+      };
+      int i = 0;
+      for (; i < min(n, stages); ++i) load_w(i, i);     // weights: nothing that this launch may overlap writes them
+      pdl_wait();
+      for (int j = 0; j < i; ++j) load_x(j, j);
+      int s = 0;
+      uint32_t par = 0;
+      for (; i < n; ++i) {
+        bar_wait(empty + s * 8, par, status, dead);
+        if (dead) break;
+        load_w(i, s);
+        load_x(i, s);
+        if (++s == stages) s = 0, par ^= 1;
+      }
+      bool late = false;
+      for (int j = max(0, i - stages); j < i; ++j) bar_wait(full + (j % stages) * 8, (j / stages) & 1, status, late);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ================= products =================
+    const uint32_t me = elect_one();
+    const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(p.mt >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+    const uint64_t w_desc0 = umma_desc(w_ring), x_desc0 = umma_desc(x_ring);
+    int s = 0, seg = 0;
+    uint32_t par = 0;
+    for (int u = u0; u < u1; ++seg) {
+      const int n = min(ku - u % ku, u1 - u), buf = seg & 1;
+      const uint32_t acc = tmem + buf * 256;
+      bar_wait(acc_empty + buf * 8, ((seg >> 1) & 1) ^ 1, status, dead);
+      for (int i = 0; i < n; ++i) {
+        bar_wait(full + s * 8, par, status, dead);
+        __syncwarp();
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint64_t dw = w_desc0 + (uint64_t)(s * (kWBytes >> 4)), dx = x_desc0 + (uint64_t)(s * (x_bytes >> 4));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) umma_i8(acc, dw + 2 * j, dx + 2 * j, idesc, (i | j) != 0, me);
+        umma_commit(empty + s * 8, me);
+        if (++s == stages) s = 0, par ^= 1;
+      }
+      umma_commit(acc_full + buf * 8, me);
+      u += n;
+    }
+    umma_commit(mma_done, me);
+    bool late = false;
+    bar_wait(mma_done, 0, status, late);
+    __syncwarp();
+  } else if (warp >= 4) {
+    // ================= epilogue: tensor memory -> registers -> global =================
+    pdl_wait();
+    const int q4 = warp & 3, te = threadIdx.x - 4 * 32;
+    T* yg = reinterpret_cast<T*>(p.y);
+    const T* bias = reinterpret_cast<const T*>(p.bias);
+    const bool pair_out = (reinterpret_cast<uintptr_t>(p.y) & 3u) == 0 && (p.ldy & 1) == 0 && (p.N & 1) == 0;
+    auto epi_sync = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
+    int* failures = p.counters + gridDim.x;
+    int seg = 0;
+    for (int u = u0; u < u1; ++seg) {
+      const int t = u / ku, k0 = u - t * ku, len = min(ku - k0, u1 - u);
+      u += len;
+      const int row0 = t / p.mtiles * kRows, m0 = t % p.mtiles * p.mt;
+      const int n = row0 + q4 * 32 + lane, mrows = min(p.mt, p.M - m0);
+      const int buf = seg & 1;
+      const uint32_t acc = tmem + buf * 256 + ((uint32_t)(q4 * 32) << 16);
+      const float bv = (bias && n < p.N) ? to_float<T>(bias[n]) : 0.f, sv = n < p.N ? p.scale[n] : 0.f;
+      // the zero-point's whole part is taken off in integers, exactly; what is left (0 for the zero-points of quantizers, or a
+      // value beyond any code) in fp32
+      const float z = (p.zero && n < p.N) ? p.zero[n] : 0.f;
+      const int zi = fabsf(z) <= 128.f ? __float2int_rn(z) : 0;
+      const float zf = z - (float)zi;
+      epi_sync();     // the tile before has been written
+      for (int i = te; i < mrows; i += 128) {
+        s_step[i] = p.step[m0 + i];
+        s_sums[i] = p.sums[m0 + i];
+      }
+      epi_sync();
+      bool bad = false;
+      const int odd = lane & 1;
+      T* const mine_at = yg + (int64_t)(m0 + odd) * p.ldy + (n & ~1);
+      auto store16 = [&](const int (&a)[16], int c) {
+        float f[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int m = min(c + i, 255), xs = s_sums[m];
+          float v = (float)(a[i] - zi * xs);
+          if (p.zero) v = fmaf(-zf, (float)xs, v);
+          f[i] = bad ? __int_as_float(0x7fffffff) : fmaf(v, s_step[m] * sv, bv);
+        }
+        if (pair_out) {   // neighbouring lanes swap so that each stores two columns of every other row
+          T* at = mine_at + (int64_t)c * p.ldy;
+#pragma unroll
+          for (int i = 0; i < 16; i += 2, at += 2 * p.ldy) {
+            const float mine = odd ? f[i + 1] : f[i], got = __shfl_xor_sync(0xffffffffu, odd ? f[i] : f[i + 1], 1);
+            const uint32_t w = odd ? Pair<T>::pack(got, mine) : Pair<T>::pack(mine, got);
+            if (c + i + odd < mrows && n < p.N) *reinterpret_cast<uint32_t*>(at) = w;
+          }
+        } else if (n < p.N) {
+          T* at = yg + (int64_t)(m0 + c) * p.ldy + n;
+#pragma unroll
+          for (int i = 0; i < 16; ++i, at += p.ldy)
+            if (c + i < mrows) *at = from_float<T>(f[i]);
+        }
+      };
+      bar_wait(acc_full + buf * 8, (seg >> 1) & 1, status, dead);
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      bad = __any_sync(0xffffffffu, dead || *const_cast<volatile int*>(&s_failed) != 0);
+      auto load16 = [&](int c, int (&a)[16]) {
+        uint32_t v[16];
+        tmem_ld16(acc + c, v);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) a[i] = (int)v[i];
+      };
+      if (len == ku) {
+        for (int c = 0; c < mrows; c += 16) {
+          int a[16];
+          load16(c, a);
+          store16(a, c);
+        }
+      } else {
+        // ---- the tile spans the runs of thread blocks first .. last; whoever arrives last adds the parts ----
+        const int first = (int)((int64_t)t * ku / p.run_units), last = (int)(((int64_t)t * ku + ku - 1) / p.run_units), me = blockIdx.x;
+        const size_t slot_ints = (size_t)p.mt * kRows;
+        int* counter = p.counters + first;
+        auto slot_of = [&](int b) {   // [mt / 4][128 n][4 m]: four rows of this thread's column per 16-byte access
+          return reinterpret_cast<int4*>(p.partial + ((size_t)b * 2 + (b == first ? 1 : 0)) * slot_ints) + q4 * 32 + lane;
+        };
+        if (bad && lane == 0) atomicExch(failures, 1);
+        epi_sync();
+        if (te == 0) {
+          int have;
+          asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(have) : "l"(counter) : "memory");
+          s_flag = have == last - first;
+        }
+        epi_sync();
+        const bool in_tmem = s_flag != 0;   // all others are there already: this part need not leave tensor memory
+        bool finish = in_tmem;
+        if (!in_tmem) {
+          int4* dst = slot_of(me);
+          for (int c = 0; c < mrows; c += 16) {
+            int a[16];
+            load16(c, a);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) __stcg(dst + (c / 4 + i) * kRows, make_int4(a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3]));
+          }
+          __threadfence();
+          epi_sync();
+          if (te == 0) s_flag = atomicAdd(counter, 1) == last - first;
+          epi_sync();
+          finish = s_flag != 0;
+        }
+        if (finish) {
+          __threadfence();
+          bad = bad || __ldcg(failures) != 0;
+          for (int c = 0; c < mrows; c += 16) {
+            int a[16];
+            if (in_tmem) {
+              load16(c, a);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) a[i] = 0;
+            }
+#pragma unroll 2
+            for (int b = first; b <= last; ++b) {
+              if (in_tmem && b == me) continue;
+              const int4* src = slot_of(b) + c / 4 * kRows;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int4 v = __ldcg(src + i * kRows);
+                a[4 * i] += v.x;
+                a[4 * i + 1] += v.y;
+                a[4 * i + 2] += v.z;
+                a[4 * i + 3] += v.w;
+              }
+            }
+            store16(a, c);
+          }
+        }
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) bar_arrive(acc_empty + buf * 8);
+    }
+  }
+
+  // ---- teardown: everyone done with tensor memory, then free it ----
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 2) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
+// ---- host side --------------------------------------------------------------------------------------------------------------------------
+struct W8Plan {
+  int mt, mtiles, ku, run, blocks, stages;
+  int64_t units;
+};
+
+// Heights of the activation tiles (equal, multiples of 16) and runs by an estimate in microseconds.
+W8Plan w8_plan(int M, int N, int K) {
+  W8Plan best{};
+  double least = 1e30;
+  const int sms = sm_count();
+  int seen = 0;
+  for (int target : {256, 192, 128, 96, 64, 32, 16}) {
+    W8Plan g{};
+    g.mtiles = (M + target - 1) / target;
+    g.mt = ((M + g.mtiles - 1) / g.mtiles + 15) / 16 * 16;
+    g.mtiles = (M + g.mt - 1) / g.mt;
+    if (g.mt == seen) continue;
+    seen = g.mt;
+    g.ku = (K + kUnitK - 1) / kUnitK;
+    const int64_t tiles = (int64_t)((N + kRows - 1) / kRows) * g.mtiles;
+    g.units = tiles * g.ku;
+    const double unit_us = 0.15 + 0.0006 * g.mt;
+    auto consider = [&](int64_t run) {
+      if (run < 1 || (g.units + run - 1) / run > sms) return;
+      double cost = run * unit_us + 0.01 * g.mt;
+      if (run % g.ku) cost += 1.5 + 0.008 * g.mt * ((g.ku + run - 1) / run + (g.ku % run != 0));
+      if (cost < least - 1e-9) {
+        least = cost;
+        g.run = (int)run;
+        best = g;
+      }
+    };
+    consider((tiles + sms - 1) / sms * g.ku);
+    consider((g.units + sms - 1) / sms);
+    for (int parts = 2; parts <= 16; ++parts) consider((g.ku + parts - 1) / parts);
+  }
+  best.blocks = (int)((best.units + best.run - 1) / best.run);
+  best.stages = kRingBytes / (kWBytes + best.mt * kUnitK);
+  if (best.stages > kMaxStages) best.stages = kMaxStages;
+  return best;
+}
+
+struct W8Space {
+  size_t codes, step, sums, counters, partial, bytes;
+  int64_t ldc;
+  W8Space(const W8Plan& g, int M, int K) {
+    auto up = [](size_t b) { return (b + 255) / 256 * 256; };
+    ldc = (K + 15) / 16 * 16;
+    codes = 0;
+    step = up((size_t)M * ldc);
+    sums = step + up((size_t)M * 4);
+    counters = sums + up((size_t)M * 4);
+    partial = counters + up(((size_t)g.blocks + 1) * 4);
+    bytes = partial + (g.run % g.ku ? (size_t)g.blocks * 2 * g.mt * kRows * 4 : 0);
+  }
+};
+
+}  // namespace
+}  // namespace pare
+
+extern "C" {
+
+using namespace pare;
+
+size_t pare_w8a8_workspace_bytes(int M, int N, int K) {
+  if (M <= 0 || N <= 0 || K <= 0 || K > kMaxK) return 0;
+  return W8Space(w8_plan(M, N, K), M, K).bytes;
+}
+
+int pare_w8a8_forward(const void* x, int x_dtype, int64_t ldx, const int8_t* weight, int64_t ldw, const float* scale, const float* zero,
+                      const float* input_scale, const void* bias, void* y, int64_t ldy, int M, int N, int K, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  PARE_REQUIRE(M > 0 && N > 0 && K > 0 && ldw >= K && ldy >= N && (M == 1 || ldx >= K), PARE_ERR_SHAPE);
+  PARE_REQUIRE(x_dtype == PARE_F16 || x_dtype == PARE_BF16, PARE_ERR_DTYPE);
+  PARE_REQUIRE(x && weight && scale && y, PARE_ERR_SHAPE);
+  PARE_REQUIRE(K <= kMaxK, PARE_ERR_UNSUPPORTED);
+  PARE_REQUIRE(aligned16(weight) && ldw % 16 == 0 && aligned16(workspace), PARE_ERR_ALIGN);
+  const W8Plan g = w8_plan(M, N, K);
+  PARE_REQUIRE(g.units + g.run < (int64_t)1 << 31, PARE_ERR_UNSUPPORTED);
+  const W8Space sp(g, M, K);
+  PARE_REQUIRE(workspace && workspace_bytes >= sp.bytes, PARE_ERR_WORKSPACE);
+  unsigned char* ws = reinterpret_cast<unsigned char*>(workspace);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  EncodeTiledFn enc = encode_fn();
+  PARE_REQUIRE(enc != nullptr, PARE_ERR_CUDA);
+
+  // tensor maps: both operands in rows of K bytes, boxes of 128 bytes, 128B swizzle; rows and columns beyond the end read as zeros
+  auto map = [&](CUtensorMap* tm, const void* base, int rows, int64_t pitch, int box_rows) {
+    const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)pitch};
+    const cuuint32_t box[2] = {(cuuint32_t)kUnitK, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+    return enc(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  CUtensorMap tw, tx;
+  PARE_REQUIRE(map(&tw, weight, N, ldw, kRows) && map(&tx, ws + sp.codes, M, sp.ldc, g.mt), PARE_ERR_CUDA);
+
+  const QuantParams q{x, ldx, input_scale, reinterpret_cast<int8_t*>(ws + sp.codes), sp.ldc, reinterpret_cast<float*>(ws + sp.step),
+                      reinterpret_cast<int*>(ws + sp.sums), reinterpret_cast<int*>(ws + sp.counters), g.blocks + 1, K};
+  const bool vec = aligned16(x) && (M == 1 || ldx % 8 == 0) && K % 8 == 0;
+  if (x_dtype == PARE_F16) {
+    if (vec) w8a8_quantize_kernel<__half, true><<<M, kQuantThreads, 0, st>>>(q);
+    else w8a8_quantize_kernel<__half, false><<<M, kQuantThreads, 0, st>>>(q);
+  } else {
+    if (vec) w8a8_quantize_kernel<__nv_bfloat16, true><<<M, kQuantThreads, 0, st>>>(q);
+    else w8a8_quantize_kernel<__nv_bfloat16, false><<<M, kQuantThreads, 0, st>>>(q);
+  }
+  if (cudaGetLastError() != cudaSuccess) return PARE_ERR_CUDA;
+
+  W8Params p{};
+  p.step = q.step;
+  p.sums = q.sums;
+  p.scale = scale;
+  p.zero = zero;
+  p.bias = bias;
+  p.y = y;
+  p.ldy = ldy;
+  p.M = M;
+  p.N = N;
+  p.mt = g.mt;
+  p.mtiles = g.mtiles;
+  p.ku = g.ku;
+  p.total_units = (int)g.units;
+  p.run_units = g.run;
+  p.stages = g.stages;
+  p.partial = reinterpret_cast<int*>(ws + sp.partial);
+  p.counters = q.zeroed;
+  const size_t smem = 1024 + (size_t)g.stages * (kWBytes + g.mt * kUnitK) + 512;
+  auto launch = [&](auto kern) -> int {
+    if (!ensure_smem_attr(reinterpret_cast<const void*>(kern), kMaxSmem)) return PARE_ERR_CUDA;
+    const int rc = launch_pdl(kern, dim3(g.blocks), dim3(kThreads), smem, st, tw, tx, p);
+    return rc != PARE_OK ? rc : launch_status();
+  };
+  return x_dtype == PARE_F16 ? launch(w8a8_gemm_kernel<__half>) : launch(w8a8_gemm_kernel<__nv_bfloat16>);
+}
+
+}  // extern "C"

@@ -74,6 +74,8 @@ SIGNATURES: dict[str, tuple] = {
                                                    _i, _i, _i, _i, _vp, _sz, _i, _i, C.POINTER(C.c_void_p), _sz, _vp]),
     "pare_workspace_status": (_i, [_vp, _vp]),
     "pare_selftest_bounded_wait": (_i, [_vp, C.c_uint, _vp]),
+    "pare_w8a8_workspace_bytes": (_sz, [_i, _i, _i]),
+    "pare_w8a8_forward": (_i, [_vp, _i, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _vp, _sz, _vp]),
     "pare_paged_step_bytes": (_sz, [_i, _i, _i]),
     "pare_paged_step_offset": (_i64, [_i, _i, _i, _i]),
     "pare_paged_plan": (_i, [_vp, _vp, _i, _vp, _i64, _i, _vp, _i, _vp, _i, _i, _vp, _sz, _vp]),

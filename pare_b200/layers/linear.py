@@ -27,6 +27,10 @@ Differences, all additive:
   honoured by ``dequantize`` / the eager branch as well as by the kernel.
 * ``kernel_meta_fp16 = True`` makes the kernel read fp16 copies of scale and zero
   (half the metadata traffic, scale rounded to 11 bits).
+* ``int8_kernel = True`` (with ``use_kernel``, on an INT8 layer with ``quantize_inputs``) multiplies the int8 activations and
+  weights as integers on the tensor cores instead of fake-quantizing and multiplying in floats; per_channel and per_tensor
+  scales.  Off by default: the eager branch rounds the activations' step and the weights to the input dtype, the integer
+  product rounds neither, so the two differ by those roundings.
 """
 
 from __future__ import annotations
@@ -41,6 +45,7 @@ from pare_b200.core.functional import dequantize_tensor, quantize_tensor
 from pare_b200.core.pack import pack_int4, unpack_int4
 from pare_b200.core.scale import compute_scale
 from pare_b200.kernels import matmul_int4 as _matmul
+from pare_b200.kernels.matmul_int8 import aligned_rows, w8a8_forward as _w8a8
 
 _FP8 = (QuantDtype.FP8_E4M3, QuantDtype.FP8_E5M2)
 
@@ -86,6 +91,7 @@ class QuantizedLinear(nn.Module):
         self.quantize_inputs = quantize_inputs
         self.use_kernel = use_kernel
         self.kernel_meta_fp16 = False
+        self.int8_kernel = False
 
     def _register_optional(self, g_idx: Tensor | None, input_scale: Tensor | None) -> None:
         self.register_buffer("g_idx", None if g_idx is None else g_idx.to(torch.int32))
@@ -113,6 +119,8 @@ class QuantizedLinear(nn.Module):
             and x.is_cuda
         ):
             return self._forward_kernel(x)
+        if self.int8_kernel and self.use_kernel and x.is_cuda:
+            return self._forward_int8(x)
 
         weight = self.dequantize().to(x.dtype)
         if self.input_scale is not None:
@@ -182,6 +190,30 @@ class QuantizedLinear(nn.Module):
         if y.dtype is not dtype:
             y = y.to(dtype)
         return y if flat else y.reshape(*shape[:-1], self.out_features)
+
+    def _forward_int8(self, x: Tensor) -> Tensor:
+        bufs, k, shape, dtype = self._buffers, self.in_features, x.shape, x.dtype
+        if "_q_weight_int8" not in bufs:
+            self._prepare_int8_buffers()
+        x2d = x if len(shape) == 2 else x.reshape(-1, shape[-1])
+        if dtype is not torch.float16 and dtype is not torch.bfloat16:
+            x2d = x2d.to(torch.float16)
+        y = _w8a8(x2d, bufs["_q_weight_int8"], bufs["_scale_int8"], bufs["_zero_int8"], bias=self.bias, input_scale=bufs["input_scale"])
+        if y.dtype is not dtype:
+            y = y.to(dtype)
+        return y if len(shape) == 2 else y.reshape(*shape[:-1], self.out_features)
+
+    def _prepare_int8_buffers(self) -> None:
+        """The derived, non-persistent tensors of the integer product (first call only)."""
+        n, scale, zero = self.out_features, self.scale, self.zero
+        if self.config.effective_dtype is not QuantDtype.INT8 or not self.quantize_inputs or self.g_idx is not None:
+            raise ValueError("int8_kernel needs an INT8 layer with quantize_inputs and without g_idx")
+        if scale.numel() not in (1, n) or zero.numel() not in (1, n):
+            raise ValueError("int8_kernel needs one scale per output channel or per tensor (granularity per_channel or per_tensor)")
+        zero = zero.reshape(-1).expand(n).contiguous()
+        self.register_buffer("_q_weight_int8", aligned_rows(self.q_weight), persistent=False)
+        self.register_buffer("_scale_int8", scale.reshape(-1).expand(n).contiguous(), persistent=False)
+        self.register_buffer("_zero_int8", zero if bool(zero.any()) else None, persistent=False)
 
     def supports_prepared(self, rows: int) -> bool:
         """True if :meth:`forward_prepared` can serve ``rows`` activation rows of this layer."""
