@@ -22,7 +22,7 @@ inline int max_items(int R, int T, int bs) {
 
 // A step: one buffer of 32-bit words, every array on a 16-byte boundary.
 struct StepLayout {
-  int64_t status, query_start, seq_lens, context_start, token_request, positions, slots, unit_start, items, words;
+  int64_t status, query_start, seq_lens, context_start, token_request, positions, slots, unit_start, info, items, words;
   int n_items;
   bool units;
   __host__ StepLayout(int R, int T, int bs) {
@@ -37,7 +37,8 @@ struct StepLayout {
     token_request = slots + up(2 * (int64_t)T);
     positions = token_request + up(T);
     unit_start = positions + up(T);
-    items = unit_start + up(units ? T + 1 : 0);
+    info = unit_start + up(units ? T + 1 : 0);     // [T] request, position, length after the step, 0
+    items = info + (units ? 4 * (int64_t)T : 0);
     words = items + (int64_t)n_items * kItemInts;
   }
 };

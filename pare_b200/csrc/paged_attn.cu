@@ -12,12 +12,11 @@
 // 2^kSlack (one vote per 16 tokens instead of a reduction); probabilities are kept times 2^kBias of that, so those down to 2^-18 of
 // the reference are normal fp16 numbers and none passes 2^15.  Their sum is taken before their rounding to fp16.
 //
-// Work.  Units of 16 tokens of one (token, group of heads), counted by the step's tables; each thread block takes one contiguous run
-// of units, all runs equally long, so ragged lengths balance by themselves and the host needs to know none of them.  Inside a run the
-// warps take units in turn; each warp feeds itself through a ring of its own (cp.async, no barrier between warps), and their
-// (maximum, sum, O) meet in shared memory at the end of a tile.  Tiles that span thread blocks leave their parts in the workspace for
-// a second kernel.  Nothing in the workspace outlives the call, no counters: calls on any streams and replays of any graphs do not
-// meet there.
+// Work.  Units of 16 tokens of one (token, group of heads), counted by the step's tables; each WARP takes one contiguous run of
+// units, all runs equally long, so ragged lengths balance by themselves and the host needs to know none of them.  A warp feeds
+// itself through a ring of its own (cp.async, no barrier between warps) and waits for nobody.  Tiles that span warps leave their
+// parts in the workspace for a second kernel.  Nothing in the workspace outlives the call, no counters: calls on any streams and
+// replays of any graphs do not meet there.
 #include <type_traits>
 
 #include "paged.cuh"
@@ -32,17 +31,16 @@ constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kBias = 4.f, kSlack = 11.f;
+constexpr int kMinRun = 4;                 // units of a warp's run at least
 
 template <int D>
 struct Shape {
   static constexpr int kStageBytes = 2 * kUnit * D;           // codes of 16 tokens: keys, then values
-  static constexpr int kStages = D == 128 ? 6 : 8;
+  static constexpr int kStages = D == 128 ? 3 : 6;
+  static constexpr int kChunks = kUnit * D / 512;             // 16-byte chunks of a unit's keys (or values) per lane
   static constexpr int kRing = kStages * kStageBytes;         // per warp
-  static constexpr int kPitch = D + 4;                        // floats per head of a warp's O at the end of a tile
-  static constexpr int kMergeFloats = kHeads * kPitch + 2 * kHeads;
-  static_assert(kMergeFloats * 4 <= kRing, "the ring holds a warp's result");
-  static constexpr size_t kSmem = (size_t)kWarps * (kRing + kStages * 8);
-  static constexpr int kPartFloats = kHeads * D + 2 * kHeads; // a part in the workspace: O, maxima, sums
+  static constexpr size_t kSmem = (size_t)kWarps * kRing;     // two thread blocks per SM
+  static constexpr int kPartFloats = kHeads * D + 2 * kHeads; // a part in the workspace: O as the lanes hold it, maxima, sums
 };
 
 struct PagedAttnParams {
@@ -50,10 +48,8 @@ struct PagedAttnParams {
   int64_t q_st, q_sh;
   void* out;
   int64_t o_st, o_sh;
-  const int* token_request;
-  const int* positions;
-  const int* seq_lens;
-  const int* unit_start;
+  const int4* info;          // [T] request, position, length after the step
+  const int* unit_start;     // [T + 1]
   const int* table;
   int64_t ld_table;
   const int8_t* k_codes;
@@ -62,7 +58,7 @@ struct PagedAttnParams {
   const float* v_scale;
   const void* tail_k;
   const void* tail_v;
-  float* parts;
+  float* parts;              // [warp][2]: of a tile that warps before it began, of one that it begins
   float scale_log2;
   int T, R, H, group, sub, bs_log2, num_blocks, max_blocks;   // sub: tiles of eight heads per KV head
 };
@@ -120,10 +116,10 @@ __device__ __forceinline__ float sum_over_g(float v) {
   return v;
 }
 
-// Units of a run per thread block: equal shares, but at least one unit per warp.
-__device__ __forceinline__ int64_t run_units(int64_t total, int blocks) {
-  const int64_t each = (total + blocks - 1) / blocks;
-  return each < kWarps ? kWarps : each;
+// Units of a run: equal shares, but not so few that the parts outweigh the work.
+__device__ __forceinline__ int64_t run_units(int64_t total, int warps) {
+  const int64_t each = (total + warps - 1) / warps;
+  return each < kMinRun ? kMinRun : each;
 }
 
 template <typename T, int D>
@@ -281,19 +277,24 @@ struct Tile {
     }
   }
 
-  // Up to 16 open tokens in 16 bits, from global memory (L2: a request's open rows are few).  Hidden rows are never loaded: what
-  // lies there (later tokens, leftovers) may be infinite.  bf16 probabilities have too few digits: value + what its rounding left.
-  __device__ __forceinline__ void open_unit(const T* k, const T* v, const T* q_row, float scale_log2, int seen, int lane) {
+  // Up to 16 open tokens in 16 bits: the keys in one stage of the ring, the values in another.  Hidden rows (later tokens,
+  // leftovers) were not loaded, they are zeros: what lies there may be infinite.  bf16 probabilities have too few digits: value +
+  // what its rounding left.
+  __device__ __forceinline__ void open_unit(uint32_t stage_k, uint32_t stage_v, const T* q_row, float scale_log2, int seen, int lane) {
     const int g = lane >> 2, t = lane & 3;
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < kJ; ++j) {
       uint4 a[2], b[2], q[2];
-      a[0] = a[1] = b[0] = b[1] = q[0] = q[1] = make_uint4(0, 0, 0, 0);
+      q[0] = q[1] = make_uint4(0, 0, 0, 0);
       const int c = 16 * (t + 4 * j);
-      if (g < seen) a[0] = *reinterpret_cast<const uint4*>(k + g * D + c), a[1] = *reinterpret_cast<const uint4*>(k + g * D + c + 8);
-      if (g + 8 < seen) b[0] = *reinterpret_cast<const uint4*>(k + (g + 8) * D + c), b[1] = *reinterpret_cast<const uint4*>(k + (g + 8) * D + c + 8);
       if (q_row) q[0] = *reinterpret_cast<const uint4*>(q_row + c), q[1] = *reinterpret_cast<const uint4*>(q_row + c + 8);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t at = stage_k + (((c / 8 + e) ^ (g & 1)) << 4);
+        a[e] = lds128(at + g * 2 * D);
+        b[e] = lds128(at + (g + 8) * 2 * D);
+      }
       const uint32_t* wa = reinterpret_cast<const uint32_t*>(a);
       const uint32_t* wb = reinterpret_cast<const uint32_t*>(b);
       const uint32_t* wq = reinterpret_cast<const uint32_t*>(q);
@@ -323,10 +324,7 @@ struct Tile {
     for (int c = 0; c < kW / 2; ++c) {   // eight channels at a time
       uint4 x[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int row = 2 * t + (e & 1) + (e >> 1) * 8;
-        x[e] = row < seen ? *reinterpret_cast<const uint4*>(v + row * D + (D / 8) * g + 8 * c) : make_uint4(0, 0, 0, 0);
-      }
+      for (int e = 0; e < 4; ++e) x[e] = lds128(stage_v + (2 * t + (e & 1) + (e >> 1) * 8) * 2 * D + ((((D / 64) * g + c) ^ open_value_swizzle(t)) << 4));
       const uint32_t* a = reinterpret_cast<const uint32_t*>(&x[0]);
       const uint32_t* b = reinterpret_cast<const uint32_t*>(&x[1]);
       const uint32_t* d = reinterpret_cast<const uint32_t*>(&x[2]);
@@ -340,85 +338,105 @@ struct Tile {
       }
     }
   }
+
+  // 16-byte chunks of a row of open values are moved by this (t: half the row's number modulo 4), so that the eight lanes of a
+  // shared-memory phase (two g, four t) meet eight different banks
+  __device__ static __forceinline__ int open_value_swizzle(int t) { return D == 128 ? (t & 1) | ((t >> 1) << 2) : 2 * t; }
 };
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const PagedAttnParams p) {
+__global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttnParams p) {
   using S = Shape<D>;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ int s_t;
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   const int tiles = p.H * p.sub;       // tiles of eight heads per token
+  const int me = blockIdx.x * kWarps + warp;
   pdl_wait();
-  const int64_t total = (int64_t)p.unit_start[p.T] * tiles, run = run_units(total, gridDim.x);
-  const int64_t u0 = blockIdx.x * run, u1 = min(u0 + run, total);
+  const int64_t total = (int64_t)p.unit_start[p.T] * tiles, run = run_units(total, gridDim.x * kWarps);
+  const int64_t u0 = me * run, u1 = min(u0 + run, total);
   if (u0 >= u1) return;
-  for (int i = threadIdx.x; i < p.T; i += kThreads) {
-    const int64_t a = (int64_t)p.unit_start[i] * tiles, b = (int64_t)p.unit_start[i + 1] * tiles;
-    if (a <= u0 && u0 < b) s_t = i;
+  int t = 0;       // the last token that begins at or before u0: 32 candidates a round
+  {
+    const int x = (int)(u0 / tiles);
+    for (int n = p.T; n > 1;) {
+      const int step = (n + 31) / 32, at = lane * step;
+      const uint32_t yes = __ballot_sync(0xffffffffu, at < n && p.unit_start[t + min(at, n - 1)] <= x);
+      const int k = 31 - __clz(yes);
+      t += k * step;
+      n = min(step, n - k * step);
+    }
   }
-  __syncthreads();
-  int t = s_t;
 
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem + warp * S::kRing);
-  float* s_scale = reinterpret_cast<float*>(smem + kWarps * S::kRing) + warp * S::kStages * 2;
-  float* mine = reinterpret_cast<float*>(smem + warp * S::kRing);
   Tile<T, D> tile;
 
-  int units = p.unit_start[t + 1] - p.unit_start[t];
-  const int64_t base = (int64_t)p.unit_start[t] * tiles;
+  // where this lane's 16-byte chunks of a unit go in a stage (chunk e * 32 + lane of the keys and of the values)
+  uint32_t at_k[S::kChunks], at_v[S::kChunks];
+#pragma unroll
+  for (int e = 0; e < S::kChunks; ++e) {
+    const int row = (e * 32 + lane) / (D / 16), c = (e * 32 + lane) % (D / 16);
+    at_k[e] = row * D + (D == 128 ? c ^ ((row & 1) << 2) : c) * 16;
+    at_v[e] = kUnit * D + row * D + (D == 128 ? c ^ (((row >> 1) & 3) << 1) : c ^ ((row >> 1) & 3)) * 16;
+  }
+
+  int first_unit = p.unit_start[t], units = p.unit_start[t + 1] - first_unit;
+  int4 info = p.info[t];
+  const int64_t base = (int64_t)first_unit * tiles;
   int h = (int)((u0 - base) / units), j0 = (int)(u0 - base - (int64_t)h * units);
   for (int64_t u = u0; u < u1;) {
     const int n = (int)min((int64_t)(units - j0), u1 - u);    // units j0 .. j0 + n - 1 of tile (t, h)
-    const int r = p.token_request[t], pos = p.positions[t], end = p.seq_lens[r];
+    const int r = info.x, pos = info.y, end = info.z;
     const int held = end >> p.bs_log2 << p.bs_log2, nq = min(pos + 1, held), nq_units = (nq + kUnit - 1) / kUnit;
     const int hk = h / p.sub, head0 = hk * p.group + (h - hk * p.sub) * kHeads, heads = min(kHeads, (hk + 1) * p.group - head0);
     const T* q_row = g < heads ? reinterpret_cast<const T*>(p.q) + t * p.q_st + (head0 + g) * p.q_sh : nullptr;
     const int* row_table = p.table + r * p.ld_table;
-    const int mine_n = n > warp ? (n - warp + kWarps - 1) / kWarps : 0;   // this warp's units: j0 + warp + i * kWarps
+    const int n8 = max(0, min(n, nq_units - j0));             // units in 8 bits, then units of open rows: two entries of the ring each
+    const int entries = n8 + 2 * (n - n8);
 
-    // block ids and scales of 32 of this warp's units at a time, one per lane
-    int ids = -1;
-    float kss = 0.f, vss = 0.f;
+    // Block ids and scales of 32 units at a time, one unit per lane.  Loads run ahead by the depth of the ring, so the scales of
+    // the next 32 wait in registers of their own.
+    int ids = -1, slot_in = 0;
+    float ks_next = 0.f, vs_next = 0.f, kss = 0.f, vss = 0.f;
     auto issue = [&](int i) {
-      if (i < mine_n) {
+      if (i < n8) {
         if ((i & 31) == 0) {
-          const int j = j0 + warp + (i + lane) * kWarps;
           ids = -1;
-          kss = vss = __int_as_float(0x7fffffff);               // a block that is not in the pool: NaN
-          if (i + lane < mine_n && j < nq_units) {
-            const int blk = j * kUnit >> p.bs_log2;
+          ks_next = vs_next = __int_as_float(0x7fffffff);       // a block that is not in the pool: NaN
+          if (i + lane < n8) {
+            const int blk = (j0 + i + lane) * kUnit >> p.bs_log2;
             ids = blk < p.max_blocks ? row_table[blk] : -1;
-            if (ids >= 0 && ids < p.num_blocks) {
-              kss = p.k_scale[(int64_t)ids * p.H + hk];
-              vss = p.v_scale[(int64_t)ids * p.H + hk];
-            } else {
-              ids = -1;
-            }
+            if (ids < 0 || ids >= p.num_blocks) ids = -1;
+          }
+          if (ids >= 0) {
+            ks_next = p.k_scale[(int64_t)ids * p.H + hk];
+            vs_next = p.v_scale[(int64_t)ids * p.H + hk];
           }
         }
-        const int j = j0 + warp + i * kWarps, id = __shfl_sync(0xffffffffu, ids, i & 31);
-        const float ks = __shfl_sync(0xffffffffu, kss, i & 31), vs = __shfl_sync(0xffffffffu, vss, i & 31);
-        if (j < nq_units) {
-          const int slot = i % S::kStages;
-          const uint32_t dst = ring + slot * S::kStageBytes;
-          const int64_t src = id < 0 ? 0 : (((int64_t)id * p.H + hk) << p.bs_log2) * D + ((j * kUnit) & ((1 << p.bs_log2) - 1)) * D;
-          const int bytes = id < 0 ? 0 : 16;
+        const int id = __shfl_sync(0xffffffffu, ids, i & 31);
+        const uint32_t dst = ring + slot_in * S::kStageBytes;
+        const int64_t src = id < 0 ? 0 : ((((int64_t)id * p.H + hk) << p.bs_log2) + (((j0 + i) * kUnit) & ((1 << p.bs_log2) - 1))) * D;
+        const int bytes = id < 0 ? 0 : 16;
+        const int8_t* sk = p.k_codes + src + lane * 16;
+        const int8_t* sv = p.v_codes + src + lane * 16;
 #pragma unroll
-          for (int e = 0; e < kUnit * D / 512; ++e) {
-            const int at = e * 32 + lane;          // 16-byte chunk of the piece
-            const int row = at / (D / 16), c = at % (D / 16);
-            const int ck = D == 128 ? c ^ ((row & 1) << 2) : c, cv = D == 128 ? c ^ (((row >> 1) & 3) << 1) : c ^ ((row >> 1) & 3);
-            cp_async16(dst + row * D + ck * 16, p.k_codes + src + at * 16, bytes);
-            cp_async16(dst + kUnit * D + row * D + cv * 16, p.v_codes + src + at * 16, bytes);
-          }
-          if (lane == 0) {
-            s_scale[2 * slot] = ks;
-            s_scale[2 * slot + 1] = vs;
-          }
+        for (int e = 0; e < S::kChunks; ++e) cp_async16(dst + at_k[e], sk + e * 512, bytes);
+#pragma unroll
+        for (int e = 0; e < S::kChunks; ++e) cp_async16(dst + at_v[e], sv + e * 512, bytes);
+      } else if (i < entries) {
+        const int from = (j0 + n8 - nq_units + (i - n8) / 2) * kUnit, seen = pos + 1 - nq - from;   // first row, visible rows
+        const bool values = (i - n8) & 1;
+        const T* src = reinterpret_cast<const T*>(values ? p.tail_v : p.tail_k) + ((((int64_t)r * p.H + hk) << p.bs_log2) + from) * D;
+        const uint32_t dst = ring + slot_in * S::kStageBytes;
+#pragma unroll 1
+        for (int e = 0; e < 2 * S::kChunks; ++e) {
+          const int row = (e * 32 + lane) / (D / 8), c = (e * 32 + lane) % (D / 8);
+          const int to = c ^ (values ? Tile<T, D>::open_value_swizzle((row >> 1) & 3) : row & 1);
+          const bool there = row < seen;
+          cp_async16(dst + row * 2 * D + to * 16, there ? src + row * D + c * 8 : src, there ? 16 : 0);
         }
       }
+      if (++slot_in == S::kStages) slot_in = 0;
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
 
@@ -426,122 +444,135 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const PagedAttn
 #pragma unroll 1
     for (int i = 0; i < S::kStages - 1; ++i) issue(i);
     tile.load_q(q_row, p.scale_log2, lane);
+    int slot = 0;
 #pragma unroll 1
-    for (int i = 0; i < mine_n; ++i) {
-      const int j = j0 + warp + i * kWarps;
+    for (int i = 0; i < n8; ++i) {
+      if ((i & 31) == 0) kss = ks_next, vss = vs_next;
+      const float ks = __shfl_sync(0xffffffffu, kss, i & 31), vs = __shfl_sync(0xffffffffu, vss, i & 31);
       asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
       __syncwarp();
-      if (j < nq_units) {
-        const int slot = i % S::kStages;
-        const float ks = s_scale[2 * slot], vs = s_scale[2 * slot + 1];
-        tile.quantized_unit(ring + slot * S::kStageBytes, ks, vs, nq - j * kUnit, lane);
-      } else {
-        const int from = (j - nq_units) * kUnit;
-        const int64_t at = ((((int64_t)r * p.H + hk) << p.bs_log2) + from) * D;
-        tile.open_unit(reinterpret_cast<const T*>(p.tail_k) + at, reinterpret_cast<const T*>(p.tail_v) + at, q_row, p.scale_log2,
-                       pos + 1 - nq - from, lane);
-      }
+      tile.quantized_unit(ring + slot * S::kStageBytes, ks, vs, nq - (j0 + i) * kUnit, lane);
+      if (++slot == S::kStages) slot = 0;
       __syncwarp();
       issue(i + S::kStages - 1);
+    }
+#pragma unroll 1
+    for (int i = n8; i < entries; i += 2) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 3) : "memory");
+      __syncwarp();
+      const int next = slot + 1 == S::kStages ? 0 : slot + 1;
+      tile.open_unit(ring + slot * S::kStageBytes, ring + next * S::kStageBytes, q_row, p.scale_log2,
+                     pos + 1 - nq - (j0 + n8 - nq_units + (i - n8) / 2) * kUnit, lane);
+      slot = next + 1 == S::kStages ? 0 : next + 1;
+      __syncwarp();
+      issue(i + S::kStages - 1);
+      issue(i + S::kStages);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncwarp();
 
-    // ---- the warps' results meet: [8 heads][D + 4], maxima, sums per warp, over its ring ----
     const float l0 = sum_over_g(tile.l0), l1 = sum_over_g(tile.l1);
-    if (g == 0) {
-      mine[kHeads * S::kPitch + 2 * t4] = tile.m0;
-      mine[kHeads * S::kPitch + 2 * t4 + 1] = tile.m1;
-      mine[kHeads * S::kPitch + kHeads + 2 * t4] = l0;
-      mine[kHeads * S::kPitch + kHeads + 2 * t4 + 1] = l1;
-    }
+    if (n == units) {
+      const float y0 = 1.f / l0, y1 = 1.f / l1;
+      T* out = reinterpret_cast<T*>(p.out) + t * p.o_st + (int64_t)(head0 + 2 * t4) * p.o_sh;
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      const int c = (D / 8) * g + 2 * i;
-      *reinterpret_cast<float2*>(mine + (2 * t4) * S::kPitch + c) = make_float2(tile.o[i][0], tile.o[i][2]);
-      *reinterpret_cast<float2*>(mine + (2 * t4 + 1) * S::kPitch + c) = make_float2(tile.o[i][1], tile.o[i][3]);
-    }
-    __syncthreads();
-    {
-      const int head = warp;   // eight warps, eight heads
-      const float* all = reinterpret_cast<const float*>(smem);
-      constexpr int kStep = S::kRing / 4;
-      const int live = min(n, kWarps);
-      float top = -INFINITY, sum = 0.f, x[D / 32];
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) x[c] = 0.f;
-      for (int w = 0; w < live; ++w) top = fmaxf(top, all[w * kStep + kHeads * S::kPitch + head]);
-      for (int w = 0; w < live; ++w) {
-        const float m = all[w * kStep + kHeads * S::kPitch + head];
-        const float f = m == top ? 1.f : ex2(m - top);
-        sum = fmaf(f, all[w * kStep + kHeads * S::kPitch + kHeads + head], sum);
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) x[c] = fmaf(f, all[w * kStep + head * S::kPitch + 32 * c + lane], x[c]);
+      for (int i = 0; i < D / 16; ++i) {
+        const int c = (D / 8) * g + 2 * i;
+        if (2 * t4 < heads) out[c] = from_float<T>(tile.o[i][0] * y0), out[c + 1] = from_float<T>(tile.o[i][2] * y0);
+        if (2 * t4 + 1 < heads) out[p.o_sh + c] = from_float<T>(tile.o[i][1] * y1), out[p.o_sh + c + 1] = from_float<T>(tile.o[i][3] * y1);
       }
-      if (n == units) {
-        if (head < heads) {
-          T* out = reinterpret_cast<T*>(p.out) + t * p.o_st + (head0 + head) * p.o_sh;
+    } else {
+      float* part = p.parts + ((int64_t)me * 2 + (j0 == 0 ? 1 : 0)) * S::kPartFloats;
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c) out[32 * c + lane] = from_float<T>(x[c] / sum);
-        }
-      } else {   // slot 0: a tile that thread blocks before this one began; slot 1: one that this one begins
-        float* part = p.parts + ((int64_t)blockIdx.x * 2 + (j0 == 0 ? 1 : 0)) * S::kPartFloats;
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) part[head * D + 32 * c + lane] = x[c];
-        if (lane == 0) {
-          part[kHeads * D + head] = top;
-          part[kHeads * D + kHeads + head] = sum;
-        }
+      for (int i = 0; i < D / 16; ++i)
+        reinterpret_cast<float4*>(part)[i * 32 + lane] = make_float4(tile.o[i][0], tile.o[i][1], tile.o[i][2], tile.o[i][3]);
+      if (g == 0) {
+        *reinterpret_cast<float2*>(part + kHeads * D + 2 * t4) = make_float2(tile.m0, tile.m1);
+        *reinterpret_cast<float2*>(part + kHeads * D + kHeads + 2 * t4) = make_float2(l0, l1);
       }
     }
-    __syncthreads();
     u += n;
     j0 = 0;
     if (++h == tiles && u < u1) {
       h = 0;
       do {
         ++t;
-        units = p.unit_start[t + 1] - p.unit_start[t];
+        first_unit += units;
+        units = p.unit_start[t + 1] - first_unit;
       } while (units == 0);
+      info = p.info[t];
     }
   }
 }
 
-// Tiles that span thread blocks: their parts, in order.  One thread block per tile, one warp per head.
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) paged_merge_kernel(const PagedAttnParams p, int blocks) {
+// Tiles that span warps.  A warp takes one piece of a tile's O (float4 per lane as the attention's lanes held it: channels
+// (D / 8) g + 2 i, + 1 x heads 2 t, 2 t + 1).  Many tiles have few parts each: a thread block per tile, a warp
+// per piece.  Few tiles have many (one sequence: 64): GROUPS warps share a piece, each every GROUPS-th part, and are added up in order.
+constexpr int kMergeGroups = 8;
+
+template <typename T, int D, int GROUPS>
+__global__ void __launch_bounds__(GROUPS > 1 ? GROUPS * 32 : D * 2) paged_merge_kernel(const PagedAttnParams p, int warps) {
   using S = Shape<D>;
+  constexpr int kFlight = 4;     // parts in flight per warp
+  __shared__ float4 s_o[GROUPS][32], s_ml[GROUPS][32];
   pdl_wait();
-  const int tiles = p.H * p.sub, t = blockIdx.x / tiles, h = blockIdx.x - t * tiles;
-  const int64_t total = (int64_t)p.unit_start[p.T] * tiles, run = run_units(total, blocks);
-  const int units = p.unit_start[t + 1] - p.unit_start[t];
-  const int64_t a = (int64_t)p.unit_start[t] * tiles + (int64_t)h * units;
-  const int first = (int)(a / run), last = units ? (int)((a + units - 1) / run) : first;
-  if (first == last) return;
-  const int head = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int hk = h / p.sub, head0 = hk * p.group + (h - hk * p.sub) * kHeads, heads = min(kHeads, (hk + 1) * p.group - head0);
-  if (head >= heads) return;
-  auto part_of = [&](int b) { return p.parts + ((int64_t)b * 2 + (b == first ? 1 : 0)) * S::kPartFloats; };
-  float top = -INFINITY;
-  for (int b = first + lane; b <= last; b += 32) top = fmaxf(top, part_of(b)[kHeads * D + head]);
-  top = warp_max(top);
-  float sum = 0.f, x[D / 32];
+  const int tiles = p.H * p.sub, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+  const int group = GROUPS > 1 ? warp : 0, piece = GROUPS > 1 ? blockIdx.y : warp;
+  const int64_t total = (int64_t)p.unit_start[p.T] * tiles, run = run_units(total, warps);
+  auto run_of = [&](int64_t u) { return total >> 32 ? (int)(u / run) : (int)((uint32_t)u / (uint32_t)run); };
+  for (int job = blockIdx.x; job < p.T * tiles; job += gridDim.x) {
+    const int t = job / tiles, h = job - t * tiles;
+    const int first_unit = p.unit_start[t], units = p.unit_start[t + 1] - first_unit;
+    const int64_t a = (int64_t)first_unit * tiles + (int64_t)h * units;
+    const int first = run_of(a), last = units ? run_of(a + units - 1) : first;
+    if (first == last) continue;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float2 top = make_float2(-INFINITY, -INFINITY), l = make_float2(0.f, 0.f);
+    auto add = [&](const float2& m, const float2& s, const float4& x) {
+      const float n0 = fmaxf(top.x, m.x), n1 = fmaxf(top.y, m.y);
+      const float a0 = n0 == top.x ? 1.f : ex2(top.x - n0), a1 = n1 == top.y ? 1.f : ex2(top.y - n1);
+      const float f0 = n0 == m.x ? 1.f : ex2(m.x - n0), f1 = n1 == m.y ? 1.f : ex2(m.y - n1);
+      top = make_float2(n0, n1);
+      l = make_float2(fmaf(a0, l.x, f0 * s.x), fmaf(a1, l.y, f1 * s.y));
+      o = make_float4(fmaf(a0, o.x, f0 * x.x), fmaf(a1, o.y, f1 * x.y), fmaf(a0, o.z, f0 * x.z), fmaf(a1, o.w, f1 * x.w));
+    };
+    for (int b = first + group; b <= last; b += GROUPS * kFlight) {
+      float2 m[kFlight], s[kFlight];
+      float4 x[kFlight];
 #pragma unroll
-  for (int c = 0; c < D / 32; ++c) x[c] = 0.f;
-#pragma unroll 4
-  for (int b = first; b <= last; ++b) {
-    const float* part = part_of(b);
-    const float m = part[kHeads * D + head], f = m == top ? 1.f : ex2(m - top);
-    sum = fmaf(f, part[kHeads * D + kHeads + head], sum);
+      for (int i = 0; i < kFlight; ++i) {
+        const int at = b + i * GROUPS;
+        const float* part = p.parts + ((int64_t)at * 2 + (at == first ? 1 : 0)) * S::kPartFloats;
+        if (at <= last) {
+          m[i] = *reinterpret_cast<const float2*>(part + kHeads * D + 2 * t4);
+          s[i] = *reinterpret_cast<const float2*>(part + kHeads * D + kHeads + 2 * t4);
+          x[i] = reinterpret_cast<const float4*>(part)[piece * 32 + lane];
+        }
+      }
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c) x[c] = fmaf(f, part[head * D + 32 * c + lane], x[c]);
+      for (int i = 0; i < kFlight; ++i)
+        if (b + i * GROUPS <= last) add(m[i], s[i], x[i]);
+    }
+    if (GROUPS > 1) {
+      __syncthreads();     // the tile before has been read
+      s_o[group][lane] = o;
+      s_ml[group][lane] = make_float4(top.x, top.y, l.x, l.y);
+      __syncthreads();
+      if (group) continue;
+#pragma unroll
+      for (int w = 1; w < GROUPS; ++w) {
+        const float4 ml = s_ml[w][lane];
+        if (first + w <= last) add(make_float2(ml.x, ml.y), make_float2(ml.z, ml.w), s_o[w][lane]);
+      }
+    }
+    const int hk = h / p.sub, head0 = hk * p.group + (h - hk * p.sub) * kHeads, heads = min(kHeads, (hk + 1) * p.group - head0);
+    T* out = reinterpret_cast<T*>(p.out) + t * p.o_st + (int64_t)(head0 + 2 * t4) * p.o_sh + (D / 8) * g + 2 * piece;
+    if (2 * t4 < heads) out[0] = from_float<T>(o.x / l.x), out[1] = from_float<T>(o.z / l.x);
+    if (2 * t4 + 1 < heads) out[p.o_sh] = from_float<T>(o.y / l.y), out[p.o_sh + 1] = from_float<T>(o.w / l.y);
   }
-  T* out = reinterpret_cast<T*>(p.out) + t * p.o_st + (head0 + head) * p.o_sh;
-#pragma unroll
-  for (int c = 0; c < D / 32; ++c) out[32 * c + lane] = from_float<T>(x[c] / sum);
 }
 
-int attn_blocks() { return sm_count(); }
+int attn_blocks() { return 2 * sm_count(); }
 
 }  // namespace
 }  // namespace pare
@@ -553,7 +584,7 @@ using namespace pare::paged;
 
 size_t pare_paged_attn_workspace_bytes(int D) {
   if (D != 64 && D != 128) return 0;
-  return (size_t)attn_blocks() * 2 * (kHeads * D + 2 * kHeads) * sizeof(float);
+  return (size_t)attn_blocks() * kWarps * 2 * (kHeads * D + 2 * kHeads) * sizeof(float);
 }
 
 int pare_paged_attn(const void* q, int dtype, int64_t q_stride_t, int64_t q_stride_h, const void* step, int R, int T, int block_size,
@@ -577,24 +608,27 @@ int pare_paged_attn(const void* q, int dtype, int64_t q_stride_t, int64_t q_stri
   PARE_REQUIRE((int64_t)T * H * sub < (int64_t)1 << 31, PARE_ERR_UNSUPPORTED);
   const StepLayout s(R, T, block_size);
   const int* w = reinterpret_cast<const int*>(step);
-  PagedAttnParams p{q, q_stride_t, q_stride_h, out, out_stride_t, out_stride_h, w + s.token_request, w + s.positions, w + s.seq_lens,
+  const int blocks = attn_blocks();
+  PagedAttnParams p{q, q_stride_t, q_stride_h, out, out_stride_t, out_stride_h, reinterpret_cast<const int4*>(w + s.info),
                     w + s.unit_start, block_table, ld_table, k_codes, v_codes, k_scale, v_scale, tail_k, tail_v,
                     reinterpret_cast<float*>(workspace), softmax_scale * kLog2e, T, R, H, group, sub,
                     block_size == 16 ? 4 : block_size == 32 ? 5 : 6, num_blocks, max_blocks};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const int blocks = attn_blocks();
-  auto go = [&](auto kern, auto merge, size_t smem) {
+  auto go = [&](auto kern, auto merge, auto merge_few, size_t smem) {
     if (!ensure_smem_attr(reinterpret_cast<const void*>(kern), (int)smem)) return (int)PARE_ERR_CUDA;
     int rc = launch_pdl(kern, dim3(blocks), dim3(kThreads), smem, st, p);
     if (rc != PARE_OK) return rc;
-    rc = launch_pdl(merge, dim3(T * H * sub), dim3(kThreads), 0, st, p, blocks);
+    const int jobs = T * H * sub, most = 32 * sm_count();
+    rc = jobs <= sm_count() ? launch_pdl(merge_few, dim3(jobs, D / 16), dim3(kMergeGroups * 32), 0, st, p, blocks * kWarps)
+                            : launch_pdl(merge, dim3(jobs < most ? jobs : most), dim3(D * 2), 0, st, p, blocks * kWarps);
     return rc != PARE_OK ? rc : launch_status();
   };
-  if (dtype == PARE_F16)
-    return D == 64 ? go(paged_attn_kernel<__half, 64>, paged_merge_kernel<__half, 64>, Shape<64>::kSmem)
-                   : go(paged_attn_kernel<__half, 128>, paged_merge_kernel<__half, 128>, Shape<128>::kSmem);
-  return D == 64 ? go(paged_attn_kernel<__nv_bfloat16, 64>, paged_merge_kernel<__nv_bfloat16, 64>, Shape<64>::kSmem)
-                 : go(paged_attn_kernel<__nv_bfloat16, 128>, paged_merge_kernel<__nv_bfloat16, 128>, Shape<128>::kSmem);
+  auto by_dim = [&](auto tag) {
+    using E = decltype(tag);
+    return D == 64 ? go(paged_attn_kernel<E, 64>, paged_merge_kernel<E, 64, 1>, paged_merge_kernel<E, 64, kMergeGroups>, Shape<64>::kSmem)
+                   : go(paged_attn_kernel<E, 128>, paged_merge_kernel<E, 128, 1>, paged_merge_kernel<E, 128, kMergeGroups>, Shape<128>::kSmem);
+  };
+  return dtype == PARE_F16 ? by_dim(__half()) : by_dim(__nv_bfloat16());
 }
 
 }  // extern "C"

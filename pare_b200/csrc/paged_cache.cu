@@ -30,7 +30,7 @@ struct PlanParams {
   const int* free_blocks;
   const int* free_count;
   int* step;
-  int64_t o_query_start, o_seq_lens, o_context, o_slots, o_request, o_positions, o_units, o_items;
+  int64_t o_query_start, o_seq_lens, o_context, o_slots, o_request, o_positions, o_units, o_info, o_items;
   int R, T, bs_log2, max_blocks, free_capacity, n_items, units;
 };
 
@@ -155,6 +155,10 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
       r = last_at_most(s_start, R, i);
       pos = s_len[r] + i - s_start[r];
       slot = ((long long)block_id(r, pos >> p.bs_log2) << p.bs_log2) + (pos & (bs - 1));
+    }
+    if (p.units) {
+      const int end = r < 0 ? 0 : s_len[r] + (r + 1 < R ? s_start[r + 1] : (int)t_new) - s_start[r];
+      *reinterpret_cast<int4*>(p.step + p.o_info + 4 * (int64_t)i) = make_int4(r, pos, end, 0);
     }
     p.step[p.o_request + i] = r;
     p.step[p.o_positions + i] = pos;
@@ -429,7 +433,7 @@ int pare_paged_plan(const int32_t* seq_lens, const int32_t* new_lens, int R, int
   PARE_REQUIRE(step_bytes >= (size_t)s.words * 4, PARE_ERR_WORKSPACE);
   PARE_REQUIRE(aligned16(step), PARE_ERR_ALIGN);
   PlanParams p{seq_lens, new_lens, block_table, ld_table, free_blocks, free_count, reinterpret_cast<int*>(step),
-               s.query_start, s.seq_lens, s.context_start, s.slots, s.token_request, s.positions, s.unit_start, s.items,
+               s.query_start, s.seq_lens, s.context_start, s.slots, s.token_request, s.positions, s.unit_start, s.info, s.items,
                R, T, log2_of(block_size), max_blocks, free_capacity, s.n_items, s.units ? 1 : 0};
   const size_t smem = (size_t)R * 4 * sizeof(int);
   if (!ensure_smem_attr(reinterpret_cast<const void*>(paged_plan_kernel), kMaxRequests * 4 * (int)sizeof(int))) return PARE_ERR_CUDA;
