@@ -8,6 +8,7 @@
 // rounding and tokens fed in pieces give what the same tokens fed at once give (the property of the reference's residual window,
 // pare/kv_cache.py:231-244).
 #include "paged.cuh"
+#include "quant8.cuh"
 
 namespace pare {
 namespace {
@@ -245,15 +246,6 @@ struct AppendParams {
   int H, num_blocks, R, T;
 };
 
-// Code of x on the grid of step s, as fp32 round(x / s): the product with 1 / s decides except next to a border between two codes
-// (within 1e-4; its own error is below 2e-5), where the quotient does.
-__device__ __forceinline__ int code_of(float x, float s, float inv, bool exact) {
-  float t = x * inv;
-  float c = rintf(t);
-  if (exact || fabsf(t - c) > 0.4999f) c = rintf(__fdiv_rn(x, s));
-  return (int)fminf(fmaxf(c, -127.f), 127.f);
-}
-
 template <typename T, int D, int BS>
 __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const AppendParams p) {
   pdl_launch_dependents();
@@ -286,8 +278,7 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
   for (int i = 0; i < kEach; ++i) {
     const int at = i * kHalf + tid, t = at / kChunks, c = at % kChunks * 8;
     x[i] = t < off ? *reinterpret_cast<const uint4*>(tail + t * D + c) : *reinterpret_cast<const uint4*>(src + (row0 + t - off) * st + c);
-    // magnitudes of 16-bit floats order like their bits, infinities and NaN above all numbers
-    top = __vmaxu2(top, __vmaxu2(__vmaxu2(x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu), __vmaxu2(x[i].z & 0x7fff7fffu, x[i].w & 0x7fff7fffu)));
+    top = __vmaxu2(top, q8::magnitudes(x[i]));
   }
   top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
   if ((threadIdx.x & 31) == 0) s_max[half][tid / 32] = top;
@@ -295,25 +286,12 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
 #pragma unroll
   for (int w = 0; w < kHalf / 32; ++w) top = max(top, s_max[half][w]);
   const uint16_t bits = (uint16_t)top;
-  const float amax = to_float<T>(*reinterpret_cast<const T*>(&bits)), s = __fdiv_rn(amax, 127.f);
-  const bool finite = s > 0.f && s < INFINITY, exact = s < 1e-30f;    // below that 1 / s may overflow
-  const float inv = finite && !exact ? __fdiv_rn(1.f, s) : 0.f;
+  const q8::Grid grid(to_float<T>(*reinterpret_cast<const T*>(&bits)));
   if (id >= 0 && id < p.num_blocks) {
     int8_t* codes = (half ? p.v_codes : p.k_codes) + ((int64_t)id * p.H + h) * BS * D;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int at = i * kHalf + tid;
-      const T* e = reinterpret_cast<const T*>(&x[i]);
-      uint32_t w[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        w[j] = 0;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) w[j] |= (finite ? (uint32_t)code_of(to_float<T>(e[4 * j + q]), s, inv, exact) & 0xffu : 0u) << (8 * q);
-      }
-      *reinterpret_cast<uint2*>(codes + at * 8) = make_uint2(w[0], w[1]);
-    }
-    if (tid == 0) (half ? p.v_scale : p.k_scale)[(int64_t)id * p.H + h] = s;
+    for (int i = 0; i < kEach; ++i) *reinterpret_cast<uint2*>(codes + (i * kHalf + tid) * 8) = grid.codes<T>(x[i]);
+    if (tid == 0) (half ? p.v_scale : p.k_scale)[(int64_t)id * p.H + h] = grid.step;
   }
   if (off > 0 && end % BS != 0 && end / BS > blk) {   // the open block behind it: its rows are free only now
     asm volatile("bar.sync %0, %1;" ::"r"(1 + half), "n"(kHalf) : "memory");

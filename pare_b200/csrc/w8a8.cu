@@ -15,6 +15,7 @@
 //   warp 0     TMA of both operands      warp 1  tcgen05.mma      warp 2  tensor memory      warps 4-7  epilogue
 // All waits are bounded; when one runs out the thread block stops waiting and loading, lets its copies and products in flight
 // end, and its outputs become NaN.
+#include "quant8.cuh"
 #include "tcgen05.cuh"
 
 namespace pare {
@@ -33,8 +34,6 @@ constexpr int kRingBytes = kMaxSmem - 1024 - 512;
 constexpr int kMaxK = 65536;             // 65536 * 127 * (128 + 128) < 2^31
 
 // ---- tokens -> codes ----------------------------------------------------------------------------------------------------------------
-constexpr int kQuantThreads = 256;
-
 struct QuantParams {
   const void* x;
   int64_t ldx;
@@ -56,26 +55,43 @@ __device__ __forceinline__ uint32_t magnitude(T v) {   // orders like |v|, infin
   return *reinterpret_cast<const uint16_t*>(&v) & 0x7fffu;
 }
 
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kQuantThreads) w8a8_quantize_kernel(const QuantParams p) {
+// VECS > 0: rows of at most VECS * THREADS vectors of eight stay in registers between the maximum and the codes (and are divided by
+// input_scale once); 0: rows of any length and alignment, read twice.
+template <typename T, int THREADS, int VECS>
+__global__ void __launch_bounds__(THREADS) w8a8_quantize_kernel(const QuantParams p) {
   pdl_launch_dependents();
-  constexpr int kW = kQuantThreads / 32;
+  constexpr int kW = THREADS / 32;
   __shared__ uint32_t s_top[kW];
   __shared__ int s_sum[kW];
   const int m = blockIdx.x, tid = threadIdx.x;
   const T* row = reinterpret_cast<const T*>(p.x) + m * p.ldx;
   int8_t* out = p.codes + m * p.ldc;
-  for (int i = m * kQuantThreads + tid; i < p.n_zeroed; i += gridDim.x * kQuantThreads) p.zeroed[i] = 0;
+  for (int i = m * THREADS + tid; i < p.n_zeroed; i += gridDim.x * THREADS) p.zeroed[i] = 0;
   uint32_t top = 0;
-  if (VEC) {
-    for (int k = tid * 8; k < p.K; k += kQuantThreads * 8) {
-      const uint4 w = *reinterpret_cast<const uint4*>(row + k);
-      const T* v = reinterpret_cast<const T*>(&w);
+  uint4 x[VECS > 0 ? VECS : 1];
+  if constexpr (VECS > 0) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) top = max(top, magnitude(smoothed<T>(v[j], p.input_scale, k + j)));
+    for (int i = 0; i < VECS; ++i) {
+      const int k = (i * THREADS + tid) * 8;
+      x[i] = k < p.K ? *reinterpret_cast<const uint4*>(row + k) : make_uint4(0, 0, 0, 0);
     }
+    if (p.input_scale) {
+#pragma unroll
+      for (int i = 0; i < VECS; ++i) {
+        const int k = (i * THREADS + tid) * 8;
+        if (k >= p.K) break;
+        const float4 a = __ldg(reinterpret_cast<const float4*>(p.input_scale + k)), b = __ldg(reinterpret_cast<const float4*>(p.input_scale + k + 4));
+        const float d[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        T* v = reinterpret_cast<T*>(&x[i]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = from_float<T>(__fdiv_rn(to_float<T>(v[j]), d[j]));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) top = __vmaxu2(top, q8::magnitudes(x[i]));
+    top = max(top & 0xffffu, top >> 16);
   } else {
-    for (int k = tid; k < p.K; k += kQuantThreads) top = max(top, magnitude(smoothed<T>(row[k], p.input_scale, k)));
+    for (int k = tid; k < p.K; k += THREADS) top = max(top, magnitude(smoothed<T>(row[k], p.input_scale, k)));
   }
   top = __reduce_max_sync(0xffffffffu, top);
   if ((tid & 31) == 0) s_top[tid >> 5] = top;
@@ -85,31 +101,23 @@ __global__ void __launch_bounds__(kQuantThreads) w8a8_quantize_kernel(const Quan
   const uint16_t bits = (uint16_t)top;
   const float amax = to_float<T>(*reinterpret_cast<const T*>(&bits));
   // a row with an infinity or NaN has a step that is not finite, so its outputs are NaN
-  const float step = __fdiv_rn(amax < 1e-6f ? 1e-6f : amax, 127.f);
-  const bool finite = step < INFINITY;
-  const float inv = finite ? __fdiv_rn(1.f, step) : 0.f;
+  const q8::Grid grid(amax < 1e-6f ? 1e-6f : amax);
   int sum = 0;
-  // round(x / step): the product with 1 / step decides except next to a border between two codes (within 1e-4; its own error is
-  // below 2e-5), where the quotient does
-  auto code = [&](T v) {
-    const float x = to_float<T>(v), t = x * inv;
-    float c = rintf(t);
-    if (fabsf(t - c) > 0.4999f) c = rintf(__fdiv_rn(x, step));
-    const int q = finite ? (int)fminf(fmaxf(c, -127.f), 127.f) : 0;
-    sum += q;
-    return q;
-  };
-  if (VEC) {
-    for (int k = tid * 8; k < p.K; k += kQuantThreads * 8) {
-      const uint4 w = *reinterpret_cast<const uint4*>(row + k);
-      const T* v = reinterpret_cast<const T*>(&w);
-      uint32_t o[2] = {0, 0};
+  if constexpr (VECS > 0) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) o[j >> 2] |= ((uint32_t)code(smoothed<T>(v[j], p.input_scale, k + j)) & 0xffu) << (8 * (j & 3));
-      *reinterpret_cast<uint2*>(out + k) = make_uint2(o[0], o[1]);
+    for (int i = 0; i < VECS; ++i) {
+      const int k = (i * THREADS + tid) * 8;
+      if (k >= p.K) break;
+      const uint2 o = grid.codes<T>(x[i]);
+      sum = __dp4a((int)o.y, 0x01010101, __dp4a((int)o.x, 0x01010101, sum));
+      *reinterpret_cast<uint2*>(out + k) = o;
     }
   } else {
-    for (int k = tid; k < p.K; k += kQuantThreads) out[k] = (int8_t)code(smoothed<T>(row[k], p.input_scale, k));
+    for (int k = tid; k < p.K; k += THREADS) {
+      const int c = grid.code(to_float<T>(smoothed<T>(row[k], p.input_scale, k)));
+      sum += c;
+      out[k] = (int8_t)c;
+    }
   }
   sum = __reduce_add_sync(0xffffffffu, sum);
   if ((tid & 31) == 0) s_sum[tid >> 5] = sum;
@@ -118,7 +126,7 @@ __global__ void __launch_bounds__(kQuantThreads) w8a8_quantize_kernel(const Quan
     int all = 0;
 #pragma unroll
     for (int w = 0; w < kW; ++w) all += s_sum[w];
-    p.step[m] = finite ? step : __int_as_float(0x7fffffff);
+    p.step[m] = grid.finite ? grid.step : __int_as_float(0x7fffffff);
     p.sums[m] = all;
   }
 }
@@ -141,6 +149,24 @@ struct W8Params {
   int* counters;         // [thread block]: arrivals at the tile that it begins and others continue; behind them a word for failures
 };
 
+// bar_wait for arrivals from another thread block of the cluster
+__device__ __forceinline__ bool bar_test_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ void bar_wait_cluster(uint32_t bar, uint32_t parity, int* status, bool& dead) {
+  if (dead || bar_test_cluster(bar, parity)) return;
+  bar_wait(bar, parity, status, dead);
+  if (!dead) bar_test_cluster(bar, parity);      // the same phase again, for its order with the other thread block's accesses
+}
+
 // both operands in shared memory, 8-bit integers
 __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate, uint32_t elected) {
   asm volatile(
@@ -150,6 +176,63 @@ __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t da, uint64_t d
       "@q tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
       "l"(da), "l"(db), "r"(idesc), "r"(accumulate), "r"(elected)
       : "memory");
+}
+
+// A thread's sums of one output column (weight row) and sixteen activation rows -> outputs.
+template <typename T>
+struct Epilogue {
+  T* y;
+  int64_t ldy;
+  int M, N, n, zi;
+  float bias, scale, zf;
+  bool has_zero, pair_out, bad;
+
+  __device__ __forceinline__ Epilogue(const W8Params& p)
+      : y(reinterpret_cast<T*>(p.y)), ldy(p.ldy), M(p.M), N(p.N), has_zero(p.zero != nullptr),
+        pair_out((reinterpret_cast<uintptr_t>(p.y) & 3u) == 0 && (p.ldy & 1) == 0 && (p.N & 1) == 0), bad(false) {}
+  // The zero-point's whole part is taken off in integers, exactly; what is left (0 for the zero-points of quantizers, or a value
+  // beyond any code) in fp32.
+  __device__ __forceinline__ void column(const W8Params& p, int col) {
+    n = col;
+    bias = (p.bias && n < N) ? to_float<T>(reinterpret_cast<const T*>(p.bias)[n]) : 0.f;
+    scale = n < N ? p.scale[n] : 0.f;
+    const float z = (p.zero && n < N) ? p.zero[n] : 0.f;
+    zi = fabsf(z) <= 128.f ? __float2int_rn(z) : 0;
+    zf = z - (float)zi;
+  }
+  // rows m0 .. m0 + 15 (those below `end`); steps, sums: of these rows, in shared memory
+  __device__ __forceinline__ void store16(const int (&a)[16], int m0, int end, const float* steps, const int* sums) const {
+    const int odd = threadIdx.x & 1;
+    float f[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int xs = sums[i];
+      float v = (float)(a[i] - zi * xs);
+      if (has_zero) v = fmaf(-zf, (float)xs, v);
+      f[i] = bad ? __int_as_float(0x7fffffff) : fmaf(v, steps[i] * scale, bias);
+    }
+    if (pair_out) {   // neighbouring lanes swap so that each stores two columns of every other row
+      T* at = y + (int64_t)(m0 + odd) * ldy + (n & ~1);
+#pragma unroll
+      for (int i = 0; i < 16; i += 2, at += 2 * ldy) {
+        const float mine = odd ? f[i + 1] : f[i], got = __shfl_xor_sync(0xffffffffu, odd ? f[i] : f[i + 1], 1);
+        const uint32_t w = odd ? Pair<T>::pack(got, mine) : Pair<T>::pack(mine, got);
+        if (m0 + i + odd < end && n < N) *reinterpret_cast<uint32_t*>(at) = w;
+      }
+    } else if (n < N) {
+      T* at = y + (int64_t)m0 * ldy + n;
+#pragma unroll
+      for (int i = 0; i < 16; ++i, at += ldy)
+        if (m0 + i < end) *at = from_float<T>(f[i]);
+    }
+  }
+};
+
+__device__ __forceinline__ void load16(uint32_t taddr, int (&a)[16]) {
+  uint32_t v[16];
+  tmem_ld16(taddr, v);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) a[i] = (int)v[i];
 }
 
 template <typename T>
@@ -255,9 +338,7 @@ __global__ void __launch_bounds__(kThreads, 1) w8a8_gemm_kernel(const __grid_con
     // ================= epilogue: tensor memory -> registers -> global =================
     pdl_wait();
     const int q4 = warp & 3, te = threadIdx.x - 4 * 32;
-    T* yg = reinterpret_cast<T*>(p.y);
-    const T* bias = reinterpret_cast<const T*>(p.bias);
-    const bool pair_out = (reinterpret_cast<uintptr_t>(p.y) & 3u) == 0 && (p.ldy & 1) == 0 && (p.N & 1) == 0;
+    Epilogue<T> epi(p);
     auto epi_sync = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
     int* failures = p.counters + gridDim.x;
     int seg = 0;
@@ -265,61 +346,23 @@ __global__ void __launch_bounds__(kThreads, 1) w8a8_gemm_kernel(const __grid_con
       const int t = u / ku, k0 = u - t * ku, len = min(ku - k0, u1 - u);
       u += len;
       const int row0 = t / p.mtiles * kRows, m0 = t % p.mtiles * p.mt;
-      const int n = row0 + q4 * 32 + lane, mrows = min(p.mt, p.M - m0);
-      const int buf = seg & 1;
+      const int mrows = min(p.mt, p.M - m0), buf = seg & 1;
       const uint32_t acc = tmem + buf * 256 + ((uint32_t)(q4 * 32) << 16);
-      const float bv = (bias && n < p.N) ? to_float<T>(bias[n]) : 0.f, sv = n < p.N ? p.scale[n] : 0.f;
-      // the zero-point's whole part is taken off in integers, exactly; what is left (0 for the zero-points of quantizers, or a
-      // value beyond any code) in fp32
-      const float z = (p.zero && n < p.N) ? p.zero[n] : 0.f;
-      const int zi = fabsf(z) <= 128.f ? __float2int_rn(z) : 0;
-      const float zf = z - (float)zi;
+      epi.column(p, row0 + q4 * 32 + lane);
       epi_sync();     // the tile before has been written
       for (int i = te; i < mrows; i += 128) {
         s_step[i] = p.step[m0 + i];
         s_sums[i] = p.sums[m0 + i];
       }
       epi_sync();
-      bool bad = false;
-      const int odd = lane & 1;
-      T* const mine_at = yg + (int64_t)(m0 + odd) * p.ldy + (n & ~1);
-      auto store16 = [&](const int (&a)[16], int c) {
-        float f[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int m = min(c + i, 255), xs = s_sums[m];
-          float v = (float)(a[i] - zi * xs);
-          if (p.zero) v = fmaf(-zf, (float)xs, v);
-          f[i] = bad ? __int_as_float(0x7fffffff) : fmaf(v, s_step[m] * sv, bv);
-        }
-        if (pair_out) {   // neighbouring lanes swap so that each stores two columns of every other row
-          T* at = mine_at + (int64_t)c * p.ldy;
-#pragma unroll
-          for (int i = 0; i < 16; i += 2, at += 2 * p.ldy) {
-            const float mine = odd ? f[i + 1] : f[i], got = __shfl_xor_sync(0xffffffffu, odd ? f[i] : f[i + 1], 1);
-            const uint32_t w = odd ? Pair<T>::pack(got, mine) : Pair<T>::pack(mine, got);
-            if (c + i + odd < mrows && n < p.N) *reinterpret_cast<uint32_t*>(at) = w;
-          }
-        } else if (n < p.N) {
-          T* at = yg + (int64_t)(m0 + c) * p.ldy + n;
-#pragma unroll
-          for (int i = 0; i < 16; ++i, at += p.ldy)
-            if (c + i < mrows) *at = from_float<T>(f[i]);
-        }
-      };
+      auto store16 = [&](const int (&a)[16], int c) { epi.store16(a, m0 + c, m0 + mrows, s_step + c, s_sums + c); };
       bar_wait(acc_full + buf * 8, (seg >> 1) & 1, status, dead);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      bad = __any_sync(0xffffffffu, dead || *const_cast<volatile int*>(&s_failed) != 0);
-      auto load16 = [&](int c, int (&a)[16]) {
-        uint32_t v[16];
-        tmem_ld16(acc + c, v);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) a[i] = (int)v[i];
-      };
+      epi.bad = __any_sync(0xffffffffu, dead || *const_cast<volatile int*>(&s_failed) != 0);
       if (len == ku) {
         for (int c = 0; c < mrows; c += 16) {
           int a[16];
-          load16(c, a);
+          load16(acc + c, a);
           store16(a, c);
         }
       } else {
@@ -330,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1) w8a8_gemm_kernel(const __grid_con
         auto slot_of = [&](int b) {   // [mt / 4][128 n][4 m]: four rows of this thread's column per 16-byte access
           return reinterpret_cast<int4*>(p.partial + ((size_t)b * 2 + (b == first ? 1 : 0)) * slot_ints) + q4 * 32 + lane;
         };
-        if (bad && lane == 0) atomicExch(failures, 1);
+        if (epi.bad && lane == 0) atomicExch(failures, 1);
         epi_sync();
         if (te == 0) {
           int have;
@@ -344,7 +387,7 @@ __global__ void __launch_bounds__(kThreads, 1) w8a8_gemm_kernel(const __grid_con
           int4* dst = slot_of(me);
           for (int c = 0; c < mrows; c += 16) {
             int a[16];
-            load16(c, a);
+            load16(acc + c, a);
 #pragma unroll
             for (int i = 0; i < 4; ++i) __stcg(dst + (c / 4 + i) * kRows, make_int4(a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3]));
           }
@@ -356,11 +399,11 @@ __global__ void __launch_bounds__(kThreads, 1) w8a8_gemm_kernel(const __grid_con
         }
         if (finish) {
           __threadfence();
-          bad = bad || __ldcg(failures) != 0;
+          epi.bad = epi.bad || __ldcg(failures) != 0;
           for (int c = 0; c < mrows; c += 16) {
             int a[16];
             if (in_tmem) {
-              load16(c, a);
+              load16(acc + c, a);
             } else {
 #pragma unroll
               for (int i = 0; i < 16; ++i) a[i] = 0;
@@ -397,9 +440,282 @@ __global__ void __launch_bounds__(kThreads, 1) w8a8_gemm_kernel(const __grid_con
   }
 }
 
+// ---- product, two SMs on a tile -------------------------------------------------------------------------------------------------------
+// With one SM per 128 x 256 tile every unit brings 48 KB from L2, and at 87 GB/s and SM (measured: half the MMAs take the same time) that, not the MMAs,
+// sets the pace.  cta_group::2 pairs two SMs on 256 weight rows x mt activation rows: each loads its own 128 weight rows and half of
+// the activation rows, the MMA reads both halves, 32 KB per unit.  The even thread block of a pair issues the MMAs; its `full`
+// barrier counts the bytes of both; commits arrive in both.
+//
+// A cluster is one pair, walking over tiles, or (few tiles) 2 or 4 pairs that split K of one tile: then each of them adds up a
+// share of the activation rows, which the others send to its shared memory.
+struct PairParams {
+  W8Params w;
+  int tiles, splits;
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t in_block(uint32_t addr, uint32_t rank) {     // the same place in another thread block of the cluster
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tma_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void umma_i8_pair(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate, uint32_t elected) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(da), "l"(db), "r"(idesc), "r"(accumulate), "r"(elected)
+      : "memory");
+}
+__device__ __forceinline__ void umma_commit_pair(uint32_t bar, uint32_t mask, uint32_t elected) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t.reg .b16 m;\n\t"
+      "setp.ne.b32 q, %2, 0;\n\t"
+      "cvt.u16.u32 m, %1;\n\t"
+      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], m;\n\t}" ::"r"(bar), "r"(mask), "r"(elected)
+      : "memory");
+}
+__device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1) w8a8_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
+                                                                const PairParams pp) {
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ int s_failed;
+  __shared__ float s_step[256];
+  __shared__ int s_sums[256];
+  const W8Params& p = pp.w;
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int ku = p.ku, stages = p.stages;
+  const uint32_t half = (uint32_t)p.mt / 2, x_bytes = half * kUnitK, w_ring = s_u32(smem), x_ring = w_ring + stages * kWBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + stages * (kWBytes + x_bytes));
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kMaxStages + 5);
+  const uint32_t full = s_u32(bars), empty = full + kMaxStages * 8, acc_full = empty + kMaxStages * 8, acc_empty = acc_full + 16,
+                 mma_done = acc_empty + 16;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank(), odd = rank & 1, leader = rank & ~1u, pair_mask = 3u << leader;
+  const int split = (int)rank >> 1, splits = pp.splits;
+  // units of K that this pair takes; clusters of one pair walk over tiles, others have one
+  const int k0 = (int)((int64_t)ku * split / splits), k1 = (int)((int64_t)ku * (split + 1) / splits), n_k = k1 - k0;
+  const int first = (int)blockIdx.x / (2 * splits), step = (int)gridDim.x / (2 * splits);
+  bool dead = false;
+  int* status = &s_failed;
+
+  if (threadIdx.x == 0) {
+    s_failed = 0;
+    for (int i = 0; i < kMaxStages; ++i) {
+      bar_init(full + i * 8, 1);
+      bar_init(empty + i * 8, 1);
+    }
+    bar_init(mma_done, 1);
+    for (int i = 0; i < 2; ++i) {
+      bar_init(acc_full + i * 8, 1);
+      bar_init(acc_empty + i * 8, 8);       // the epilogue warps of both thread blocks
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_u32(tmem_slot)), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  cluster_sync();         // barriers of the others are ready
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+
+  if (warp == 0) {
+    // ================= operands: own weight rows, own half of the activation rows =================
+    if (lane == 0) {
+      const uint32_t full_at = in_block(full, leader);
+      const int mine = first < pp.tiles ? (pp.tiles - first + step - 1) / step * n_k : 0;      // units of all tiles
+      struct Place {      // of a unit, kept by counting
+        int t, k, row, m0;
+      };
+      auto at_tile = [&](int t) { return Place{t, k0, t / p.mtiles * 2 * kRows + (int)(odd * kRows), t % p.mtiles * p.mt + (int)(odd * half)}; };
+      auto next = [&](Place& a) {
+        if (++a.k == k1) a = at_tile(a.t + step);
+      };
+      auto load_w = [&](const Place& a, int s) {
+        if (!odd) bar_expect(full + s * 8, 2 * (kWBytes + x_bytes));
+        tma_pair(w_ring + s * kWBytes, &tm_w, a.k * kUnitK, a.row, full_at + s * 8);
+      };
+      auto load_x = [&](const Place& a, int s) { tma_pair(x_ring + s * x_bytes, &tm_x, a.k * kUnitK, a.m0, full_at + s * 8); };
+      Place at = at_tile(first), x_at = at;
+      int i = 0;
+      for (; i < min(mine, stages); ++i, next(at)) load_w(at, i);      // weights: nothing that this launch may overlap writes them
+      pdl_wait();
+      for (int j = 0; j < i; ++j, next(x_at)) load_x(x_at, j);
+      int s = 0;
+      uint32_t par = 0;
+      for (; i < mine; ++i, next(at)) {
+        bar_wait(empty + s * 8, par, status, dead);
+        if (dead) break;
+        load_w(at, s);
+        load_x(at, s);
+        if (++s == stages) s = 0, par ^= 1;
+      }
+      bool late = false;
+      if (!odd)       // the copies of both thread blocks end here
+        for (int j = max(0, i - stages); j < i; ++j) bar_wait(full + (j % stages) * 8, (j / stages) & 1, status, late);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ================= products =================
+    if (!odd) {
+      const uint32_t me = elect_one();
+      const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(p.mt >> 3) << 17) | ((uint32_t)(2 * kRows >> 4) << 24);
+      const uint64_t w_desc0 = umma_desc(w_ring), x_desc0 = umma_desc(x_ring);
+      int s = 0, seg = 0;
+      uint32_t par = 0;
+      for (int t = first; t < pp.tiles; t += step, ++seg) {
+        const int buf = seg & 1;
+        const uint32_t acc = tmem + buf * 256;
+        bar_wait_cluster(acc_empty + buf * 8, ((seg >> 1) & 1) ^ 1, status, dead);
+        for (int i = 0; i < n_k; ++i) {
+          bar_wait(full + s * 8, par, status, dead);
+          __syncwarp();
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint64_t dw = w_desc0 + (uint64_t)(s * (kWBytes >> 4)), dx = x_desc0 + (uint64_t)(s * (x_bytes >> 4));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) umma_i8_pair(acc, dw + 2 * j, dx + 2 * j, idesc, (i | j) != 0, me);
+          umma_commit_pair(empty + s * 8, pair_mask, me);
+          if (++s == stages) s = 0, par ^= 1;
+        }
+        if (dead)       // the other thread block's outputs are no good either
+          asm volatile("st.shared::cluster.s32 [%0], %1;\n\tfence.acq_rel.cluster;" ::"r"(in_block(s_u32(&s_failed), leader + 1)), "r"((int)PARE_ERR_TIMEOUT) : "memory");
+        umma_commit_pair(acc_full + buf * 8, pair_mask, me);
+      }
+      umma_commit_pair(mma_done, 1u << leader, me);
+      bool late = false;
+      bar_wait(mma_done, 0, status, late);
+    }
+    __syncwarp();
+  } else if (warp >= 4 && splits == 1) {
+    // ================= epilogue: tensor memory -> registers -> global =================
+    pdl_wait();
+    const int q4 = warp & 3, te = threadIdx.x - 4 * 32;
+    const uint32_t empty_at = in_block(acc_empty, leader);
+    Epilogue<T> epi(p);
+    int seg = 0;
+    for (int t = first; t < pp.tiles; t += step, ++seg) {
+      const int m0 = t % p.mtiles * p.mt, mrows = min(p.mt, p.M - m0), buf = seg & 1;
+      const uint32_t acc = tmem + buf * 256 + ((uint32_t)(q4 * 32) << 16);
+      epi.column(p, t / p.mtiles * 2 * kRows + odd * kRows + q4 * 32 + lane);
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      for (int i = te; i < mrows; i += 128) {
+        s_step[i] = p.step[m0 + i];
+        s_sums[i] = p.sums[m0 + i];
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      bar_wait(acc_full + buf * 8, (seg >> 1) & 1, status, dead);
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      epi.bad = __any_sync(0xffffffffu, dead || *const_cast<volatile int*>(&s_failed) != 0);
+      for (int c = 0; c < mrows; c += 16) {
+        int a[16];
+        load16(acc + c, a);
+        epi.store16(a, m0 + c, m0 + mrows, s_step + c, s_sums + c);
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) arrive_at(empty_at + buf * 8);
+    }
+  }
+
+  if (splits > 1) {
+    // ================= one tile: its sums meet in the cluster =================
+    const int q4 = warp & 3, te = threadIdx.x - 4 * 32;
+    const int m0 = first % p.mtiles * p.mt, mrows = min(p.mt, p.M - m0), share = p.mt / splits;
+    const uint32_t acc = tmem + ((uint32_t)(q4 * 32) << 16), row = (uint32_t)(q4 * 32 + lane);
+    if (warp >= 4) {
+      bar_wait(acc_full, 0, status, dead);
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    }
+    __syncthreads();
+    cluster_sync();       // everybody's products are done: the rings are free
+    // [sender's number without the receiver][share / 4][128 weight rows][4 activation rows]
+    const uint32_t slot_bytes = (uint32_t)share * kRows * 4;
+    if (warp >= 4) {
+      for (int q = 0; q < splits; ++q) {
+        if (q == split || q * share >= mrows) continue;
+        const uint32_t to = in_block(w_ring + (split < q ? split : split - 1) * slot_bytes, 2 * q + odd);
+        for (int c = 0; c < share; c += 16) {
+          int a[16];
+          load16(acc + q * share + c, a);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            asm volatile("st.shared::cluster.v4.s32 [%0], {%1, %2, %3, %4};" ::"r"(to + ((c / 4 + i) * kRows + row) * 16), "r"(a[4 * i]),
+                         "r"(a[4 * i + 1]), "r"(a[4 * i + 2]), "r"(a[4 * i + 3])
+                         : "memory");
+        }
+      }
+      if (*const_cast<volatile int*>(&s_failed) != 0 && te == 0) {     // a failure of one is a failure of the tile
+        for (int q = 0; q < 2 * splits; ++q)
+          asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(in_block(s_u32(&s_failed), q)), "r"((int)PARE_ERR_TIMEOUT) : "memory");
+      }
+    }
+    __syncthreads();
+    cluster_sync();
+    if (warp >= 4) {
+      pdl_wait();
+      const int from = split * share, to = min(from + share, mrows);
+      Epilogue<T> epi(p);
+      epi.column(p, first / p.mtiles * 2 * kRows + odd * kRows + (int)row);
+      epi.bad = *const_cast<volatile int*>(&s_failed) != 0;
+      for (int i = te; i < to - from; i += 128) {
+        s_step[i] = p.step[m0 + from + i];
+        s_sums[i] = p.sums[m0 + from + i];
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      for (int c = 0; c < to - from; c += 16) {
+        int a[16];
+        load16(acc + from + c, a);
+        for (int e = 0; e < splits - 1; ++e) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint4 v = ld_s128(w_ring + e * slot_bytes + ((c / 4 + i) * kRows + row) * 16);
+            a[4 * i] += (int)v.x;
+            a[4 * i + 1] += (int)v.y;
+            a[4 * i + 2] += (int)v.z;
+            a[4 * i + 3] += (int)v.w;
+          }
+        }
+        epi.store16(a, m0 + from + c, m0 + to, s_step + c, s_sums + c);
+      }
+    }
+  }
+
+  // ---- teardown: both thread blocks done with tensor memory and each other's shared memory, then free it ----
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  cluster_sync();
+  if (warp == 2) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
 // ---- host side --------------------------------------------------------------------------------------------------------------------------
 struct W8Plan {
   int mt, mtiles, ku, run, blocks, stages;
+  int splits;        // 0: one SM per tile (runs of units); 1, 2, 4: pairs of SMs
+  int tiles;         // weight tiles x activation tiles
   int64_t units;
 };
 
@@ -407,7 +723,7 @@ struct W8Plan {
 W8Plan w8_plan(int M, int N, int K) {
   W8Plan best{};
   double least = 1e30;
-  const int sms = sm_count();
+  const int sms = sm_count(), ku = (K + kUnitK - 1) / kUnitK;
   int seen = 0;
   for (int target : {256, 192, 128, 96, 64, 32, 16}) {
     W8Plan g{};
@@ -416,9 +732,9 @@ W8Plan w8_plan(int M, int N, int K) {
     g.mtiles = (M + g.mt - 1) / g.mt;
     if (g.mt == seen) continue;
     seen = g.mt;
-    g.ku = (K + kUnitK - 1) / kUnitK;
-    const int64_t tiles = (int64_t)((N + kRows - 1) / kRows) * g.mtiles;
-    g.units = tiles * g.ku;
+    g.ku = ku;
+    g.tiles = (N + kRows - 1) / kRows * g.mtiles;
+    g.units = (int64_t)g.tiles * g.ku;
     const double unit_us = 0.15 + 0.0006 * g.mt;
     auto consider = [&](int64_t run) {
       if (run < 1 || (g.units + run - 1) / run > sms) return;
@@ -430,12 +746,40 @@ W8Plan w8_plan(int M, int N, int K) {
         best = g;
       }
     };
-    consider((tiles + sms - 1) / sms * g.ku);
+    consider((int64_t)(g.tiles + sms - 1) / sms * g.ku);
     consider((g.units + sms - 1) / sms);
     for (int parts = 2; parts <= 16; ++parts) consider((g.ku + parts - 1) / parts);
   }
-  best.blocks = (int)((best.units + best.run - 1) / best.run);
-  best.stages = kRingBytes / (kWBytes + best.mt * kUnitK);
+  for (int target : {256, 192, 128, 96, 64}) {
+    for (int splits : {1, 2, 4}) {
+      W8Plan g{};
+      const int grain = splits == 4 ? 64 : 32;
+      g.mtiles = (M + target - 1) / target;
+      g.mt = ((M + g.mtiles - 1) / g.mtiles + grain - 1) / grain * grain;
+      g.mtiles = (M + g.mt - 1) / g.mt;
+      g.ku = ku;
+      g.splits = splits;
+      g.tiles = (N + 2 * kRows - 1) / (2 * kRows) * g.mtiles;
+      g.units = (int64_t)g.tiles * g.ku;
+      if (g.mt > 256 || splits > ku) continue;
+      const int clusters = sms / (2 * splits), rounds = (g.tiles + clusters - 1) / clusters;
+      if (splits > 1 && rounds > 1) continue;
+      const double cost = (double)rounds * ((ku + splits - 1) / splits) * (0.15 + 0.0005 * g.mt) + 0.01 * g.mt + 1.0 * (splits > 1);
+      if (cost < least - 1e-9) {
+        least = cost;
+        best = g;
+      }
+    }
+  }
+  if (best.splits) {
+    const int clusters = sms / (2 * best.splits);
+    best.run = ku;
+    best.blocks = 2 * best.splits * (best.splits > 1 || best.tiles < clusters ? best.tiles : clusters);
+    best.stages = kRingBytes / (kWBytes + best.mt / 2 * kUnitK);
+  } else {
+    best.blocks = (int)((best.units + best.run - 1) / best.run);
+    best.stages = kRingBytes / (kWBytes + best.mt * kUnitK);
+  }
   if (best.stages > kMaxStages) best.stages = kMaxStages;
   return best;
 }
@@ -493,18 +837,26 @@ int pare_w8a8_forward(const void* x, int x_dtype, int64_t ldx, const int8_t* wei
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
   };
   CUtensorMap tw, tx;
-  PARE_REQUIRE(map(&tw, weight, N, ldw, kRows) && map(&tx, ws + sp.codes, M, sp.ldc, g.mt), PARE_ERR_CUDA);
+  PARE_REQUIRE(map(&tw, weight, N, ldw, kRows) && map(&tx, ws + sp.codes, M, sp.ldc, g.splits ? g.mt / 2 : g.mt), PARE_ERR_CUDA);
 
   const QuantParams q{x, ldx, input_scale, reinterpret_cast<int8_t*>(ws + sp.codes), sp.ldc, reinterpret_cast<float*>(ws + sp.step),
                       reinterpret_cast<int*>(ws + sp.sums), reinterpret_cast<int*>(ws + sp.counters), g.blocks + 1, K};
-  const bool vec = aligned16(x) && (M == 1 || ldx % 8 == 0) && K % 8 == 0;
-  if (x_dtype == PARE_F16) {
-    if (vec) w8a8_quantize_kernel<__half, true><<<M, kQuantThreads, 0, st>>>(q);
-    else w8a8_quantize_kernel<__half, false><<<M, kQuantThreads, 0, st>>>(q);
-  } else {
-    if (vec) w8a8_quantize_kernel<__nv_bfloat16, true><<<M, kQuantThreads, 0, st>>>(q);
-    else w8a8_quantize_kernel<__nv_bfloat16, false><<<M, kQuantThreads, 0, st>>>(q);
-  }
+  const bool vec = aligned16(x) && (M == 1 || ldx % 8 == 0) && K % 8 == 0 && (!input_scale || aligned16(input_scale));
+  // Many rows: few threads with several vectors in flight each, so that all rows are resident at once; few rows: many threads.
+  auto quantize = [&](auto tag) {
+    using E = decltype(tag);
+    auto go = [&](auto kern, int threads) { kern<<<M, threads, 0, st>>>(q); };
+    const bool many = M > 2 * sm_count();
+    if (!vec || K > 32768) go(w8a8_quantize_kernel<E, 512, 0>, 512);
+    else if (many && K <= 4096) go(w8a8_quantize_kernel<E, 128, 4>, 128);
+    else if (K <= 4096) go(w8a8_quantize_kernel<E, 512, 1>, 512);
+    else if (many && K <= 8192) go(w8a8_quantize_kernel<E, 256, 4>, 256);
+    else if (K <= 16384) go(w8a8_quantize_kernel<E, 512, 4>, 512);
+    else if (K <= 20480) go(w8a8_quantize_kernel<E, 512, 5>, 512);
+    else go(w8a8_quantize_kernel<E, 512, 8>, 512);
+  };
+  if (x_dtype == PARE_F16) quantize(__half());
+  else quantize(__nv_bfloat16());
   if (cudaGetLastError() != cudaSuccess) return PARE_ERR_CUDA;
 
   W8Params p{};
@@ -525,13 +877,27 @@ int pare_w8a8_forward(const void* x, int x_dtype, int64_t ldx, const int8_t* wei
   p.stages = g.stages;
   p.partial = reinterpret_cast<int*>(ws + sp.partial);
   p.counters = q.zeroed;
-  const size_t smem = 1024 + (size_t)g.stages * (kWBytes + g.mt * kUnitK) + 512;
-  auto launch = [&](auto kern) -> int {
+  const size_t smem = 1024 + (size_t)g.stages * (kWBytes + (g.splits ? g.mt / 2 : g.mt) * kUnitK) + 512;
+  auto launch = [&](auto kern, const auto& params, int cluster) -> int {
     if (!ensure_smem_attr(reinterpret_cast<const void*>(kern), kMaxSmem)) return PARE_ERR_CUDA;
-    const int rc = launch_pdl(kern, dim3(g.blocks), dim3(kThreads), smem, st, tw, tx, p);
-    return rc != PARE_OK ? rc : launch_status();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(g.blocks);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim = {(unsigned)cluster, 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kern, tw, tx, params) == cudaSuccess ? launch_status() : (int)PARE_ERR_CUDA;
   };
-  return x_dtype == PARE_F16 ? launch(w8a8_gemm_kernel<__half>) : launch(w8a8_gemm_kernel<__nv_bfloat16>);
+  const bool half = x_dtype == PARE_F16;
+  if (g.splits == 0) return half ? launch(w8a8_gemm_kernel<__half>, p, 1) : launch(w8a8_gemm_kernel<__nv_bfloat16>, p, 1);
+  const PairParams pp{p, g.tiles, g.splits};
+  return half ? launch(w8a8_pair_kernel<__half>, pp, 2 * g.splits) : launch(w8a8_pair_kernel<__nv_bfloat16>, pp, 2 * g.splits);
 }
 
 }  // extern "C"
