@@ -300,14 +300,14 @@ int pare_rope(const void* x, int64_t stride_b, int64_t stride_h, int64_t stride_
  * themselves are multiplied:
  *   x~ = x, or dtype(x / input_scale);  step = max(max_k |x~|, 1e-6) / 127;  c = round_half_even(x~ / step) in [-127, 127]
  *   y = dtype((sum_k c q - zero sum_k c) * step * scale + bias)
- *   x            [M, ldx]  F16 or BF16
+ *   x            [M, ldx]  F16 or BF16; 16-byte aligned with ldx % 8 == 0 if M <= 16 and K % 8 == 0
  *   weight       [N, ldw]  int8, ldw >= K a multiple of 16, 16-byte aligned
  *   scale, zero  [N] float32 (zero may be NULL = 0)
  *   input_scale  optional [K] float32, divides the activations first (the quotient rounded to their dtype)
  *   bias         optional [N] x_dtype;   y [M, ldy] x_dtype
  * The integer sums are exact (K <= 65536; zero-points up to 128 in magnitude are taken off in integers, others in float32).  Rows
- * with an infinity or NaN give NaN.  The workspace (16-byte aligned, pare_w8a8_workspace_bytes(), 0: sizes not supported) need
- * not be initialised and holds nothing between calls.  A bounded wait that runs out shows as NaN in the outputs it concerns. */
+ * with an infinity or NaN give NaN.  The workspace (16-byte aligned, pare_w8a8_workspace_bytes(); 0: none is needed, or the call
+ * refuses these sizes) need not be initialised and holds nothing between calls.  A bounded wait that runs out shows as NaN in the outputs it concerns. */
 size_t pare_w8a8_workspace_bytes(int M, int N, int K);
 int pare_w8a8_forward(const void* x, int x_dtype, int64_t ldx, const int8_t* weight, int64_t ldw, const float* scale,
                       const float* zero, const float* input_scale, const void* bias, void* y, int64_t ldy,

@@ -15,6 +15,8 @@
 //   warp 0     TMA of both operands      warp 1  tcgen05.mma      warp 2  tensor memory      warps 4-7  epilogue
 // All waits are bounded; when one runs out the thread block stops waiting and loading, lets its copies and products in flight
 // end, and its outputs become NaN.
+#include <algorithm>
+
 #include "quant8.cuh"
 #include "tcgen05.cuh"
 
@@ -186,6 +188,7 @@ struct Epilogue {
   int M, N, n, zi;
   float bias, scale, zf;
   bool has_zero, pair_out, bad;
+  int row_sum = 0;       // where no array of sums is given: of row `lane`
 
   __device__ __forceinline__ Epilogue(const W8Params& p)
       : y(reinterpret_cast<T*>(p.y)), ldy(p.ldy), M(p.M), N(p.N), has_zero(p.zero != nullptr),
@@ -201,12 +204,12 @@ struct Epilogue {
     zf = z - (float)zi;
   }
   // rows m0 .. m0 + 15 (those below `end`); steps, sums: of these rows, in shared memory
-  __device__ __forceinline__ void store16(const int (&a)[16], int m0, int end, const float* steps, const int* sums) const {
+  __device__ __forceinline__ void store16(const int (&a)[16], int m0, int end, const float* steps, const int* sums = nullptr) const {
     const int odd = threadIdx.x & 1;
     float f[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const int xs = sums[i];
+      const int xs = sums ? sums[i] : __shfl_sync(0xffffffffu, row_sum, i);
       float v = (float)(a[i] - zi * xs);
       if (has_zero) v = fmaf(-zf, (float)xs, v);
       f[i] = bad ? __int_as_float(0x7fffffff) : fmaf(v, steps[i] * scale, bias);
@@ -711,10 +714,338 @@ __global__ void __launch_bounds__(kThreads, 1) w8a8_pair_kernel(const __grid_con
   }
 }
 
+// ---- product of up to 16 rows, tokens quantized on the way ---------------------------------------------------------------------------------
+// Streams the weights once, and what counts besides is the number of steps that wait for one another: so one launch, in which the
+// weights are on their way from the first moment while the tokens become codes.  `splits` thread blocks (a cluster of 1, 2, 4) share a
+// weight tile's K; each quantizes its own columns (row maxima are exchanged through shared memory), keeps their codes there in the
+// order of the MMA's operand for all its tiles, and finishes the sums of its share of the 128 weight rows with what the others send.
+//   warp 0  TMA of weights     warp 1  tcgen05.mma     warp 2  tensor memory     warps 4-11  tokens, then (4-7) the epilogue
+constexpr int kFewRows = 16;
+constexpr int kFewThreads = 384;
+constexpr int kFewCodes = 256;                        // threads that quantize
+constexpr int kFewUnitBytes = kFewRows * kUnitK;      // codes of a unit
+constexpr int kFewVecs = 8;                           // vectors of eight columns per thread: they stay in registers
+constexpr int kFewMaxUnits = 60;                      // units of K per thread block: 120 KB of codes
+constexpr uint32_t kFewTmem = 32;                     // two accumulators of 16 columns
+
+struct FewParams {
+  W8Params w;
+  const void* x;
+  int64_t ldx;
+  const float* input_scale;
+  int K, tiles, splits;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kFewThreads, 1) w8a8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const FewParams fp) {
+  extern __shared__ unsigned char smem_raw[];
+  pdl_launch_dependents();
+  __shared__ int s_failed;
+  __shared__ uint32_t s_top[4][kFewRows];             // row maxima, from each thread block of the cluster
+  __shared__ int s_sum[4][kFewRows];                  // sums of codes likewise
+  __shared__ float s_step[kFewRows];
+  __shared__ int4 s_in[3 * 128 / 4 * 4];              // sums from the others: [sender][4][rows of this share] of four activation rows
+  __shared__ uint64_t s_bars[2 * kMaxStages + 8];
+  __shared__ uint32_t s_tmem;
+  const W8Params& p = fp.w;
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int ku = p.ku, stages = p.stages, M = p.M, splits = fp.splits;
+  const uint32_t w_ring = s_u32(smem), codes = w_ring + stages * kWBytes;
+  const uint32_t full = s_u32(s_bars), empty = full + kMaxStages * 8, acc_full = empty + kMaxStages * 8, acc_empty = acc_full + 16,
+                 mma_done = acc_empty + 16, x_ready = mma_done + 8, tops_in = x_ready + 8, sums_in = tops_in + 8;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int rank = splits > 1 ? (int)cluster_rank() : 0;
+  const int k0 = ku * rank / splits, k1 = ku * (rank + 1) / splits, n_k = k1 - k0;
+  const int first = (int)blockIdx.x / splits, step = (int)gridDim.x / splits;
+  bool dead = false;
+  int* status = &s_failed;
+
+  if (threadIdx.x == 0) {
+    s_failed = 0;
+    for (int i = 0; i < kMaxStages; ++i) {
+      bar_init(full + i * 8, 1);
+      bar_init(empty + i * 8, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      bar_init(acc_full + i * 8, 1);
+      bar_init(acc_empty + i * 8, 4);
+    }
+    bar_init(mma_done, 1);
+    bar_init(x_ready, kFewCodes / 32);
+    bar_init(tops_in, splits);
+    bar_init(sums_in, splits > 1 ? (splits - 1) * (4 / splits) : 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (threadIdx.x < 4 * kFewRows) (&s_top[0][0])[threadIdx.x] = 0, (&s_sum[0][0])[threadIdx.x] = 0;
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_u32(&s_tmem)), "r"(kFewTmem) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
+  if (splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");    // the others' barriers: waited for below
+
+  if (warp == 0) {
+    // ================= weights =================
+    if (lane == 0) {
+      const int mine = first < fp.tiles ? (fp.tiles - first + step - 1) / step * n_k : 0;
+      int t = first, k = k0, s = 0, i = 0;
+      uint32_t par = 1;
+      for (; i < mine; ++i) {
+        bar_wait(empty + s * 8, par, status, dead);
+        if (dead) break;
+        bar_expect(full + s * 8, kWBytes);
+        tma_tile(w_ring + s * kWBytes, &tm_w, k * kUnitK, t * kRows, full + s * 8);
+        if (++s == stages) s = 0, par ^= 1;
+        if (++k == k1) k = k0, t += step;
+      }
+      bool late = false;
+      for (int j = max(0, i - stages); j < i; ++j) bar_wait(full + (j % stages) * 8, (j / stages) & 1, status, late);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ================= products =================
+    const uint32_t me = elect_one();
+    const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kFewRows >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+    const uint64_t w_desc0 = umma_desc(w_ring), x_desc0 = umma_desc(codes);
+    bar_wait(x_ready, 0, status, dead);
+    int s = 0, seg = 0;
+    uint32_t par = 0;
+    for (int t = first; t < fp.tiles; t += step, ++seg) {
+      const int buf = seg & 1;
+      bar_wait(acc_empty + buf * 8, ((seg >> 1) & 1) ^ 1, status, dead);
+      for (int i = 0; i < n_k; ++i) {
+        bar_wait(full + s * 8, par, status, dead);
+        __syncwarp();
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint64_t dw = w_desc0 + (uint64_t)(s * (kWBytes >> 4)), dx = x_desc0 + (uint64_t)(i * (kFewUnitBytes >> 4));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) umma_i8(tmem + buf * kFewRows, dw + 2 * j, dx + 2 * j, idesc, (i | j) != 0, me);
+        umma_commit(empty + s * 8, me);
+        if (++s == stages) s = 0, par ^= 1;
+      }
+      umma_commit(acc_full + buf * 8, me);
+    }
+    umma_commit(mma_done, me);
+    bool late = false;
+    bar_wait(mma_done, 0, status, late);
+    __syncwarp();
+  } else if (warp >= 4) {
+    // ================= tokens =================
+    pdl_wait();
+    const int tid = threadIdx.x - 4 * 32;
+    int per = kFewCodes;                              // threads per row
+    for (int r = 1; r < M; r <<= 1) per >>= 1;
+    const int m = tid / per, at = tid % per, c0 = k0 * kUnitK, c1 = min(k1 * kUnitK, fp.K);
+    const T* row = reinterpret_cast<const T*>(fp.x) + m * fp.ldx;
+    // all of a row if that is little (then nobody has to ask for a maximum), else this thread block's columns of it
+    const bool whole = splits == 1 || (fp.K / 8 + per - 1) / per <= kFewVecs;
+    const int lo = whole ? 0 : c0, hi = whole ? fp.K : c1;
+    uint4 v[kFewVecs];
+    uint32_t top = 0;
+    if (m < M) {
+#pragma unroll
+      for (int i = 0; i < kFewVecs; ++i) {
+        const int c = lo + (i * per + at) * 8;
+        v[i] = c < hi ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
+      }
+      if (fp.input_scale) {
+#pragma unroll
+        for (int i = 0; i < kFewVecs; ++i) {
+          const int c = lo + (i * per + at) * 8;
+          T* e = reinterpret_cast<T*>(&v[i]);
+          if (c < hi) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) e[j] = smoothed<T>(e[j], fp.input_scale, c + j);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kFewVecs; ++i) top = __vmaxu2(top, q8::magnitudes(v[i]));
+      top = max(top & 0xffffu, top >> 16);
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));      // at least sixteen threads share a row
+    if (m < M && (lane & 15) == 0) atomicMax(&s_top[rank][m], top);
+    asm volatile("bar.sync 2, 256;" ::: "memory");
+    if (splits > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    if (!whole) {      // to everybody, this thread block among them
+      if (tid < kFewRows)
+        for (int q = 0; q < splits; ++q)
+          if (q != rank)
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(in_block(s_u32(&s_top[rank][tid]), q)), "r"(s_top[rank][tid]) : "memory");
+      if (warp == 4) {
+        asm volatile("fence.acq_rel.cluster;" ::: "memory");
+        __syncwarp();
+        if (lane < splits) arrive_at(in_block(tops_in, lane));
+      }
+      bar_wait_cluster(tops_in, 0, status, dead);
+    }
+    if (m < M) {
+      top = s_top[rank][m];
+      if (!whole)
+        for (int q = 0; q < splits; ++q) top = max(top, s_top[q][m]);
+      const uint16_t bits = (uint16_t)top;
+      const float amax = to_float<T>(*reinterpret_cast<const T*>(&bits));
+      const q8::Grid grid(amax < 1e-6f ? 1e-6f : amax);
+      if (at == 0) s_step[m] = grid.finite ? grid.step : __int_as_float(0x7fffffff);
+      int sum = 0;
+#pragma unroll
+      for (int i = 0; i < kFewVecs; ++i) {
+        const int c = lo + (i * per + at) * 8;
+        if (c < c0 || c >= c1) continue;
+        const uint2 o = grid.codes<T>(v[i]);
+        sum = __dp4a((int)o.y, 0x01010101, __dp4a((int)o.x, 0x01010101, sum));
+        const int u = (c - c0) / kUnitK, chunk = (c % kUnitK) / 16;
+        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(codes + u * kFewUnitBytes + m * kUnitK + ((chunk ^ (m & 7)) << 4) + (c & 8)), "r"(o.x), "r"(o.y)
+                     : "memory");
+      }
+      if (p.zero) atomicAdd(&s_sum[rank][m], sum);
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    asm volatile("bar.sync 2, 256;" ::: "memory");    // steps and sums are there for the epilogue
+    if (lane == 0) bar_arrive(x_ready);
+
+    if (warp < 8) {
+      // ================= epilogue =================
+      const int q4 = warp & 3, share = 4 / splits, owner = q4 / share;      // which thread block finishes this warp's 32 weight rows
+      Epilogue<T> epi(p);
+      int seg = 0;
+      for (int t = first; t < fp.tiles; t += step, ++seg) {
+        const int buf = seg & 1;
+        const uint32_t acc = tmem + buf * kFewRows + ((uint32_t)(q4 * 32) << 16);
+        epi.column(p, t * kRows + q4 * 32 + lane);
+        bar_wait(acc_full + buf * 8, (seg >> 1) & 1, status, dead);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        int a[16];
+        load16(acc, a);
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) bar_arrive(acc_empty + buf * 8);
+        bool bad = __any_sync(0xffffffffu, dead || *const_cast<volatile int*>(&s_failed) != 0);
+        if (splits > 1) {      // one tile
+          // slot of the sender among the others; [4][rows of the share]
+          auto slot = [&](int sender, int receiver) { return (sender < receiver ? sender : sender - 1) * 4 * share * 32 + (q4 % share) * 32 + lane; };
+          if (owner != rank) {
+            const uint32_t to = in_block(s_u32(s_in), owner);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              asm volatile("st.shared::cluster.v4.s32 [%0], {%1, %2, %3, %4};" ::"r"(to + (slot(rank, owner) + i * share * 32) * 16), "r"(a[4 * i]),
+                           "r"(a[4 * i + 1]), "r"(a[4 * i + 2]), "r"(a[4 * i + 3])
+                           : "memory");
+            if (p.zero && q4 % share == 0 && lane < kFewRows)
+              asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(in_block(s_u32(&s_sum[rank][lane]), owner)), "r"(s_sum[rank][lane]) : "memory");
+            if (bad && lane == 0)
+              asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(in_block(s_u32(&s_failed), owner)), "r"((int)PARE_ERR_TIMEOUT) : "memory");
+            asm volatile("fence.acq_rel.cluster;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) arrive_at(in_block(sums_in, owner));
+            continue;
+          }
+          bar_wait_cluster(sums_in, 0, status, dead);
+          bad = __any_sync(0xffffffffu, dead || *const_cast<volatile int*>(&s_failed) != 0);
+          for (int q = 0; q < splits; ++q) {
+            if (q == rank) continue;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int4 v = s_in[slot(q, rank) + i * share * 32];
+              a[4 * i] += v.x;
+              a[4 * i + 1] += v.y;
+              a[4 * i + 2] += v.z;
+              a[4 * i + 3] += v.w;
+            }
+          }
+          if (p.zero) {        // sums over all of K in this warp's own copy
+            int all = 0;
+            if (lane < kFewRows)
+              for (int q = 0; q < splits; ++q) all += s_sum[q][lane];
+            epi.row_sum = all;
+          }
+        } else if (p.zero) {
+          epi.row_sum = lane < kFewRows ? s_sum[0][lane] : 0;
+        }
+        epi.bad = bad;
+        epi.store16(a, 0, M, s_step);
+      }
+    }
+  }
+  if (splits > 1 && warp < 4) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+
+  // ---- teardown ----
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (splits > 1) cluster_sync();      // nobody writes here any more
+  if (warp == 2) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kFewTmem) : "memory");
+  }
+}
+
 // ---- host side --------------------------------------------------------------------------------------------------------------------------
+// How many clusters of `size` thread blocks of a kernel fit the device at once (cached per device by the caller).
+int resident_clusters(const void* kern, int size, int threads, int smem, int (&cached)[64]) {
+  static std::mutex mu;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  std::lock_guard<std::mutex> lock(mu);
+  if (cached[dev] == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(size);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {(unsigned)size, 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      n = 0;
+    }
+    cached[dev] = n + 1;
+  }
+  return cached[dev] - 1;
+}
+
+// Up to 16 rows: the kernel that quantizes on the way, if a thread block's codes fit beside a ring of weights and its threads have little to
+// quantize: four vectors of eight columns each, or eight if that is whole rows and no maxima are exchanged.  Measured against the
+// two launches: 4096 x 4096, 1 / 4 / 8 / 16 rows 7.9 / 9.0 / 10.6 / 12.9 us (10.7 / 10.7 / 10.9 / 11.8); 28672 x 4096, 1 / 4 rows 22.4 / 25.9
+// (26.2 / 25.2).  K is shared by as many thread blocks (4, 2) as keep every SM to one tile.
+struct FewPlan {
+  int splits, tiles, blocks, stages, units;      // splits 0: not this kernel
+};
+constexpr int kFewSmem = 216 * 1024;
+
+FewPlan few_plan(int M, int N, int K) {
+  FewPlan f{};
+  if (M > kFewRows || K % 8) return f;
+  const int ku = (K + kUnitK - 1) / kUnitK;
+  f.tiles = (N + kRows - 1) / kRows;
+  const void* kern = reinterpret_cast<const void*>(w8a8_few_kernel<__half>);
+  static int cached4[64] = {}, cached2[64] = {};
+  int splits = 1;
+  if (ku >= 8 && f.tiles <= sm_count() / 2 && ensure_smem_attr(kern, kFewSmem)) {
+    if (f.tiles <= resident_clusters(kern, 4, kFewThreads, kFewSmem, cached4)) splits = 4;
+    else if (f.tiles <= resident_clusters(kern, 2, kFewThreads, kFewSmem, cached2)) splits = 2;
+  }
+  f.units = (ku + splits - 1) / splits;
+  int per = kFewCodes;      // threads per row
+  for (int r = 1; r < M; r <<= 1) per >>= 1;
+  const int whole = (K / 8 + per - 1) / per, share = (f.units * (kUnitK / 8) + per - 1) / per;      // vectors of eight columns per thread
+  if (f.units > kFewMaxUnits || !(share <= kFewVecs / 2 || (splits > 1 && whole <= kFewVecs))) return f;
+  f.splits = splits;
+  f.blocks = splits > 1 ? f.tiles * splits : f.tiles < sm_count() ? f.tiles : sm_count();
+  f.stages = (kFewSmem - 1024 - f.units * kFewUnitBytes) / kWBytes;
+  if (f.stages > kMaxStages) f.stages = kMaxStages;
+  return f;
+}
+
 struct W8Plan {
   int mt, mtiles, ku, run, blocks, stages;
-  int splits;        // 0: one SM per tile (runs of units); 1, 2, 4: pairs of SMs
+  int splits;        // 0: one SM per tile (runs of units); 1, 2: pairs of SMs
   int tiles;         // weight tiles x activation tiles
   int64_t units;
 };
@@ -724,6 +1055,7 @@ W8Plan w8_plan(int M, int N, int K) {
   W8Plan best{};
   double least = 1e30;
   const int sms = sm_count(), ku = (K + kUnitK - 1) / kUnitK;
+  const double stream_us = (double)N * K / 6.0e6;       // the weights from memory
   int seen = 0;
   for (int target : {256, 192, 128, 96, 64, 32, 16}) {
     W8Plan g{};
@@ -735,11 +1067,11 @@ W8Plan w8_plan(int M, int N, int K) {
     g.ku = ku;
     g.tiles = (N + kRows - 1) / kRows * g.mtiles;
     g.units = (int64_t)g.tiles * g.ku;
-    const double unit_us = 0.15 + 0.0006 * g.mt;
+    const double unit_us = 0.19 + 0.0013 * g.mt;
     auto consider = [&](int64_t run) {
       if (run < 1 || (g.units + run - 1) / run > sms) return;
-      double cost = run * unit_us + 0.01 * g.mt;
-      if (run % g.ku) cost += 1.5 + 0.008 * g.mt * ((g.ku + run - 1) / run + (g.ku % run != 0));
+      double cost = std::max(run * unit_us, stream_us) + 0.01 * g.mt;
+      if (run % g.ku) cost += 2.5 + 0.02 * g.mt * ((g.ku + run - 1) / run + (g.ku % run != 0));
       if (cost < least - 1e-9) {
         least = cost;
         g.run = (int)run;
@@ -750,12 +1082,11 @@ W8Plan w8_plan(int M, int N, int K) {
     consider((g.units + sms - 1) / sms);
     for (int parts = 2; parts <= 16; ++parts) consider((g.ku + parts - 1) / parts);
   }
-  for (int target : {256, 192, 128, 96, 64}) {
-    for (int splits : {1, 2, 4}) {
+  for (int target : {256, 192, 160, 128, 96, 64, 32}) {
+    for (int splits : {1, 2}) {
       W8Plan g{};
-      const int grain = splits == 4 ? 64 : 32;
       g.mtiles = (M + target - 1) / target;
-      g.mt = ((M + g.mtiles - 1) / g.mtiles + grain - 1) / grain * grain;
+      g.mt = ((M + g.mtiles - 1) / g.mtiles + 31) / 32 * 32;
       g.mtiles = (M + g.mt - 1) / g.mt;
       g.ku = ku;
       g.splits = splits;
@@ -764,7 +1095,7 @@ W8Plan w8_plan(int M, int N, int K) {
       if (g.mt > 256 || splits > ku) continue;
       const int clusters = sms / (2 * splits), rounds = (g.tiles + clusters - 1) / clusters;
       if (splits > 1 && rounds > 1) continue;
-      const double cost = (double)rounds * ((ku + splits - 1) / splits) * (0.15 + 0.0005 * g.mt) + 0.01 * g.mt + 1.0 * (splits > 1);
+      const double cost = std::max((double)rounds * ((ku + splits - 1) / splits) * (0.2 + 0.00055 * g.mt), stream_us) + 0.01 * g.mt + 1.5 * (splits > 1);
       if (cost < least - 1e-9) {
         least = cost;
         best = g;
@@ -795,7 +1126,7 @@ struct W8Space {
     sums = step + up((size_t)M * 4);
     counters = sums + up((size_t)M * 4);
     partial = counters + up(((size_t)g.blocks + 1) * 4);
-    bytes = partial + (g.run % g.ku ? (size_t)g.blocks * 2 * g.mt * kRows * 4 : 0);
+    bytes = partial + (g.ku && g.run % g.ku ? (size_t)g.blocks * 2 * g.mt * kRows * 4 : 0);
   }
 };
 
@@ -807,7 +1138,7 @@ extern "C" {
 using namespace pare;
 
 size_t pare_w8a8_workspace_bytes(int M, int N, int K) {
-  if (M <= 0 || N <= 0 || K <= 0 || K > kMaxK) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || K > kMaxK || few_plan(M, N, K).splits) return 0;
   return W8Space(w8_plan(M, N, K), M, K).bytes;
 }
 
@@ -819,16 +1150,19 @@ int pare_w8a8_forward(const void* x, int x_dtype, int64_t ldx, const int8_t* wei
   PARE_REQUIRE(x && weight && scale && y, PARE_ERR_SHAPE);
   PARE_REQUIRE(K <= kMaxK, PARE_ERR_UNSUPPORTED);
   PARE_REQUIRE(aligned16(weight) && ldw % 16 == 0 && aligned16(workspace), PARE_ERR_ALIGN);
-  const W8Plan g = w8_plan(M, N, K);
-  PARE_REQUIRE(g.units + g.run < (int64_t)1 << 31, PARE_ERR_UNSUPPORTED);
+  const FewPlan f = few_plan(M, N, K);
+  const W8Plan g = f.splits ? W8Plan{} : w8_plan(M, N, K);
   const W8Space sp(g, M, K);
-  PARE_REQUIRE(workspace && workspace_bytes >= sp.bytes, PARE_ERR_WORKSPACE);
-  unsigned char* ws = reinterpret_cast<unsigned char*>(workspace);
+  if (f.splits) {
+    PARE_REQUIRE(aligned16(x) && (M == 1 || ldx % 8 == 0), PARE_ERR_ALIGN);
+  } else {
+    PARE_REQUIRE(g.units + g.run < (int64_t)1 << 31, PARE_ERR_UNSUPPORTED);
+    PARE_REQUIRE(workspace && workspace_bytes >= sp.bytes, PARE_ERR_WORKSPACE);
+  }
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   EncodeTiledFn enc = encode_fn();
   PARE_REQUIRE(enc != nullptr, PARE_ERR_CUDA);
-
-  // tensor maps: both operands in rows of K bytes, boxes of 128 bytes, 128B swizzle; rows and columns beyond the end read as zeros
+  // tensor maps: operands in rows of K bytes, boxes of 128 bytes, 128B swizzle; rows and columns beyond the end read as zeros
   auto map = [&](CUtensorMap* tm, const void* base, int rows, int64_t pitch, int box_rows) {
     const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
     const cuuint64_t strides[1] = {(cuuint64_t)pitch};
@@ -837,7 +1171,44 @@ int pare_w8a8_forward(const void* x, int x_dtype, int64_t ldx, const int8_t* wei
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
   };
   CUtensorMap tw, tx;
-  PARE_REQUIRE(map(&tw, weight, N, ldw, kRows) && map(&tx, ws + sp.codes, M, sp.ldc, g.splits ? g.mt / 2 : g.mt), PARE_ERR_CUDA);
+  PARE_REQUIRE(map(&tw, weight, N, ldw, kRows), PARE_ERR_CUDA);
+  // with programmatic launch, and in clusters
+  auto launch = [&](auto kern, int blocks, int threads, size_t smem, int cluster, auto... args) -> int {
+    if (!ensure_smem_attr(reinterpret_cast<const void*>(kern), threads == kFewThreads ? kFewSmem : kMaxSmem)) return PARE_ERR_CUDA;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim = {(unsigned)cluster, 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess ? launch_status() : (int)PARE_ERR_CUDA;
+  };
+  W8Params p{};
+  p.scale = scale;
+  p.zero = zero;
+  p.bias = bias;
+  p.y = y;
+  p.ldy = ldy;
+  p.M = M;
+  p.N = N;
+  p.ku = (K + kUnitK - 1) / kUnitK;
+
+  if (f.splits) {
+    p.stages = f.stages;
+    const FewParams fp{p, x, ldx, input_scale, K, f.tiles, f.splits};
+    const size_t smem = 1024 + (size_t)f.stages * kWBytes + (size_t)f.units * kFewUnitBytes;
+    return x_dtype == PARE_F16 ? launch(w8a8_few_kernel<__half>, f.blocks, kFewThreads, smem, f.splits, tw, fp)
+                               : launch(w8a8_few_kernel<__nv_bfloat16>, f.blocks, kFewThreads, smem, f.splits, tw, fp);
+  }
+
+  unsigned char* ws = reinterpret_cast<unsigned char*>(workspace);
+  PARE_REQUIRE(map(&tx, ws + sp.codes, M, sp.ldc, g.splits ? g.mt / 2 : g.mt), PARE_ERR_CUDA);
 
   const QuantParams q{x, ldx, input_scale, reinterpret_cast<int8_t*>(ws + sp.codes), sp.ldc, reinterpret_cast<float*>(ws + sp.step),
                       reinterpret_cast<int*>(ws + sp.sums), reinterpret_cast<int*>(ws + sp.counters), g.blocks + 1, K};
@@ -859,45 +1230,23 @@ int pare_w8a8_forward(const void* x, int x_dtype, int64_t ldx, const int8_t* wei
   else quantize(__nv_bfloat16());
   if (cudaGetLastError() != cudaSuccess) return PARE_ERR_CUDA;
 
-  W8Params p{};
   p.step = q.step;
   p.sums = q.sums;
-  p.scale = scale;
-  p.zero = zero;
-  p.bias = bias;
-  p.y = y;
-  p.ldy = ldy;
-  p.M = M;
-  p.N = N;
   p.mt = g.mt;
   p.mtiles = g.mtiles;
-  p.ku = g.ku;
   p.total_units = (int)g.units;
   p.run_units = g.run;
   p.stages = g.stages;
   p.partial = reinterpret_cast<int*>(ws + sp.partial);
   p.counters = q.zeroed;
   const size_t smem = 1024 + (size_t)g.stages * (kWBytes + (g.splits ? g.mt / 2 : g.mt) * kUnitK) + 512;
-  auto launch = [&](auto kern, const auto& params, int cluster) -> int {
-    if (!ensure_smem_attr(reinterpret_cast<const void*>(kern), kMaxSmem)) return PARE_ERR_CUDA;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(g.blocks);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim = {(unsigned)cluster, 1, 1};
-    cfg.attrs = attr;
-    cfg.numAttrs = cluster > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kern, tw, tx, params) == cudaSuccess ? launch_status() : (int)PARE_ERR_CUDA;
-  };
   const bool half = x_dtype == PARE_F16;
-  if (g.splits == 0) return half ? launch(w8a8_gemm_kernel<__half>, p, 1) : launch(w8a8_gemm_kernel<__nv_bfloat16>, p, 1);
+  if (g.splits == 0)
+    return half ? launch(w8a8_gemm_kernel<__half>, g.blocks, kThreads, smem, 1, tw, tx, p)
+                : launch(w8a8_gemm_kernel<__nv_bfloat16>, g.blocks, kThreads, smem, 1, tw, tx, p);
   const PairParams pp{p, g.tiles, g.splits};
-  return half ? launch(w8a8_pair_kernel<__half>, pp, 2 * g.splits) : launch(w8a8_pair_kernel<__nv_bfloat16>, pp, 2 * g.splits);
+  return half ? launch(w8a8_pair_kernel<__half>, g.blocks, kThreads, smem, 2 * g.splits, tw, tx, pp)
+              : launch(w8a8_pair_kernel<__nv_bfloat16>, g.blocks, kThreads, smem, 2 * g.splits, tw, tx, pp);
 }
 
 }  // extern "C"

@@ -66,15 +66,17 @@ def w8a8_forward(x: Tensor, q_weight: Tensor, scale: Tensor, zero: Tensor | None
         return out
     if x.stride(1) != 1 or (m > 1 and x.stride(0) < k):
         x = x.contiguous()
+    if m <= 16 and k % 8 == 0 and (x.data_ptr() % 16 or (m > 1 and x.stride(0) % 8)):     # a few rows are read in 16-byte pieces
+        x = x.clone(memory_format=torch.contiguous_format)
     ldw = q_weight.stride(0) if n > 1 else -(-k // 16) * 16
     if q_weight.stride(1) != 1 or ldw < k or ldw % 16 or q_weight.data_ptr() % 16:
         q_weight = aligned_rows(q_weight)
         ldw = q_weight.stride(0)
     # from the allocator for each call: it belongs to this call's stream, or to the graph that captures it
     nbytes = _workspace_bytes(m, n, k, dev.index)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     args = (x.data_ptr(), 0 if dtype is torch.float16 else 1, x.stride(0) if m > 1 else k, q_weight.data_ptr(), ldw, s, z, i, _lib.ptr(bias),
-            out.data_ptr(), out.stride(0) if m > 1 else n, m, n, k, ws.data_ptr(), nbytes)
+            out.data_ptr(), out.stride(0) if m > 1 else n, m, n, k, _lib.ptr(ws), nbytes)
     if dev.index == _lib.current_device():
         status = _lib.lib().pare_w8a8_forward(*args, _lib.current_stream(dev))
     else:

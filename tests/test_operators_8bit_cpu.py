@@ -98,15 +98,22 @@ def test_c_entries_refuse():
         return L.pare_w8a8_forward(x, dtype, ldx, w, ldw, p, None, None, None, p, ldy, M, N, K, ws, size, None)
     assert linear(M=0) == linear(N=0) == linear(K=0) == linear(ldw=16) == linear(ldx=31) == linear(ldy=3) == linear(x=None) == SHAPE
     assert linear(dtype=2) == DTYPE and linear(K=65537, ldx=70000, ldw=70000) == UNSUPPORTED
-    assert linear(w=p + 8) == linear(ldw=40) == linear(ws=p + 4) == ALIGN and linear(size=8) == linear(ws=None) == SPACE
+    assert linear(w=p + 8) == linear(ldw=40) == linear(ws=p + 4) == linear(x=p + 2) == linear(ldx=36) == ALIGN
+    assert linear(M=20, size=8) == linear(M=20, ws=None) == SPACE
     assert L.pare_w8a8_workspace_bytes(0, 1, 1) == L.pare_w8a8_workspace_bytes(1, 1, 65537) == 0
     del buf
 
 
 def test_workspace_covers_the_codes():
     L = _lib.lib()
-    for m, n, k in ((1, 1, 1), (17, 4096, 4096), (333, 3584, 18944), (5000, 100, 65536)):
+    for m, n, k in ((1, 1, 1), (3, 5, 4097), (17, 4096, 4096), (333, 3584, 18944), (5000, 100, 65536)):
         assert L.pare_w8a8_workspace_bytes(m, n, k) >= m * k + 8 * m
+
+
+def test_a_few_rows_need_no_workspace():
+    L = _lib.lib()
+    assert all(L.pare_w8a8_workspace_bytes(m, n, k) == 0 for m in (1, 2) for n, k in ((1, 8), (4096, 4096), (28672, 4096)))
+    assert L.pare_w8a8_workspace_bytes(1, 60000, 65536) > 0      # too long a row to keep its codes beside the weights
 
 
 def test_aligned_rows():
