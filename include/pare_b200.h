@@ -347,6 +347,21 @@ enum {
   PARE_PAGED_TABLE = 4,      /* a request would not fit its row of block_table */
   PARE_PAGED_BLOCKS = 8      /* not enough free blocks (or free_count out of range) */
 };
+typedef struct {             /* one layer (a host struct of device pointers, all 16-byte aligned) */
+  int8_t* k_codes;
+  int8_t* v_codes;
+  float* k_scale;
+  float* v_scale;
+  void* tail_k;
+  void* tail_v;
+  int num_blocks, R, H, block_size, D, dtype;   /* dtype of the open rows, and of q, k, v: F16 or BF16 */
+} pare_paged_layer;
+typedef struct {             /* a planned step (a host struct of device pointers) */
+  const void* step;
+  const int32_t* block_table;
+  int64_t ld_table;
+  int max_blocks, R, T, block_size;
+} pare_paged_tables;
 size_t pare_paged_step_bytes(int R, int T, int block_size);
 int64_t pare_paged_step_offset(int field, int R, int T, int block_size);
 int pare_paged_plan(const int32_t* seq_lens, const int32_t* new_lens, int R, int32_t* block_table, int64_t ld_table, int max_blocks,
@@ -359,28 +374,20 @@ int pare_paged_release(const int32_t* release, int32_t* seq_lens, int R, const i
 
 /* The step's new keys and values [T][H][D] (element strides, multiples of 8; channels contiguous; 16-byte aligned) into one layer.
  * Ids that are not in the pool are not written to. */
-int pare_paged_append(const void* k, const void* v, int dtype, int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t,
-                      int64_t v_stride_h, const void* step, int R, int T, int block_size,
-                      int8_t* k_codes, int8_t* v_codes, float* k_scale, float* v_scale, void* tail_k, void* tail_v,
-                      int num_blocks, int H, int D, void* stream);
+int pare_paged_append(const void* k, const void* v, int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h,
+                      const pare_paged_layer* layer, const pare_paged_tables* tables, void* stream);
 
 /* Keys and values, after the step, of every request with new tokens in it: out_k / out_v [total][H][D] dense, request r's from row
  * context_start[r] on; rows behind the last are zeros, rows beyond `total` are left out.  Ids not in the pool read as NaN. */
-int pare_paged_dense(const void* step, int R, int T, int block_size, const int32_t* block_table, int64_t ld_table, int max_blocks,
-                     const int8_t* k_codes, const int8_t* v_codes, const float* k_scale, const float* v_scale,
-                     const void* tail_k, const void* tail_v, int num_blocks, int H, int D,
-                     void* out_k, void* out_v, int dtype, int64_t total, void* stream);
+int pare_paged_dense(const pare_paged_layer* layer, const pare_paged_tables* tables, void* out_k, void* out_v, int64_t total, void* stream);
 
 /* Attention of the step's tokens over the layer, after the step's append: token t of request r attends to the positions up to its
  * own.  q, out [T][Hq][D] (element strides; q's multiples of 8, 16-byte aligned), query head hq reads KV head hq / (Hq / H), any
  * ratio; T <= 4096.  Rows that belong to nobody are left as they were.  Ids not in the pool read as NaN.  The workspace
  * (16-byte aligned, pare_paged_attn_workspace_bytes()) need not be initialised and holds nothing between calls. */
 size_t pare_paged_attn_workspace_bytes(int D);
-int pare_paged_attn(const void* q, int dtype, int64_t q_stride_t, int64_t q_stride_h, const void* step, int R, int T, int block_size,
-                    const int32_t* block_table, int64_t ld_table, int max_blocks,
-                    const int8_t* k_codes, const int8_t* v_codes, const float* k_scale, const float* v_scale,
-                    const void* tail_k, const void* tail_v, int num_blocks, int Hq, int H, int D,
-                    void* out, int64_t out_stride_t, int64_t out_stride_h, float softmax_scale,
+int pare_paged_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h, const pare_paged_layer* layer, const pare_paged_tables* tables,
+                    int Hq, void* out, int64_t out_stride_t, int64_t out_stride_h, float softmax_scale,
                     void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------

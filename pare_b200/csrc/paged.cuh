@@ -43,5 +43,16 @@ struct StepLayout {
   }
 };
 
+// What append, dense and attention ask of their layer and step
+inline int check(const pare_paged_layer* l, const pare_paged_tables* t) {
+  PARE_REQUIRE(l && t && t->step && t->block_table && l->k_codes && l->v_codes && l->k_scale && l->v_scale && l->tail_k && l->tail_v, PARE_ERR_SHAPE);
+  PARE_REQUIRE(t->R > 0 && t->R <= kMaxRequests && t->T >= 0 && t->T <= kMaxTokens && t->max_blocks > 0 && t->ld_table >= t->max_blocks, PARE_ERR_SHAPE);
+  PARE_REQUIRE(l->num_blocks > 0 && l->H > 0 && l->H <= 65535 && l->R == t->R && l->block_size == t->block_size, PARE_ERR_SHAPE);
+  PARE_REQUIRE(l->dtype == PARE_F16 || l->dtype == PARE_BF16, PARE_ERR_DTYPE);
+  PARE_REQUIRE(block_size_ok(l->block_size) && (l->D == 64 || l->D == 128), PARE_ERR_UNSUPPORTED);
+  PARE_REQUIRE(aligned16(t->step) && aligned16(l->k_codes) && aligned16(l->v_codes) && aligned16(l->tail_k) && aligned16(l->tail_v), PARE_ERR_ALIGN);
+  return PARE_OK;
+}
+
 }  // namespace paged
 }  // namespace pare

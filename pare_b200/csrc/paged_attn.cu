@@ -573,6 +573,7 @@ __global__ void __launch_bounds__(GROUPS > 1 ? GROUPS * 32 : D * 2) paged_merge_
 }
 
 int attn_blocks() { return 2 * sm_count(); }
+size_t workspace_of(int D, int blocks) { return (size_t)blocks * kWarps * 2 * (kHeads * D + 2 * kHeads) * sizeof(float); }
 
 }  // namespace
 }  // namespace pare
@@ -584,51 +585,46 @@ using namespace pare::paged;
 
 size_t pare_paged_attn_workspace_bytes(int D) {
   if (D != 64 && D != 128) return 0;
-  return (size_t)attn_blocks() * kWarps * 2 * (kHeads * D + 2 * kHeads) * sizeof(float);
+  return workspace_of(D, attn_blocks());
 }
 
-int pare_paged_attn(const void* q, int dtype, int64_t q_stride_t, int64_t q_stride_h, const void* step, int R, int T, int block_size,
-                    const int32_t* block_table, int64_t ld_table, int max_blocks, const int8_t* k_codes, const int8_t* v_codes,
-                    const float* k_scale, const float* v_scale, const void* tail_k, const void* tail_v, int num_blocks, int Hq, int H,
-                    int D, void* out, int64_t out_stride_t, int64_t out_stride_h, float softmax_scale, void* workspace,
-                    size_t workspace_bytes, void* stream) {
-  PARE_REQUIRE(step && block_table && k_codes && v_codes && k_scale && v_scale && tail_k && tail_v, PARE_ERR_SHAPE);
-  PARE_REQUIRE(R > 0 && R <= kMaxRequests && T >= 0 && num_blocks > 0 && H > 0 && Hq > 0 && Hq % H == 0 && max_blocks > 0 &&
-                   ld_table >= max_blocks,
-               PARE_ERR_SHAPE);
-  PARE_REQUIRE(dtype == PARE_F16 || dtype == PARE_BF16, PARE_ERR_DTYPE);
-  PARE_REQUIRE(block_size_ok(block_size) && (D == 64 || D == 128) && T <= kMaxQueryTokens, PARE_ERR_UNSUPPORTED);
+int pare_paged_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h, const pare_paged_layer* l, const pare_paged_tables* tb, int Hq,
+                    void* out, int64_t out_stride_t, int64_t out_stride_h, float softmax_scale, void* workspace, size_t workspace_bytes,
+                    void* stream) {
+  const int rc = check(l, tb);
+  if (rc != PARE_OK) return rc;
+  const int T = tb->T, H = l->H, D = l->D;
+  PARE_REQUIRE(Hq > 0 && Hq % H == 0, PARE_ERR_SHAPE);
+  PARE_REQUIRE(T <= kMaxQueryTokens, PARE_ERR_UNSUPPORTED);
   if (T == 0) return PARE_OK;
   PARE_REQUIRE(q && out, PARE_ERR_SHAPE);
-  PARE_REQUIRE(aligned16(q) && (q_stride_t | q_stride_h) % 8 == 0 && aligned16(step) && aligned16(k_codes) && aligned16(v_codes) &&
-                   aligned16(tail_k) && aligned16(tail_v) && aligned16(workspace),
-               PARE_ERR_ALIGN);
-  PARE_REQUIRE(workspace && workspace_bytes >= pare_paged_attn_workspace_bytes(D), PARE_ERR_WORKSPACE);
+  PARE_REQUIRE(aligned16(q) && (q_stride_t | q_stride_h) % 8 == 0 && aligned16(workspace), PARE_ERR_ALIGN);
+  const int blocks = attn_blocks();
+  PARE_REQUIRE(workspace && workspace_bytes >= workspace_of(D, blocks), PARE_ERR_WORKSPACE);
   const int group = Hq / H, sub = (group + kHeads - 1) / kHeads;
   PARE_REQUIRE((int64_t)T * H * sub < (int64_t)1 << 31, PARE_ERR_UNSUPPORTED);
-  const StepLayout s(R, T, block_size);
-  const int* w = reinterpret_cast<const int*>(step);
-  const int blocks = attn_blocks();
-  PagedAttnParams p{q, q_stride_t, q_stride_h, out, out_stride_t, out_stride_h, reinterpret_cast<const int4*>(w + s.info),
-                    w + s.unit_start, block_table, ld_table, k_codes, v_codes, k_scale, v_scale, tail_k, tail_v,
-                    reinterpret_cast<float*>(workspace), softmax_scale * kLog2e, T, R, H, group, sub,
-                    block_size == 16 ? 4 : block_size == 32 ? 5 : 6, num_blocks, max_blocks};
+  const StepLayout s(tb->R, T, l->block_size);
+  const int* w = reinterpret_cast<const int*>(tb->step);
+  const PagedAttnParams p{q, q_stride_t, q_stride_h, out, out_stride_t, out_stride_h, reinterpret_cast<const int4*>(w + s.info),
+                          w + s.unit_start, tb->block_table, tb->ld_table, l->k_codes, l->v_codes, l->k_scale, l->v_scale, l->tail_k, l->tail_v,
+                          reinterpret_cast<float*>(workspace), softmax_scale * kLog2e, T, tb->R, H, group, sub,
+                          l->block_size == 16 ? 4 : l->block_size == 32 ? 5 : 6, l->num_blocks, tb->max_blocks};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   auto go = [&](auto kern, auto merge, auto merge_few, size_t smem) {
     if (!ensure_smem_attr(reinterpret_cast<const void*>(kern), (int)smem)) return (int)PARE_ERR_CUDA;
-    int rc = launch_pdl(kern, dim3(blocks), dim3(kThreads), smem, st, p);
-    if (rc != PARE_OK) return rc;
-    const int jobs = T * H * sub, most = 32 * sm_count();
-    rc = jobs <= sm_count() ? launch_pdl(merge_few, dim3(jobs, D / 16), dim3(kMergeGroups * 32), 0, st, p, blocks * kWarps)
+    int status = launch_pdl(kern, dim3(blocks), dim3(kThreads), smem, st, p);
+    if (status != PARE_OK) return status;
+    const int jobs = T * H * sub, most = 16 * blocks;
+    status = 2 * jobs <= blocks ? launch_pdl(merge_few, dim3(jobs, D / 16), dim3(kMergeGroups * 32), 0, st, p, blocks * kWarps)
                             : launch_pdl(merge, dim3(jobs < most ? jobs : most), dim3(D * 2), 0, st, p, blocks * kWarps);
-    return rc != PARE_OK ? rc : launch_status();
+    return status != PARE_OK ? status : launch_status();
   };
   auto by_dim = [&](auto tag) {
     using E = decltype(tag);
     return D == 64 ? go(paged_attn_kernel<E, 64>, paged_merge_kernel<E, 64, 1>, paged_merge_kernel<E, 64, kMergeGroups>, Shape<64>::kSmem)
                    : go(paged_attn_kernel<E, 128>, paged_merge_kernel<E, 128, 1>, paged_merge_kernel<E, 128, kMergeGroups>, Shape<128>::kSmem);
   };
-  return dtype == PARE_F16 ? by_dim(__half()) : by_dim(__nv_bfloat16());
+  return l->dtype == PARE_F16 ? by_dim(__half()) : by_dim(__nv_bfloat16());
 }
 
 }  // extern "C"

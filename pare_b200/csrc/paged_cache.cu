@@ -431,22 +431,16 @@ int pare_paged_release(const int32_t* release, int32_t* seq_lens, int R, const i
   return launch_status();
 }
 
-int pare_paged_append(const void* k, const void* v, int dtype, int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t,
-                      int64_t v_stride_h, const void* step, int R, int T, int block_size, int8_t* k_codes, int8_t* v_codes,
-                      float* k_scale, float* v_scale, void* tail_k, void* tail_v, int num_blocks, int H, int D, void* stream) {
-  PARE_REQUIRE(step && k_codes && v_codes && k_scale && v_scale && tail_k && tail_v, PARE_ERR_SHAPE);
-  PARE_REQUIRE(R > 0 && R <= kMaxRequests && T >= 0 && T <= kMaxTokens && num_blocks > 0 && H > 0 && H <= 65535, PARE_ERR_SHAPE);
-  PARE_REQUIRE(dtype == PARE_F16 || dtype == PARE_BF16, PARE_ERR_DTYPE);
-  PARE_REQUIRE(block_size_ok(block_size) && (D == 64 || D == 128), PARE_ERR_UNSUPPORTED);
-  if (T == 0) return PARE_OK;
+int pare_paged_append(const void* k, const void* v, int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h,
+                      const pare_paged_layer* l, const pare_paged_tables* t, void* stream) {
+  const int rc = check(l, t);
+  if (rc != PARE_OK || t->T == 0) return rc;
   PARE_REQUIRE(k && v, PARE_ERR_SHAPE);
-  PARE_REQUIRE(aligned16(k) && aligned16(v) && (k_stride_t | k_stride_h | v_stride_t | v_stride_h) % 8 == 0 && aligned16(step) &&
-                   aligned16(k_codes) && aligned16(v_codes) && aligned16(tail_k) && aligned16(tail_v),
-               PARE_ERR_ALIGN);
-  const StepLayout s(R, T, block_size);
-  AppendParams p{k, v, k_stride_t, k_stride_h, v_stride_t, v_stride_h, reinterpret_cast<const int*>(step) + s.items,
-                 k_codes, v_codes, k_scale, v_scale, tail_k, tail_v, H, num_blocks, R, T};
-  const dim3 grid(s.n_items, H);
+  PARE_REQUIRE(aligned16(k) && aligned16(v) && (k_stride_t | k_stride_h | v_stride_t | v_stride_h) % 8 == 0, PARE_ERR_ALIGN);
+  const StepLayout s(t->R, t->T, t->block_size);
+  const AppendParams p{k, v, k_stride_t, k_stride_h, v_stride_t, v_stride_h, reinterpret_cast<const int*>(t->step) + s.items,
+                       l->k_codes, l->v_codes, l->k_scale, l->v_scale, l->tail_k, l->tail_v, l->H, l->num_blocks, l->R, t->T};
+  const dim3 grid(s.n_items, l->H);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   auto go = [&](auto kern) {
     kern<<<grid, kAppendThreads, 0, st>>>(p);
@@ -454,39 +448,33 @@ int pare_paged_append(const void* k, const void* v, int dtype, int64_t k_stride_
   };
   auto by_size = [&](auto tag) {
     using E = decltype(tag);
-    if (D == 64) return block_size == 16 ? go(paged_append_kernel<E, 64, 16>) : block_size == 32 ? go(paged_append_kernel<E, 64, 32>) : go(paged_append_kernel<E, 64, 64>);
-    return block_size == 16 ? go(paged_append_kernel<E, 128, 16>) : block_size == 32 ? go(paged_append_kernel<E, 128, 32>) : go(paged_append_kernel<E, 128, 64>);
+    const int bs = l->block_size;
+    if (l->D == 64) return bs == 16 ? go(paged_append_kernel<E, 64, 16>) : bs == 32 ? go(paged_append_kernel<E, 64, 32>) : go(paged_append_kernel<E, 64, 64>);
+    return bs == 16 ? go(paged_append_kernel<E, 128, 16>) : bs == 32 ? go(paged_append_kernel<E, 128, 32>) : go(paged_append_kernel<E, 128, 64>);
   };
-  return dtype == PARE_F16 ? by_size(__half()) : by_size(__nv_bfloat16());
+  return l->dtype == PARE_F16 ? by_size(__half()) : by_size(__nv_bfloat16());
 }
 
-int pare_paged_dense(const void* step, int R, int T, int block_size, const int32_t* block_table, int64_t ld_table, int max_blocks,
-                     const int8_t* k_codes, const int8_t* v_codes, const float* k_scale, const float* v_scale, const void* tail_k,
-                     const void* tail_v, int num_blocks, int H, int D, void* out_k, void* out_v, int dtype, int64_t total, void* stream) {
-  PARE_REQUIRE(step && block_table && k_codes && v_codes && k_scale && v_scale && tail_k && tail_v, PARE_ERR_SHAPE);
-  PARE_REQUIRE(R > 0 && R <= kMaxRequests && T >= 0 && T <= kMaxTokens && num_blocks > 0 && H > 0 && max_blocks > 0 &&
-                   ld_table >= max_blocks && total >= 0 && total < (int64_t)1 << 35,
-               PARE_ERR_SHAPE);
-  PARE_REQUIRE(dtype == PARE_F16 || dtype == PARE_BF16, PARE_ERR_DTYPE);
-  PARE_REQUIRE(block_size_ok(block_size) && (D == 64 || D == 128), PARE_ERR_UNSUPPORTED);
+int pare_paged_dense(const pare_paged_layer* l, const pare_paged_tables* t, void* out_k, void* out_v, int64_t total, void* stream) {
+  const int rc = check(l, t);
+  if (rc != PARE_OK) return rc;
+  PARE_REQUIRE(total >= 0 && total < (int64_t)1 << 35, PARE_ERR_SHAPE);
   if (total == 0) return PARE_OK;
   PARE_REQUIRE(out_k && out_v, PARE_ERR_SHAPE);
-  PARE_REQUIRE(aligned16(out_k) && aligned16(out_v) && aligned16(k_codes) && aligned16(v_codes) && aligned16(tail_k) && aligned16(tail_v),
-               PARE_ERR_ALIGN);
-  const StepLayout s(R, T, block_size);
-  const int* w = reinterpret_cast<const int*>(step);
-  DenseParams p{reinterpret_cast<const long long*>(w + s.context_start), w + s.seq_lens, block_table, ld_table, k_codes, v_codes, k_scale,
-                v_scale, tail_k, tail_v, out_k, out_v, total, R, H, log2_of(block_size), num_blocks, max_blocks};
+  PARE_REQUIRE(aligned16(out_k) && aligned16(out_v), PARE_ERR_ALIGN);
+  const StepLayout s(t->R, t->T, t->block_size);
+  const int* w = reinterpret_cast<const int*>(t->step);
+  const DenseParams p{reinterpret_cast<const long long*>(w + s.context_start), w + s.seq_lens, t->block_table, t->ld_table, l->k_codes,
+                      l->v_codes, l->k_scale, l->v_scale, l->tail_k, l->tail_v, out_k, out_v, total, t->R, l->H, log2_of(l->block_size),
+                      l->num_blocks, t->max_blocks};
   const unsigned grid = (unsigned)((total + kDenseTokens - 1) / kDenseTokens);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == PARE_F16) {
-    if (D == 64) paged_dense_kernel<__half, 64><<<grid, kDenseThreads, 0, st>>>(p);
-    else paged_dense_kernel<__half, 128><<<grid, kDenseThreads, 0, st>>>(p);
-  } else {
-    if (D == 64) paged_dense_kernel<__nv_bfloat16, 64><<<grid, kDenseThreads, 0, st>>>(p);
-    else paged_dense_kernel<__nv_bfloat16, 128><<<grid, kDenseThreads, 0, st>>>(p);
-  }
-  return launch_status();
+  auto go = [&](auto kern) {
+    kern<<<grid, kDenseThreads, 0, st>>>(p);
+    return launch_status();
+  };
+  if (l->dtype == PARE_F16) return l->D == 64 ? go(paged_dense_kernel<__half, 64>) : go(paged_dense_kernel<__half, 128>);
+  return l->D == 64 ? go(paged_dense_kernel<__nv_bfloat16, 64>) : go(paged_dense_kernel<__nv_bfloat16, 128>);
 }
 
 }  // extern "C"

@@ -26,6 +26,19 @@ _lib: C.CDLL | None = None
 
 _vp, _i, _i64, _sz = C.c_void_p, C.c_int, C.c_int64, C.c_size_t
 
+class PagedLayerStruct(C.Structure):
+    """``pare_paged_layer``."""
+
+    _fields_ = [(n, _vp) for n in ("k_codes", "v_codes", "k_scale", "v_scale", "tail_k", "tail_v")] + [
+        (n, _i) for n in ("num_blocks", "requests", "heads", "block_size", "head_dim", "dtype")]
+
+
+class PagedTablesStruct(C.Structure):
+    """``pare_paged_tables``."""
+
+    _fields_ = [("step", _vp), ("block_table", _vp), ("ld_table", _i64)] + [(n, _i) for n in ("max_blocks", "requests", "tokens", "block_size")]
+
+
 # name -> (restype, argtypes); kept in the order of the header
 SIGNATURES: dict[str, tuple] = {
     "pare_version": (_i, []),
@@ -80,13 +93,10 @@ SIGNATURES: dict[str, tuple] = {
     "pare_paged_step_offset": (_i64, [_i, _i, _i, _i]),
     "pare_paged_plan": (_i, [_vp, _vp, _i, _vp, _i64, _i, _vp, _i, _vp, _i, _i, _vp, _sz, _vp]),
     "pare_paged_release": (_i, [_vp, _vp, _i, _vp, _i64, _i, _vp, _i, _vp, _i, _vp]),
-    "pare_paged_append": (_i, [_vp, _vp, _i, _i64, _i64, _i64, _i64, _vp, _i, _i, _i,
-                               _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
-    "pare_paged_dense": (_i, [_vp, _i, _i, _i, _vp, _i64, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i,
-                              _vp, _vp, _i, _i64, _vp]),
+    "pare_paged_append": (_i, [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "pare_paged_dense": (_i, [_vp, _vp, _vp, _vp, _i64, _vp]),
     "pare_paged_attn_workspace_bytes": (_sz, [_i]),
-    "pare_paged_attn": (_i, [_vp, _i, _i64, _i64, _vp, _i, _i, _i, _vp, _i64, _i, _vp, _vp, _vp, _vp, _vp, _vp,
-                             _i, _i, _i, _i, _vp, _i64, _i64, C.c_float, _vp, _sz, _vp]),
+    "pare_paged_attn": (_i, [_vp, _i64, _i64, _vp, _vp, _i, _vp, _i64, _i64, C.c_float, _vp, _sz, _vp]),
     "pare_w4a16_static_status": (_i, [_vp]),
     "pare_w4a16_static_scratch_bytes": (_sz, []),
     "pare_w4a16_forward_static": (_i, [_vp, _i, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64,
@@ -186,6 +196,22 @@ def workspace_status(device: torch.device) -> int:
     if buf is None:
         return 0
     return lib().pare_workspace_status(buf.data_ptr(), key[1])
+
+
+# Scratch memory that calls leave nothing in, one per device and stream.  Graphs never work in it: see scratch().
+_scratch: dict[tuple[int, int], torch.Tensor] = {}
+
+
+def scratch(device: torch.device, nbytes: int, stream: int) -> torch.Tensor:
+    """Memory for one call on the current stream of ``device``, which must be the current device.  Calls on a stream follow one
+    another, so they share it; while a graph is captured it comes from the allocator, i.e. belongs to that graph."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    key = (device.index, stream)
+    buf = _scratch.get(key)
+    if buf is None or buf.numel() < nbytes:
+        _scratch[key] = buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return buf
 
 
 def workspace(device: torch.device, nbytes: int, stream: int | None = None) -> torch.Tensor:

@@ -59,7 +59,7 @@ def w8a8_forward(x: Tensor, q_weight: Tensor, scale: Tensor, zero: Tensor | None
         if bias.dtype is not dtype or not bias.is_contiguous():
             bias = bias.to(dtype).contiguous()
     if out is None:
-        out = torch.empty(m, n, device=dev, dtype=dtype)
+        out = x.new_empty(m, n)
     elif out.shape != (m, n) or out.dtype is not dtype or out.device != dev or out.stride(1) != 1 or (m > 1 and out.stride(0) < n):
         raise ValueError(f"out must be {dtype} [{m}, {n}] on {dev} with adjacent columns")
     if m == 0:
@@ -72,16 +72,14 @@ def w8a8_forward(x: Tensor, q_weight: Tensor, scale: Tensor, zero: Tensor | None
     if q_weight.stride(1) != 1 or ldw < k or ldw % 16 or q_weight.data_ptr() % 16:
         q_weight = aligned_rows(q_weight)
         ldw = q_weight.stride(0)
-    # from the allocator for each call: it belongs to this call's stream, or to the graph that captures it
-    nbytes = _workspace_bytes(m, n, k, dev.index)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    args = (x.data_ptr(), 0 if dtype is torch.float16 else 1, x.stride(0) if m > 1 else k, q_weight.data_ptr(), ldw, s, z, i, _lib.ptr(bias),
-            out.data_ptr(), out.stride(0) if m > 1 else n, m, n, k, _lib.ptr(ws), nbytes)
-    if dev.index == _lib.current_device():
-        status = _lib.lib().pare_w8a8_forward(*args, _lib.current_stream(dev))
-    else:
+    if dev.index != _lib.current_device():
         with torch.cuda.device(dev):
-            status = _lib.lib().pare_w8a8_forward(*args, _lib.current_stream(dev))
+            return w8a8_forward(x, q_weight, scale, zero, bias=bias, input_scale=input_scale, out=out)
+    stream, nbytes = _lib.current_stream(dev), _workspace_bytes(m, n, k, dev.index)
+    ws = _lib.scratch(dev, nbytes, stream).data_ptr() if nbytes else None
+    status = _lib.lib().pare_w8a8_forward(
+        x.data_ptr(), 0 if dtype is torch.float16 else 1, x.stride(0) if m > 1 else k, q_weight.data_ptr(), ldw, s, z, i, _lib.ptr(bias),
+        out.data_ptr(), out.stride(0) if m > 1 else n, m, n, k, ws, nbytes, stream)
     if status:
         _lib.check(status, "pare_w8a8_forward")
     return out

@@ -20,6 +20,7 @@ Nothing here computes gradients, and everything runs on CUDA tensors only.
 
 from __future__ import annotations
 
+import ctypes
 import functools
 import math
 from dataclasses import dataclass
@@ -39,16 +40,41 @@ _REFUSED = {1: "a length or number of new tokens is negative", 2: "more new toke
             4: "a request would not fit its row of the block table", 8: "not enough free blocks"}
 
 
-class PagedLayer(NamedTuple):
-    """One layer's storage: codes int8 ``[num_blocks, H, block_size, D]``, scales float32 ``[num_blocks, H]`` (value = code * scale),
-    open blocks' tokens float16 / bfloat16 ``[requests, H, block_size, D]``."""
-
+class _LayerTensors(NamedTuple):
     k_codes: Tensor
     v_codes: Tensor
     k_scale: Tensor
     v_scale: Tensor
     tail_k: Tensor
     tail_v: Tensor
+
+
+class PagedLayer(_LayerTensors):
+    """One layer's storage, ``PagedLayer(k_codes, v_codes, k_scale, v_scale, tail_k, tail_v)``: codes int8
+    ``[num_blocks, H, block_size, D]``, scales float32 ``[num_blocks, H]`` (value = code * scale), open blocks' tokens float16 /
+    bfloat16 ``[requests, H, block_size, D]``, all contiguous on one device.  Checked once, here; the tensors stay where they are."""
+
+    def __new__(cls, *tensors: Tensor, **named: Tensor) -> "PagedLayer":
+        self = super().__new__(cls, *tensors, **named)
+        codes = self.k_codes
+        if codes.dim() != 4 or self.tail_k.dim() != 4:
+            raise ValueError("paged layer: codes [num_blocks, heads, block_size, head_dim], open rows [requests, heads, block_size, head_dim]")
+        (n, h, bs, d), requests, dtype, device = codes.shape, self.tail_k.shape[0], self.tail_k.dtype, codes.device
+        if bs not in BLOCK_SIZES or d not in HEAD_DIMS or dtype not in (torch.float16, torch.bfloat16) or n < 1 or h < 1 or requests < 1:
+            raise ValueError(f"paged layer: {n} blocks of {bs} tokens (one of {BLOCK_SIZES}), {h} heads of {d} channels (one of {HEAD_DIMS}), "
+                             f"{requests} requests, open rows in {dtype}")
+        if device.type != "cuda":
+            raise RuntimeError("paged layers are CUDA tensors")
+        for t, shape, want in zip(self, ((n, h, bs, d),) * 2 + ((n, h),) * 2 + ((requests, h, bs, d),) * 2,
+                                  (torch.int8,) * 2 + (torch.float32,) * 2 + (dtype,) * 2):
+            if t.shape != shape or t.dtype is not want or t.device != device or not t.is_contiguous() or t.data_ptr() % 16:
+                raise ValueError(f"paged layer: expected a contiguous, 16-byte aligned {want} tensor {list(shape)} on {device}, got {t.dtype} "
+                                 f"{list(t.shape)} on {t.device}")
+        self.num_blocks, self.heads, self.block_size, self.head_dim, self.requests = n, h, bs, d, requests
+        self.dtype, self.device = dtype, device
+        self._struct = _lib.PagedLayerStruct(*(t.data_ptr() for t in self), n, requests, h, bs, d, _lib.dtype_code(dtype))
+        self._c = ctypes.addressof(self._struct)
+        return self
 
 
 @functools.lru_cache(maxsize=4096)
@@ -64,47 +90,51 @@ def _step_layout(requests: int, tokens: int, block_size: int) -> tuple[int, tupl
 class PagedStep:
     """Tables of one step (made by :func:`plan_blocks`); the properties are views of one buffer on the GPU."""
 
-    __slots__ = ("words", "requests", "tokens", "block_size", "block_table", "_at", "_ptr", "lengths")
+    __slots__ = ("words", "requests", "tokens", "block_size", "block_table", "device", "lengths", "_at", "_ld", "_struct", "_c")
 
     def __init__(self, words: Tensor, at: tuple[int, ...], requests: int, tokens: int, block_size: int, block_table: Tensor) -> None:
-        self.words, self._at, self._ptr = words, at, words.data_ptr()
+        self.words, self._at, self.device = words, at, words.device
         self.requests, self.tokens, self.block_size, self.block_table = requests, tokens, block_size, block_table
         self.lengths: list[tuple[int, int]] | None = None    # (old, new) per request where the host knows them
+        width = block_table.shape[1]
+        self._ld = max(block_table.stride(0), width)
+        self._struct = _lib.PagedTablesStruct(words.data_ptr(), block_table.data_ptr(), self._ld, width, requests, tokens, block_size)
+        self._c = ctypes.addressof(self._struct)
 
     @property
     def query_start(self) -> Tensor:
         """int32 ``[requests + 1]``: first row of each request's new tokens."""
-        return self.words.narrow(0, self._at[1], self.requests + 1)
+        return self.words.as_strided((self.requests + 1,), (1,), self._at[1])
 
     @property
     def seq_lens(self) -> Tensor:
         """int32 ``[requests]``: lengths after the step."""
-        return self.words.narrow(0, self._at[2], self.requests)
+        return self.words.as_strided((self.requests,), (1,), self._at[2])
 
     @property
     def free_count(self) -> Tensor:
         """int32 ``[1]``: free blocks after the step."""
-        return self.words.narrow(0, self._at[2] + self.requests, 1)
+        return self.words.as_strided((1,), (1,), self._at[2] + self.requests)
 
     @property
     def context_start(self) -> Tensor:
         """int64 ``[requests + 1]``: first row of each request in :func:`dense_blocks`' result."""
-        return self.words.narrow(0, self._at[3], 2 * (self.requests + 1)).view(torch.int64)
+        return self.words.as_strided((2 * (self.requests + 1),), (1,), self._at[3]).view(torch.int64)
 
     @property
     def slots(self) -> Tensor:
         """int64 ``[tokens]``: ``block id * block_size + offset`` of each row, -1 for rows that belong to nobody."""
-        return self.words.narrow(0, self._at[4], 2 * self.tokens).view(torch.int64)
+        return self.words.as_strided((2 * self.tokens,), (1,), self._at[4]).view(torch.int64)
 
     @property
     def token_request(self) -> Tensor:
         """int32 ``[tokens]``: request of each row, -1 for nobody."""
-        return self.words.narrow(0, self._at[5], self.tokens)
+        return self.words.as_strided((self.tokens,), (1,), self._at[5])
 
     @property
     def positions(self) -> Tensor:
         """int32 ``[tokens]``: position of each row in its request, -1 for rows that belong to nobody."""
-        return self.words.narrow(0, self._at[6], self.tokens)
+        return self.words.as_strided((self.tokens,), (1,), self._at[6])
 
     def check(self) -> None:
         """Raise if the step was refused (waits for the GPU)."""
@@ -125,7 +155,7 @@ def _call(device: torch.device, fn, what: str, *args) -> None:
 
 
 def _ints(t: Tensor, shape: tuple, device, what: str) -> None:
-    if t.dtype is not torch.int32 or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous int32 tensor {list(shape)} on {device}, got {t.dtype} {list(t.shape)} on {t.device}")
 
 
@@ -144,70 +174,55 @@ def plan_blocks(seq_lens: Tensor, new_lens: Tensor, block_table: Tensor, free_bl
     if dev.type != "cuda":
         raise RuntimeError("plan_blocks runs on CUDA tensors only")
     n = seq_lens.shape[0] if seq_lens.dim() == 1 else 0
-    _ints(seq_lens, (n,), dev, "seq_lens")
-    _ints(new_lens, (n,), dev, "new_lens")
+    per_request, capacity = (n,), free_blocks.numel()
+    _ints(seq_lens, per_request, dev, "seq_lens")
+    _ints(new_lens, per_request, dev, "new_lens")
     _ints(free_count, (1,), dev, "free_count")
-    if (block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.shape[0] != n or block_table.device != dev
-            or block_table.stride(1) != 1 or (n > 1 and block_table.stride(0) < block_table.shape[1])):
+    _ints(free_blocks, (capacity,), dev, "free_blocks")
+    rows = block_table.shape
+    if (block_table.dtype is not torch.int32 or len(rows) != 2 or rows[0] != n or rows[1] == 0 or block_table.device != dev
+            or not (block_table.is_contiguous() or (block_table.stride(1) == 1 and block_table.stride(0) >= rows[1]))):
         raise ValueError(f"block_table must be int32 [{n}, blocks per request] with adjacent columns on {dev}")
-    _ints(free_blocks, (free_blocks.numel(),), dev, "free_blocks")
     nbytes, at = _step_layout(n, tokens, block_size)
-    words = torch.empty(nbytes // 4, dtype=torch.int32, device=dev)
+    words = seq_lens.new_empty(nbytes // 4)
     step = PagedStep(words, at, n, tokens, block_size, block_table)
     _call(dev, _lib.lib().pare_paged_plan, "pare_paged_plan", seq_lens.data_ptr(), new_lens.data_ptr(), n, block_table.data_ptr(),
-          max(block_table.stride(0), block_table.shape[1]), block_table.shape[1], free_blocks.data_ptr(), free_blocks.numel(), free_count.data_ptr(), block_size, tokens,
-          step._ptr, nbytes)
+          step._ld, rows[1], free_blocks.data_ptr(), capacity, free_count.data_ptr(), block_size, tokens, words.data_ptr(), nbytes)
     return step
 
 
-def _geometry(layer: PagedLayer, step: PagedStep) -> tuple[int, int, int]:
-    """``(num_blocks, heads, head_dim)`` of a layer that fits the step."""
-    num_blocks, h, bs, d = layer.k_codes.shape
-    device, dtype = step.words.device, layer.tail_k.dtype
-    codes, scale, tail = (num_blocks, h, bs, d), (num_blocks, h), (step.requests, h, bs, d)
-    if bs != step.block_size or d not in HEAD_DIMS or (dtype is not torch.float16 and dtype is not torch.bfloat16):
-        raise ValueError(f"paged layer: blocks of {bs} tokens (the step's: {step.block_size}), head_dim {d} (one of {HEAD_DIMS}), open rows in {dtype}")
-    for t, shape, want in ((layer.k_codes, codes, torch.int8), (layer.v_codes, codes, torch.int8), (layer.k_scale, scale, torch.float32),
-                           (layer.v_scale, scale, torch.float32), (layer.tail_k, tail, dtype), (layer.tail_v, tail, dtype)):
-        if t.shape != shape or t.dtype is not want or t.device != device or not t.is_contiguous():
-            raise ValueError(f"paged layer: expected a contiguous {want} tensor {list(shape)} on {device}, got {t.dtype} {list(t.shape)} on {t.device}")
-    return num_blocks, h, d
+def _fits(layer: PagedLayer, step: PagedStep) -> None:
+    if layer.block_size != step.block_size or layer.requests != step.requests or layer.device != step.device:
+        raise ValueError(f"the layer ({layer.requests} requests, blocks of {layer.block_size}, {layer.device}) and the step ({step.requests}, "
+                         f"{step.block_size}, {step.device}) do not belong together")
 
 
-def _rows(t: Tensor, shape: tuple, layer: PagedLayer, what: str) -> Tensor:
+def _rows(t: Tensor, tokens: int, heads: int, layer: PagedLayer, what: str) -> Tensor:
     """A step's rows as the kernels take them: channels adjacent, 16-byte aligned rows."""
-    if t.shape != shape or t.dtype is not layer.tail_k.dtype or t.device != layer.tail_k.device:
-        raise ValueError(f"{what} must be {layer.tail_k.dtype} {list(shape)} on {layer.tail_k.device}, got {t.dtype} {list(t.shape)} on {t.device}")
-    s = t.stride()
-    return t if s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+    if t.shape != (tokens, heads, layer.head_dim) or t.dtype is not layer.dtype or t.device != layer.device:
+        raise ValueError(f"{what} must be {layer.dtype} {[tokens, heads, layer.head_dim]} on {layer.device}, got {t.dtype} {list(t.shape)} on {t.device}")
+    a, b, c = t.stride()
+    return t if c == 1 and (a | b) % 8 == 0 and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def append_blocks(layer: PagedLayer, step: PagedStep, k: Tensor, v: Tensor) -> None:
     """Store the step's new keys and values ``[tokens, H, D]`` in one layer: blocks that fill up are quantized into the pool, the
     rest goes to the open rows."""
-    num_blocks, h, d = _geometry(layer, step)
-    shape = (step.tokens, h, d)
-    k, v = _rows(k, shape, layer, "k"), _rows(v, shape, layer, "v")
-    _call(k.device, _lib.lib().pare_paged_append, "pare_paged_append", k.data_ptr(), v.data_ptr(), _lib.dtype_code(k.dtype),
-          k.stride(0), k.stride(1), v.stride(0), v.stride(1), step._ptr, step.requests, step.tokens, step.block_size,
-          *(t.data_ptr() for t in layer), num_blocks, h, d)
-
-
-def _pool(layer: PagedLayer, step: PagedStep) -> tuple:
-    table = step.block_table
-    return (step._ptr, step.requests, step.tokens, step.block_size, table.data_ptr(), max(table.stride(0), table.shape[1]), table.shape[1],
-            *(t.data_ptr() for t in layer))
+    _fits(layer, step)
+    k, v = _rows(k, step.tokens, layer.heads, layer, "k"), _rows(v, step.tokens, layer.heads, layer, "v")
+    ks, vs = k.stride(), v.stride()
+    _call(layer.device, _lib.lib().pare_paged_append, "pare_paged_append", k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1],
+          layer._c, step._c)
 
 
 def dense_blocks(layer: PagedLayer, step: PagedStep, total: int) -> tuple[Tensor, Tensor]:
     """Keys and values, after the step's append, of every request with new tokens in it: two tensors ``[total, H, D]`` of the open
     rows' dtype, request ``r`` from row ``step.context_start[r]`` on (``total``: the sum of those requests' lengths; rows beyond it
     are left out, rows behind the last token are zeros)."""
-    num_blocks, h, d = _geometry(layer, step)
-    k = torch.empty(total, h, d, dtype=layer.tail_k.dtype, device=layer.tail_k.device)
+    _fits(layer, step)
+    k = layer.tail_k.new_empty(total, layer.heads, layer.head_dim)
     v = torch.empty_like(k)
-    _call(k.device, _lib.lib().pare_paged_dense, "pare_paged_dense", *_pool(layer, step), num_blocks, h, d, k.data_ptr(), v.data_ptr(),
-          _lib.dtype_code(k.dtype), total)
+    _call(layer.device, _lib.lib().pare_paged_dense, "pare_paged_dense", layer._c, step._c, k.data_ptr(), v.data_ptr(), total)
     return k, v
 
 
@@ -221,23 +236,28 @@ def attend_blocks(layer: PagedLayer, step: PagedStep, q: Tensor, scale: float | 
     """``softmax(q K^T * scale) V`` of the step's queries ``q [tokens, Hq, D]`` over their request's tokens up to and with their own
     (the step's keys and values have been appended).  ``Hq`` is a multiple of the KV heads; default scale ``1 / sqrt(D)``.  At most
     4096 rows: longer prompts go through :meth:`PagedKVCache.prefill`.  Rows that belong to nobody are left as they were in
-    ``out`` (``[tokens, Hq, D]``, channels adjacent; a new tensor if not given)."""
-    num_blocks, h, d = _geometry(layer, step)
-    if q.dim() != 3 or q.shape[1] == 0 or q.shape[1] % h:
-        raise ValueError(f"attend_blocks: q [tokens, heads, {d}] with a multiple of {h} heads, got {list(q.shape)}")
-    if step.tokens > MAX_QUERY_TOKENS:
-        raise ValueError(f"attend_blocks takes at most {MAX_QUERY_TOKENS} rows, got {step.tokens}")
-    hq = q.shape[1]
-    q = _rows(q, (step.tokens, hq, d), layer, "q")
+    ``out`` (``[tokens, Hq, D]``, channels adjacent, not overlapping ``q``; a new tensor if not given)."""
+    _fits(layer, step)
+    tokens, d, dev = step.tokens, layer.head_dim, layer.device
+    hq = q.shape[1] if q.dim() == 3 else 0
+    if hq == 0 or hq % layer.heads:
+        raise ValueError(f"attend_blocks: q [tokens, heads, {d}] with a multiple of {layer.heads} heads, got {list(q.shape)}")
+    if tokens > MAX_QUERY_TOKENS:
+        raise ValueError(f"attend_blocks takes at most {MAX_QUERY_TOKENS} rows, got {tokens}")
+    q = _rows(q, tokens, hq, layer, "q")
     if out is None:
-        out = torch.empty(step.tokens, hq, d, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype is not q.dtype or out.device != q.device or out.stride(2) != 1:
-        raise ValueError(f"out must be {q.dtype} {list(q.shape)} on {q.device} with adjacent channels")
-    # from the allocator for each call: it belongs to this call's stream, or to the graph that captures it
-    ws = torch.empty(_attn_workspace(d, q.device.index), dtype=torch.uint8, device=q.device)
-    _call(q.device, _lib.lib().pare_paged_attn, "pare_paged_attn", q.data_ptr(), _lib.dtype_code(q.dtype), q.stride(0), q.stride(1),
-          *_pool(layer, step), num_blocks, hq, h, d, out.data_ptr(), out.stride(0), out.stride(1),
-          float(scale if scale is not None else 1.0 / math.sqrt(d)), ws.data_ptr(), ws.numel())
+        out = q.new_empty(tokens, hq, d)
+    elif out.shape != q.shape or out.dtype is not q.dtype or out.device != dev or out.stride(2) != 1:
+        raise ValueError(f"out must be {q.dtype} {list(q.shape)} on {dev} with adjacent channels")
+    if dev.index != _lib.current_device():
+        with torch.cuda.device(dev):
+            return attend_blocks(layer, step, q, scale, out)
+    stream, nbytes, qs, os = _lib.current_stream(dev), _attn_workspace(d, dev.index), q.stride(), out.stride()
+    ws = _lib.scratch(dev, nbytes, stream)
+    status = _lib.lib().pare_paged_attn(q.data_ptr(), qs[0], qs[1], layer._c, step._c, hq, out.data_ptr(), os[0], os[1],
+                                        1.0 / math.sqrt(d) if scale is None else scale, ws.data_ptr(), nbytes, stream)
+    if status:
+        _lib.check(status, "pare_paged_attn")
     return out
 
 
@@ -381,7 +401,7 @@ class PagedKVCache:
         request on the prompt attention kernel).  The host needs the lengths: where they were given as tensors it waits for
         them."""
         layer = self.layers[layer_idx]
-        if layer.k_codes.shape[3] != 128:
+        if layer.head_dim != 128:
             raise ValueError("prefill needs head_dim 128: use attend")
         if step.lengths is None:
             step.check()

@@ -74,24 +74,45 @@ def test_c_entries_refuse():
         return L.pare_paged_release(mask, p, R, p, ld, 4, p, 8, p, bs, None)
     assert release(R=0) == release(ld=3) == release(mask=None) == SHAPE and release(bs=17) == UNSUPPORTED
 
-    def append(k=p, dtype=0, st=256, T=2, bs=16, NB=4, H=2, D=128, tail=p):
-        return L.pare_paged_append(k, p, dtype, st, 128, st, 128, p, 2, T, bs, p, p, p, p, tail, p, NB, H, D, None)
-    assert append(k=None) == append(NB=0) == append(H=0) == append(T=-1) == append(tail=None) == SHAPE and append(dtype=2) == DTYPE
-    assert append(D=96) == append(bs=8) == UNSUPPORTED and append(k=p + 2) == append(st=130) == append(tail=p + 8) == ALIGN
-    assert append(T=0) == OK
+    def layer(dtype=0, NB=4, H=2, D=128, bs=16, R=2, tail=p, codes=p):
+        return _lib.PagedLayerStruct(codes, p, p, p, tail, p, NB, R, H, bs, D, dtype)
 
-    def dense(total=3, dtype=0, D=128, out=p, ld=4):
-        return L.pare_paged_dense(p, 2, 2, 16, p, ld, 4, p, p, p, p, p, p, 4, 2, D, out, p, dtype, total, None)
-    assert dense(total=-1) == dense(out=None) == dense(ld=3) == SHAPE and dense(dtype=2) == DTYPE and dense(D=32) == UNSUPPORTED
-    assert dense(out=p + 2) == ALIGN and dense(total=0) == OK
+    def tables(T=2, ld=4, width=4, bs=16, R=2, step=p):
+        return _lib.PagedTablesStruct(step, p, ld, width, R, T, bs)
+
+    calls = (lambda l, t: L.pare_paged_append(p, p, 256, 128, 256, 128, ctypes.addressof(l), ctypes.addressof(t), None),
+             lambda l, t: L.pare_paged_dense(ctypes.addressof(l), ctypes.addressof(t), p, p, 3, None),
+             lambda l, t: L.pare_paged_attn(p, 1024, 128, ctypes.addressof(l), ctypes.addressof(t), 8, p, 1024, 128, 0.1, p, 1 << 26, None))
+    for call in calls:
+        for l, t in ((layer(NB=0), tables()), (layer(H=0), tables()), (layer(H=70000), tables()), (layer(tail=None), tables()), (layer(), tables(T=-1)),
+                     (layer(), tables(ld=3)), (layer(), tables(width=0)), (layer(), tables(R=3)), (layer(), tables(bs=32)), (layer(), tables(step=None)),
+                     (layer(R=0), tables(R=0))):
+            assert call(l, t) == SHAPE
+        assert call(layer(dtype=2), tables()) == DTYPE
+        assert call(layer(D=96), tables()) == call(layer(bs=8), tables(bs=8)) == call(layer(bs=128), tables(bs=128)) == UNSUPPORTED
+        assert call(layer(codes=p + 8), tables()) == call(layer(tail=p + 2), tables()) == call(layer(), tables(step=p + 4)) == ALIGN
+    ok, some = layer(), tables()
+    lp, tp, none = ctypes.addressof(ok), ctypes.addressof(some), tables(T=0)
+
+    def append(k=p, st=256):
+        return L.pare_paged_append(k, p, st, 128, st, 128, lp, tp, None)
+    assert append(k=None) == SHAPE and append(k=p + 2) == append(st=130) == ALIGN
+    assert L.pare_paged_append(p, p, 256, 128, 256, 128, None, tp, None) == L.pare_paged_append(p, p, 256, 128, 256, 128, lp, None, None) == SHAPE
+    assert L.pare_paged_append(None, None, 256, 128, 256, 128, lp, ctypes.addressof(none), None) == OK
+
+    def dense(total=3, out=p):
+        return L.pare_paged_dense(lp, tp, out, p, total, None)
+    assert dense(total=-1) == dense(out=None) == SHAPE and dense(out=p + 2) == ALIGN and dense(total=0) == OK
 
     need = 1 << 26
 
-    def attend(q=p, dtype=0, T=2, bs=16, Hq=8, H=2, D=128, ws=p, size=need, sh=128):
-        return L.pare_paged_attn(q, dtype, 1024, sh, p, 2, T, bs, p, 4, 4, p, p, p, p, p, p, 4, Hq, H, D, p, 1024, 128, 0.1, ws, size, None)
-    assert attend(q=None) == attend(Hq=7) == attend(Hq=0) == attend(H=0) == attend(T=-1) == SHAPE and attend(dtype=2) == DTYPE
-    assert attend(D=256) == attend(bs=128) == attend(T=4097) == UNSUPPORTED and attend(size=16) == attend(ws=None) == SPACE
-    assert attend(q=p + 4) == attend(sh=130) == attend(ws=p + 8) == ALIGN and attend(T=0) == OK
+    many = tables(T=4097)
+
+    def attend(q=p, t=tp, Hq=8, ws=p, size=need, sh=128):
+        return L.pare_paged_attn(q, 1024, sh, lp, t, Hq, p, 1024, 128, 0.1, ws, size, None)
+    assert attend(q=None) == attend(Hq=7) == attend(Hq=0) == SHAPE and attend(t=ctypes.addressof(many)) == UNSUPPORTED
+    assert attend(size=16) == attend(ws=None) == SPACE and attend(q=p + 4) == attend(sh=130) == attend(ws=p + 8) == ALIGN
+    assert attend(t=ctypes.addressof(none)) == OK
     assert L.pare_paged_attn_workspace_bytes(96) == 0
 
     def linear(M=2, N=4, K=32, ldw=32, ldx=32, ldy=4, dtype=0, x=p, w=p, ws=p, size=need):
