@@ -353,19 +353,19 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
   const int tiles = p.H * p.sub;       // tiles of eight heads per token
   const int me = blockIdx.x * kWarps + warp;
   pdl_wait();
-  const int64_t total = (int64_t)p.unit_start[p.T] * tiles, run = run_units(total, gridDim.x * kWarps);
+  // The last token that begins at or before this run: 32 candidates a round, the first round together with the number of units
+  const int all = p.unit_start[p.T], spread = (p.T + 31) / 32;
+  const int mark = lane * spread < p.T ? p.unit_start[lane * spread] : 0x7fffffff;
+  const int64_t total = (int64_t)all * tiles, run = run_units(total, gridDim.x * kWarps);
   const int64_t u0 = me * run, u1 = min(u0 + run, total);
   if (u0 >= u1) return;
-  int t = 0;       // the last token that begins at or before u0: 32 candidates a round
-  {
-    const int x = (int)(u0 / tiles);
-    for (int n = p.T; n > 1;) {
-      const int step = (n + 31) / 32, at = lane * step;
-      const uint32_t yes = __ballot_sync(0xffffffffu, at < n && p.unit_start[t + min(at, n - 1)] <= x);
-      const int k = 31 - __clz(yes);
-      t += k * step;
-      n = min(step, n - k * step);
-    }
+  const int x = (int)(u0 / tiles), k0 = 31 - __clz(__ballot_sync(0xffffffffu, mark <= x));
+  int t = k0 * spread;
+  for (int n = min(spread, p.T - t); n > 1;) {
+    const int step = (n + 31) / 32, at = lane * step;
+    const int k = 31 - __clz(__ballot_sync(0xffffffffu, at < n && p.unit_start[t + min(at, n - 1)] <= x));
+    t += k * step;
+    n = min(step, n - k * step);
   }
 
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem + warp * S::kRing);

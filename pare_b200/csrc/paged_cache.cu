@@ -7,6 +7,8 @@
 // Until then its tokens stay in the input type in the request's open rows (tail_k / tail_v), so every code is the result of one
 // rounding and tokens fed in pieces give what the same tokens fed at once give (the property of the reference's residual window,
 // pare/kv_cache.py:231-244).
+#include <type_traits>
+
 #include "paged.cuh"
 #include "quant8.cuh"
 
@@ -35,27 +37,39 @@ struct PlanParams {
   int R, T, bs_log2, max_blocks, free_capacity, n_items, units;
 };
 
-// Exclusive prefix sum of one value per thread, and the total.  All threads call it.
-__device__ __forceinline__ long long block_scan(long long v, long long* sums, long long& total) {
+// Exclusive prefix sums of N values per thread, and their totals.  All threads call it.
+template <int N>
+__device__ __forceinline__ void block_scan(const long long (&v)[N], long long (&before)[N], long long (&total)[N], long long (*sums)[kPlanWarps]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long x = v;
+  long long x[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = v[i];
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
-  __syncthreads();
-  if (lane == 31) sums[warp] = x;
-  __syncthreads();
-  long long before = 0, all = 0;
 #pragma unroll
-  for (int w = 0; w < kPlanWarps; ++w) {
-    const long long s = sums[w];
-    if (w < warp) before += s;
-    all += s;
+    for (int i = 0; i < N; ++i) {
+      const long long y = __shfl_up_sync(0xffffffffu, x[i], o);
+      if (lane >= o) x[i] += y;
+    }
   }
-  total = all;
-  return before + x - v;
+  __syncthreads();
+  if (lane == 31) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) sums[i][warp] = x[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    // the warps' sums, one per lane
+    long long s = lane < kPlanWarps ? sums[i][lane] : 0, mine = lane < warp ? s : 0;
+#pragma unroll
+    for (int o = kPlanWarps / 2; o > 0; o >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, o);
+      mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    }
+    total[i] = __shfl_sync(0xffffffffu, s, 0);
+    before[i] = __shfl_sync(0xffffffffu, mine, 0) + x[i] - v[i];
+  }
 }
 
 // Largest i in [0, n) with start[i] <= x (start[0] = 0 <= x, not decreasing).
@@ -71,7 +85,11 @@ __device__ __forceinline__ int last_at_most(const int* start, int n, int x) {
 
 __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanParams p) {
   extern __shared__ int s_mem[];
-  __shared__ long long s_sums[kPlanWarps];
+  pdl_launch_dependents();
+  pdl_wait();
+  __shared__ long long s_sums[4][kPlanWarps];
+  __shared__ int s_bad;
+  if (threadIdx.x == 0) s_bad = 0;
   int* s_start = s_mem;              // [R] first row of the new tokens
   int* s_len = s_start + p.R;        // [R] tokens before the step
   int* s_take = s_len + p.R;         // [R] blocks taken from the stack by the requests before
@@ -82,7 +100,8 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
   const int64_t max_len = (int64_t)p.max_blocks << p.bs_log2;
 
   int bad = 0;
-  long long n_new = 0, n_take = 0, n_item = 0, n_ctx = 0;
+  const int count = *p.free_count;
+  long long sum[4] = {0, 0, 0, 0}, before[4], total[4];      // new tokens, blocks taken, blocks touched, tokens of requests with new ones
   for (int r = r0; r < r1; ++r) {
     const int len = p.seq_lens[r], add = p.new_lens[r];
     if (len < 0 || add < 0) bad |= PARE_PAGED_NEGATIVE;
@@ -90,38 +109,32 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
     else if ((int64_t)len + add > max_len) bad |= PARE_PAGED_TABLE;
     else {
       const int end = len + add;
-      s_start[r] = (int)n_new;
+      s_start[r] = (int)sum[0];
       s_len[r] = len;
-      s_take[r] = (int)n_take;
-      s_item[r] = (int)n_item;
-      n_new += add;
-      n_take += ((end + bs - 1) >> p.bs_log2) - ((len + bs - 1) >> p.bs_log2);
+      s_take[r] = (int)sum[1];
+      s_item[r] = (int)sum[2];
+      sum[0] += add;
+      sum[1] += ((end + bs - 1) >> p.bs_log2) - ((len + bs - 1) >> p.bs_log2);
       if (add) {
-        n_item += ((end - 1) >> p.bs_log2) - (len >> p.bs_log2) + 1;
-        n_ctx += end;
+        sum[2] += ((end - 1) >> p.bs_log2) - (len >> p.bs_log2) + 1;
+        sum[3] += end;
       }
     }
   }
-  const int count = *p.free_count;
   if (count < 0 || count > p.free_capacity) bad |= PARE_PAGED_BLOCKS;
-  long long t_new, t_take, t_item, t_ctx;
-  const long long b_new = block_scan(n_new, s_sums, t_new), b_take = block_scan(n_take, s_sums, t_take);
-  const long long b_item = block_scan(n_item, s_sums, t_item), b_ctx = block_scan(n_ctx, s_sums, t_ctx);
-  if (t_new > p.T) bad |= PARE_PAGED_ROWS;
-  if (t_take > count) bad |= PARE_PAGED_BLOCKS;
-  __shared__ int s_bad;
-  if (threadIdx.x == 0) s_bad = 0;
-  __syncthreads();
+  block_scan<4>(sum, before, total, s_sums);
+  if (total[0] > p.T) bad |= PARE_PAGED_ROWS;
+  if (total[1] > count) bad |= PARE_PAGED_BLOCKS;
   if (bad) atomicOr(&s_bad, bad);
   __syncthreads();
   bad = s_bad;                       // the step is done or refused as a whole
-  if (bad) t_new = t_take = t_item = 0;
-  long long ctx = b_ctx;
+  const long long t_new = bad ? 0 : total[0], t_take = bad ? 0 : total[1], t_item = bad ? 0 : total[2];
+  long long ctx = before[3];
   for (int r = r0; r < r1; ++r) {
     if (!bad) {
-      s_start[r] += (int)b_new;
-      s_take[r] += (int)b_take;
-      s_item[r] += (int)b_item;
+      s_start[r] += (int)before[0];
+      s_take[r] += (int)before[1];
+      s_item[r] += (int)before[2];
     }
     if (lead) {
       const int len = p.seq_lens[r], add = bad ? 0 : p.new_lens[r];
@@ -138,7 +151,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
     p.step[3] = 0;
     p.step[p.o_query_start + R] = (int)t_new;
     p.step[p.o_seq_lens + R] = count - (int)t_take;
-    reinterpret_cast<long long*>(p.step + p.o_context)[R] = bad ? 0 : t_ctx;
+    reinterpret_cast<long long*>(p.step + p.o_context)[R] = bad ? 0 : total[3];
   }
   __syncthreads();
 
@@ -192,14 +205,15 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
       const int held = end >> p.bs_log2 << p.bs_log2, nq = min(seen, held);
       return (nq + kUnit - 1) / kUnit + (seen - nq + kUnit - 1) / kUnit;
     };
-    long long n = 0, all;
-    for (int t = t0; t < t1; ++t) n += units_of(t);
-    int at = (int)block_scan(n, s_sums, all);
+    long long n[1] = {0}, first[1], all[1];
+    for (int t = t0; t < t1; ++t) n[0] += units_of(t);
+    block_scan<1>(n, first, all, s_sums);
+    int at = (int)first[0];
     for (int t = t0; t < t1; ++t) {
       p.step[p.o_units + t] = at;
       at += units_of(t);
     }
-    if (threadIdx.x == 0) p.step[p.o_units + p.T] = (int)all;
+    if (threadIdx.x == 0) p.step[p.o_units + p.T] = (int)all[0];
   }
 }
 
@@ -207,16 +221,17 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
 __global__ void __launch_bounds__(kPlanThreads) paged_release_kernel(const int* release, int* seq_lens, const int* table, int64_t ld_table,
                                                                      int* free_blocks, int free_capacity, int* free_count, int R, int bs_log2,
                                                                      int max_blocks) {
-  __shared__ long long s_sums[kPlanWarps];
+  __shared__ long long s_sums[1][kPlanWarps];
   const int per = (R + kPlanThreads - 1) / kPlanThreads, r0 = min(R, (int)threadIdx.x * per), r1 = min(R, r0 + per);
   auto blocks_of = [&](int r) {
     const int len = seq_lens[r];
     return release[r] == 0 || len <= 0 ? 0 : min(max_blocks, (int)(((int64_t)len + (1 << bs_log2) - 1) >> bs_log2));
   };
-  long long n = 0, all;
-  for (int r = r0; r < r1; ++r) n += blocks_of(r);
+  long long n[1] = {0}, before[1], all[1];
+  for (int r = r0; r < r1; ++r) n[0] += blocks_of(r);
   const int count = max(0, *free_count);
-  long long at = count + block_scan(n, s_sums, all);
+  block_scan<1>(n, before, all, s_sums);
+  long long at = count + before[0];
   for (int r = r0; r < r1; ++r) {
     const int nb = blocks_of(r);
     for (int b = 0; b < nb; ++b, ++at)
@@ -224,13 +239,15 @@ __global__ void __launch_bounds__(kPlanThreads) paged_release_kernel(const int* 
     if (release[r] != 0) seq_lens[r] = 0;
   }
   __syncthreads();
-  if (threadIdx.x == 0) *free_count = (int)min((long long)free_capacity, count + all);
+  if (threadIdx.x == 0) *free_count = (int)min((long long)free_capacity, count + all[0]);
 }
 
 // ---- append -----------------------------------------------------------------------------------------------------------------------
-// One thread block per (touched block of tokens, head); half the threads take the keys, half the values.  A block that fills up is
-// held in registers (at most 64 values a thread) between the maximum and the codes, so its tokens are read once.
-constexpr int kAppendThreads = 256;
+// A team of threads takes one (touched block of tokens, head) of the keys or of the values.  A block that fills up is held in registers
+// between the maximum and the codes, so its tokens are read once.  Four threads per token (32 values each, all loads in flight at
+// once) where eight per token would take several rounds of the SMs, else eight: 32768 tokens of 4 heads 25.6 us against 34, but 2056 tokens of 8
+// heads 8.7 against 6.2 (two threads per token: 26.7).
+__host__ __device__ constexpr int append_threads(int team) { return team > 256 ? team : 256; }
 
 struct AppendParams {
   const void* k;
@@ -246,22 +263,27 @@ struct AppendParams {
   int H, num_blocks, R, T;
 };
 
-template <typename T, int D, int BS>
-__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const AppendParams p) {
+template <typename T, int D, int BS, int PER_TOKEN>
+__global__ void __launch_bounds__(append_threads(BS * PER_TOKEN)) paged_append_kernel(const AppendParams p) {
   pdl_launch_dependents();
-  constexpr int kChunks = D / 8, kHalf = kAppendThreads / 2, kEach = BS * kChunks / kHalf > 0 ? BS * kChunks / kHalf : 1;
-  static_assert(BS * kChunks % kHalf == 0, "whole rounds");
-  __shared__ uint32_t s_max[2][kHalf / 32];
+  pdl_wait();
+  constexpr int kChunks = D / 8, kTeam = BS * PER_TOKEN, kThreads = append_threads(kTeam), kEach = BS * kChunks / kTeam;      // threads of a team, vectors of eight per thread
+  __shared__ uint32_t s_max[kThreads / 32];
   const int4* item = reinterpret_cast<const int4*>(p.items + (int64_t)blockIdx.x * kItemInts);
   const int4 a = item[0], b = item[1];
-  const int r = a.x, id = a.y, row0 = a.z, off = a.w, n = b.x, blk = b.y, len = b.z, end = b.w, h = blockIdx.y;
-  if (r < 0 || r >= p.R || row0 < 0 || row0 + n > p.T) return;
-  const int half = threadIdx.x / kHalf, tid = threadIdx.x % kHalf;
+  const int r = a.x, id = a.y, row0 = a.z, off = a.w, n = b.x, blk = b.y, len = b.z, end = b.w;
+  const int team = threadIdx.x / kTeam, tid = threadIdx.x % kTeam, job = blockIdx.y * (kThreads / kTeam) + team;      // heads' keys, then heads' values
+  if (r < 0 || r >= p.R || row0 < 0 || row0 + n > p.T || job >= 2 * p.H) return;
+  const int half = job >= p.H, h = job - half * p.H;
+  auto team_sync = [&] {
+    if (kTeam == 32) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(kTeam) : "memory");
+  };
   const T* src = reinterpret_cast<const T*>(half ? p.v : p.k) + h * (half ? p.v_sh : p.k_sh);
   const int64_t st = half ? p.v_st : p.k_st;
   T* tail = reinterpret_cast<T*>(half ? p.tail_v : p.tail_k) + ((int64_t)r * p.H + h) * BS * D;
   auto new_rows_to_tail = [&](int row, int to, int count) {
-    for (int i = tid; i < count * kChunks; i += kHalf) {
+    for (int i = tid; i < count * kChunks; i += kTeam) {
       const int t = i / kChunks, c = i % kChunks * 8;
       *reinterpret_cast<uint4*>(tail + (to + t) * D + c) = *reinterpret_cast<const uint4*>(src + (row + t) * st + c);
     }
@@ -276,33 +298,35 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
-    const int at = i * kHalf + tid, t = at / kChunks, c = at % kChunks * 8;
+    const int at = i * kTeam + tid, t = at / kChunks, c = at % kChunks * 8;
     x[i] = t < off ? *reinterpret_cast<const uint4*>(tail + t * D + c) : *reinterpret_cast<const uint4*>(src + (row0 + t - off) * st + c);
     top = __vmaxu2(top, q8::magnitudes(x[i]));
   }
   top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
-  if ((threadIdx.x & 31) == 0) s_max[half][tid / 32] = top;
-  __syncthreads();
+  if (kTeam > 32) {
+    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x / 32] = top;
+    team_sync();
 #pragma unroll
-  for (int w = 0; w < kHalf / 32; ++w) top = max(top, s_max[half][w]);
+    for (int w = 0; w < kTeam / 32; ++w) top = max(top, s_max[team * (kTeam / 32) + w]);
+  }
   const uint16_t bits = (uint16_t)top;
   const q8::Grid grid(to_float<T>(*reinterpret_cast<const T*>(&bits)));
   if (id >= 0 && id < p.num_blocks) {
     int8_t* codes = (half ? p.v_codes : p.k_codes) + ((int64_t)id * p.H + h) * BS * D;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) *reinterpret_cast<uint2*>(codes + (i * kHalf + tid) * 8) = grid.codes<T>(x[i]);
+    for (int i = 0; i < kEach; ++i) *reinterpret_cast<uint2*>(codes + (i * kTeam + tid) * 8) = grid.codes<T>(x[i]);
     if (tid == 0) (half ? p.v_scale : p.k_scale)[(int64_t)id * p.H + h] = grid.step;
   }
   if (off > 0 && end % BS != 0 && end / BS > blk) {   // the open block behind it: its rows are free only now
-    asm volatile("bar.sync %0, %1;" ::"r"(1 + half), "n"(kHalf) : "memory");
+    team_sync();
     new_rows_to_tail(row0 + end / BS * BS - (blk * BS + off), 0, end % BS);
   }
 }
 
 // ---- dense ------------------------------------------------------------------------------------------------------------------------
-// Keys and values of every request with new tokens, one request after the other: [total][H][D].  A warp takes a token with all its
-// heads: 16 codes (or 8 open values twice) per lane and round.
-constexpr int kDenseTokens = 32, kDenseThreads = 256;
+// Keys and values of every request with new tokens, one request after the other: [total][H][D].  A warp takes two tokens with all
+// their heads, 16 channels per lane and round (one token: 24.4 us for 32768 of 4 heads, two 20.3, four 20.7, eight 20.7).
+constexpr int kDenseThreads = 256, kDenseEach = 2, kDenseTokens = kDenseThreads / 32 * kDenseEach;
 
 struct DenseParams {
   const long long* context_start;
@@ -321,8 +345,19 @@ struct DenseParams {
   int R, H, bs_log2, num_blocks, max_blocks;
 };
 
+// sixteen codes times their scale, rounded
+template <typename T>
+__device__ __forceinline__ void scaled16(const uint4& c, float s, uint4 (&out)[2]) {
+  const int8_t* q = reinterpret_cast<const int8_t*>(&c);
+  T* e = reinterpret_cast<T*>(out);
+#pragma unroll
+  for (int j = 0; j < 16; ++j) e[j] = from_float<T>((float)q[j] * s);
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kDenseThreads) paged_dense_kernel(const DenseParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
   const int64_t first = (int64_t)blockIdx.x * kDenseTokens;
   __shared__ int s_r;
   if (threadIdx.x == 0) s_r = 0;
@@ -333,46 +368,62 @@ __global__ void __launch_bounds__(kDenseThreads) paged_dense_kernel(const DenseP
   if ((threadIdx.x & 31) == 0) atomicAdd(&s_r, before);
   __syncthreads();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, bs = 1 << p.bs_log2;
-  int r = s_r - 1;
-  for (int i = warp; i < kDenseTokens; i += kDenseThreads / 32) {
-    const int64_t t = first + i;
-    if (t >= p.total) return;
+  const int64_t t0 = first + warp * kDenseEach;
+  // lane i finds out about token i: its row of codes (>= 0), of open tokens (-1 - row), or what else it is
+  constexpr long long kNothing = (1ll << 62), kBad = kNothing + 1;      // behind the last request; a block that is not in the pool
+  long long where = kNothing;
+  int id = 0;
+  if (lane < kDenseEach) {
+    const int64_t t = t0 + lane;
+    int r = s_r - 1;
     while (r < p.R && p.context_start[r + 1] <= t) ++r;
-    T* ok = reinterpret_cast<T*>(p.out_k) + t * p.H * D;
-    T* ov = reinterpret_cast<T*>(p.out_v) + t * p.H * D;
-    const bool real = r >= 0 && r < p.R;
-    const int pos = real ? (int)(t - p.context_start[r]) : 0, end = real ? p.seq_lens[r] : 0;
-    const bool held = pos < (end >> p.bs_log2 << p.bs_log2);
-    int id = 0;
-    if (real && held) id = (pos >> p.bs_log2) < p.max_blocks ? p.table[r * p.ld_table + (pos >> p.bs_log2)] : -1;
-    const bool good = id >= 0 && id < p.num_blocks;
-    for (int c = lane * 16; c < p.H * D; c += 32 * 16) {
-      const int h = c / D, ch = c % D;
-      uint4 wk[2], wv[2];
-      if (real && held && good) {
-        const int64_t row = (((int64_t)id * p.H + h) << p.bs_log2) + (pos & (bs - 1));
-        const uint4 ck = ld_stream_v4(p.k_codes + row * D + ch), cv = ld_stream_v4(p.v_codes + row * D + ch);
-        const float sk = p.k_scale[(int64_t)id * p.H + h], sv = p.v_scale[(int64_t)id * p.H + h];
-        const int8_t* qk = reinterpret_cast<const int8_t*>(&ck);
-        const int8_t* qv = reinterpret_cast<const int8_t*>(&cv);
-        T* ek = reinterpret_cast<T*>(wk);
-        T* ev = reinterpret_cast<T*>(wv);
+    if (r < p.R) {
+      const int pos = (int)(t - p.context_start[r]), blk = pos >> p.bs_log2, off = pos & (bs - 1);
+      if (blk < p.seq_lens[r] >> p.bs_log2) {
+        id = blk < p.max_blocks ? p.table[r * p.ld_table + blk] : -1;
+        where = id >= 0 && id < p.num_blocks ? ((((long long)id * p.H) << p.bs_log2) + off) : kBad;
+      } else {
+        where = -1 - ((((long long)r * p.H) << p.bs_log2) + off);
+      }
+    }
+  }
+  const int tokens = (int)min((int64_t)kDenseEach, p.total - t0);
+  for (int base = 0; base < p.H * D; base += 32 * 16) {
+    const int c = base + lane * 16, h = c / D, ch = c % D;
+    const bool inside = c < p.H * D;
+    const int64_t skip = ((int64_t)h << p.bs_log2) * D + ch;       // from head 0 to this lane's channels
+    uint4 ck[kDenseEach], cv[kDenseEach];
+    float sk[kDenseEach], sv[kDenseEach];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          ek[j] = from_float<T>((float)qk[j] * sk);
-          ev[j] = from_float<T>((float)qv[j] * sv);
-        }
-      } else if (real && !held) {
-        const int64_t at = ((((int64_t)r * p.H + h) << p.bs_log2) + (pos & (bs - 1))) * D + ch;
-        const uint4* tk = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.tail_k) + at);
-        const uint4* tv = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.tail_v) + at);
+    for (int i = 0; i < kDenseEach; ++i) {
+      const long long w = __shfl_sync(0xffffffffu, where, i);
+      const int block = __shfl_sync(0xffffffffu, id, i);
+      if (inside && i < tokens && w >= 0 && w < kNothing) {
+        ck[i] = ld_stream_v4(p.k_codes + w * D + skip);
+        cv[i] = ld_stream_v4(p.v_codes + w * D + skip);
+        sk[i] = p.k_scale[(int64_t)block * p.H + h];
+        sv[i] = p.v_scale[(int64_t)block * p.H + h];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kDenseEach; ++i) {
+      const long long w = __shfl_sync(0xffffffffu, where, i);
+      if (!inside || i >= tokens) continue;
+      uint4 wk[2], wv[2];
+      if (w >= 0 && w < kNothing) {
+        scaled16<T>(ck[i], sk[i], wk);
+        scaled16<T>(cv[i], sv[i], wv);
+      } else if (w < 0) {
+        const uint4* tk = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.tail_k) + (-1 - w) * D + skip);
+        const uint4* tv = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.tail_v) + (-1 - w) * D + skip);
         wk[0] = tk[0], wk[1] = tk[1], wv[0] = tv[0], wv[1] = tv[1];
       } else {   // behind the last request: zeros; a block that is not in the pool: NaN
-        const uint32_t w = real ? 0x7fff7fffu : 0u;
-        wk[0] = wk[1] = wv[0] = wv[1] = make_uint4(w, w, w, w);
+        const uint32_t x = w == kBad ? 0x7fff7fffu : 0u;
+        wk[0] = wk[1] = wv[0] = wv[1] = make_uint4(x, x, x, x);
       }
-      reinterpret_cast<uint4*>(ok + c)[0] = wk[0], reinterpret_cast<uint4*>(ok + c)[1] = wk[1];
-      reinterpret_cast<uint4*>(ov + c)[0] = wv[0], reinterpret_cast<uint4*>(ov + c)[1] = wv[1];
+      uint4* ok = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out_k) + (t0 + i) * p.H * D + c);
+      uint4* ov = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out_v) + (t0 + i) * p.H * D + c);
+      ok[0] = wk[0], ok[1] = wk[1], ov[0] = wv[0], ov[1] = wv[1];
     }
   }
 }
@@ -417,8 +468,8 @@ int pare_paged_plan(const int32_t* seq_lens, const int32_t* new_lens, int R, int
   if (!ensure_smem_attr(reinterpret_cast<const void*>(paged_plan_kernel), kMaxRequests * 4 * (int)sizeof(int))) return PARE_ERR_CUDA;
   int blocks = (T + kPlanThreads - 1) / kPlanThreads;
   blocks = blocks < 1 ? 1 : blocks > sm_count() ? sm_count() : blocks;
-  paged_plan_kernel<<<blocks, kPlanThreads, smem, reinterpret_cast<cudaStream_t>(stream)>>>(p);
-  return launch_status();
+  const int rc = launch_pdl(paged_plan_kernel, dim3(blocks), dim3(kPlanThreads), smem, reinterpret_cast<cudaStream_t>(stream), p);
+  return rc != PARE_OK ? rc : launch_status();
 }
 
 int pare_paged_release(const int32_t* release, int32_t* seq_lens, int R, const int32_t* block_table, int64_t ld_table, int max_blocks,
@@ -440,19 +491,23 @@ int pare_paged_append(const void* k, const void* v, int64_t k_stride_t, int64_t 
   const StepLayout s(t->R, t->T, t->block_size);
   const AppendParams p{k, v, k_stride_t, k_stride_h, v_stride_t, v_stride_h, reinterpret_cast<const int*>(t->step) + s.items,
                        l->k_codes, l->v_codes, l->k_scale, l->v_scale, l->tail_k, l->tail_v, l->H, l->num_blocks, l->R, t->T};
-  const dim3 grid(s.n_items, l->H);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  auto go = [&](auto kern) {
-    kern<<<grid, kAppendThreads, 0, st>>>(p);
-    return launch_status();
+  const int bs = l->block_size;
+  const bool many = (int64_t)s.n_items * 2 * l->H * 8 * bs > (int64_t)sm_count() * 8192;
+  auto go = [&](auto kern, int team) {
+    const int threads = append_threads(team), teams = threads / team;
+    const int rc = launch_pdl(kern, dim3(s.n_items, (2 * l->H + teams - 1) / teams), dim3(threads), 0, st, p);
+    return rc != PARE_OK ? rc : launch_status();
   };
-  auto by_size = [&](auto tag) {
+  auto by_size = [&](auto tag, auto dim) {
     using E = decltype(tag);
-    const int bs = l->block_size;
-    if (l->D == 64) return bs == 16 ? go(paged_append_kernel<E, 64, 16>) : bs == 32 ? go(paged_append_kernel<E, 64, 32>) : go(paged_append_kernel<E, 64, 64>);
-    return bs == 16 ? go(paged_append_kernel<E, 128, 16>) : bs == 32 ? go(paged_append_kernel<E, 128, 32>) : go(paged_append_kernel<E, 128, 64>);
+    constexpr int kD = decltype(dim)::value;
+    if (bs == 16) return many ? go(paged_append_kernel<E, kD, 16, 4>, 64) : go(paged_append_kernel<E, kD, 16, 8>, 128);
+    if (bs == 32) return many ? go(paged_append_kernel<E, kD, 32, 4>, 128) : go(paged_append_kernel<E, kD, 32, 8>, 256);
+    return many ? go(paged_append_kernel<E, kD, 64, 4>, 256) : go(paged_append_kernel<E, kD, 64, 8>, 512);
   };
-  return l->dtype == PARE_F16 ? by_size(__half()) : by_size(__nv_bfloat16());
+  auto by_type = [&](auto dim) { return l->dtype == PARE_F16 ? by_size(__half(), dim) : by_size(__nv_bfloat16(), dim); };
+  return l->D == 64 ? by_type(std::integral_constant<int, 64>()) : by_type(std::integral_constant<int, 128>());
 }
 
 int pare_paged_dense(const pare_paged_layer* l, const pare_paged_tables* t, void* out_k, void* out_v, int64_t total, void* stream) {
@@ -470,8 +525,8 @@ int pare_paged_dense(const pare_paged_layer* l, const pare_paged_tables* t, void
   const unsigned grid = (unsigned)((total + kDenseTokens - 1) / kDenseTokens);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   auto go = [&](auto kern) {
-    kern<<<grid, kDenseThreads, 0, st>>>(p);
-    return launch_status();
+    const int rc = launch_pdl(kern, dim3(grid), dim3(kDenseThreads), 0, st, p);
+    return rc != PARE_OK ? rc : launch_status();
   };
   if (l->dtype == PARE_F16) return l->D == 64 ? go(paged_dense_kernel<__half, 64>) : go(paged_dense_kernel<__half, 128>);
   return l->D == 64 ? go(paged_dense_kernel<__nv_bfloat16, 64>) : go(paged_dense_kernel<__nv_bfloat16, 128>);
