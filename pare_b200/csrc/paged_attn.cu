@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   const int tiles = p.H * p.sub;       // tiles of eight heads per token
-  const int me = blockIdx.x * kWarps + warp;
+  const int me = warp * gridDim.x + blockIdx.x;      // a few runs spread over all SMs
   pdl_wait();
   // The last token that begins at or before this run: 32 candidates a round, the first round together with the number of units
   const int all = p.unit_start[p.T], spread = (p.T + 31) / 32;

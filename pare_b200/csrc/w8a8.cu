@@ -6,7 +6,8 @@
 // The sums are exact 32-bit integers, so neither tiles nor splits of K nor their order change a bit of the result.
 //
 // Two launches: the tokens' codes (one thread block per row), then the product.  The second starts while the first runs and fills
-// its ring with weights, which the first does not write; it waits before it touches anything else.
+// its ring with weights, which the first does not write (and what came before the first has ended); it waits before it touches
+// anything else.  A few rows take one launch (w8a8_few_kernel below).
 //
 // The product: as in w4a16_gemm.cu the 128 rows of a weight tile sit on the MMA's M axis (the TMEM lanes), activation rows on its N
 // axis, one persistent thread block per SM, each with one contiguous run of (weight tile, activation tile, 128-column unit); tiles
@@ -716,7 +717,7 @@ __global__ void __launch_bounds__(kThreads, 1) w8a8_pair_kernel(const __grid_con
 
 // ---- product of up to 16 rows, tokens quantized on the way ---------------------------------------------------------------------------------
 // Streams the weights once, and what counts besides is the number of steps that wait for one another: so one launch, in which the
-// weights are on their way from the first moment while the tokens become codes.  `splits` thread blocks (a cluster of 1, 2, 4) share a
+// weights are on their way while the tokens become codes.  `splits` thread blocks (a cluster of 1, 2, 4) share a
 // weight tile's K; each quantizes its own columns (row maxima are exchanged through shared memory), keeps their codes there in the
 // order of the MMA's operand for all its tiles, and finishes the sums of its share of the 128 weight rows with what the others send.
 //   warp 0  TMA of weights     warp 1  tcgen05.mma     warp 2  tensor memory     warps 4-11  tokens, then (4-7) the epilogue
@@ -790,6 +791,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) w8a8_few_kernel(const __grid_c
   if (warp == 0) {
     // ================= weights =================
     if (lane == 0) {
+      pdl_wait();      // whoever made the weights may be the kernel before
       const int mine = first < fp.tiles ? (fp.tiles - first + step - 1) / step * n_k : 0;
       int t = first, k = k0, s = 0, i = 0;
       uint32_t par = 1;

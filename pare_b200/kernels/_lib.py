@@ -198,19 +198,21 @@ def workspace_status(device: torch.device) -> int:
     return lib().pare_workspace_status(buf.data_ptr(), key[1])
 
 
-# Scratch memory that calls leave nothing in, one per device and stream.  Graphs never work in it: see scratch().
-_scratch: dict[tuple[int, int], torch.Tensor] = {}
+# Scratch memory that calls leave nothing in, one per thread, device and stream (a call may be two launches, and another thread's could
+# come between them on the same stream).  Graphs never work in it: see scratch().
+_scratch = threading.local()
 
 
 def scratch(device: torch.device, nbytes: int, stream: int) -> torch.Tensor:
-    """Memory for one call on the current stream of ``device``, which must be the current device.  Calls on a stream follow one
-    another, so they share it; while a graph is captured it comes from the allocator, i.e. belongs to that graph."""
+    """Memory for one call on the current stream of ``device``, which must be the current device.  A thread's calls on a stream
+    follow one another, so they share it; while a graph is captured it comes from the allocator, i.e. belongs to that graph."""
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    buffers = _scratch.__dict__
     key = (device.index, stream)
-    buf = _scratch.get(key)
+    buf = buffers.get(key)
     if buf is None or buf.numel() < nbytes:
-        _scratch[key] = buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        buffers[key] = buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
     return buf
 
 

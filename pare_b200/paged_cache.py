@@ -332,7 +332,6 @@ class PagedKVCache:
         if isinstance(new_lens, Tensor):
             if tokens is None:
                 raise ValueError("plan: the number of rows is needed when lengths are on the GPU")
-            self._lens = None
         else:
             if isinstance(new_lens, dict):
                 if any(not 0 <= r < c.max_requests for r in new_lens):
@@ -358,9 +357,8 @@ class PagedKVCache:
             new_lens = torch.tensor(new, dtype=torch.int32).to(self.device)
         step = plan_blocks(self.seq_lens, new_lens, self.block_table, self.free_blocks, self.free_count, c.block_size, tokens)
         self._state.copy_(step.words.narrow(0, step._at[2], c.max_requests + 1))
-        if lengths is not None:
-            step.lengths = lengths
-            self._lens = [a + n for a, n in lengths]
+        step.lengths = lengths
+        self._lens = None if lengths is None else [a + n for a, n in lengths]
         return step
 
     def release(self, requests: Sequence[int] | Tensor) -> None:
@@ -413,17 +411,18 @@ class PagedKVCache:
         if any(old and new for old, new in step.lengths):
             full_k, full_v = dense_blocks(layer, step, sum(old + new for old, new in step.lengths if new))
         row = ctx = 0
-        for old, new in step.lengths:
-            if not new:
-                continue
-            k, v = new_k[row:row + new], new_v[row:row + new]
-            if old:
-                full_k[ctx + old:ctx + old + new] = k
-                full_v[ctx + old:ctx + old + new] = v
-                k, v = full_k[ctx:ctx + old + new], full_v[ctx:ctx + old + new]
-            out[row:row + new] = prefill_attention(*(t.unsqueeze(0).transpose(1, 2) for t in (q[row:row + new], k, v)), scale)[0].transpose(0, 1)
-            row += new
-            ctx += old + new
+        with torch.cuda.device(self.device):
+            for old, new in step.lengths:
+                if not new:
+                    continue
+                k, v = new_k[row:row + new], new_v[row:row + new]
+                if old:
+                    full_k[ctx + old:ctx + old + new] = k
+                    full_v[ctx + old:ctx + old + new] = v
+                    k, v = full_k[ctx:ctx + old + new], full_v[ctx:ctx + old + new]
+                out[row:row + new] = prefill_attention(*(t.unsqueeze(0).transpose(1, 2) for t in (q[row:row + new], k, v)), scale)[0].transpose(0, 1)
+                row += new
+                ctx += old + new
         return out
 
     def memory_bytes(self) -> dict[str, int]:
