@@ -17,6 +17,7 @@
 // itself through a ring of its own (cp.async, no barrier between warps) and waits for nobody.  Tiles that span warps leave their
 // parts in the workspace for a second kernel.  Nothing in the workspace outlives the call, no counters: calls on any streams and
 // replays of any graphs do not meet there.
+#include <algorithm>
 #include <type_traits>
 
 #include "paged.cuh"
@@ -31,7 +32,7 @@ constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kBias = 4.f, kSlack = 11.f;
-constexpr int kMinRun = 4;                 // units of a warp's run at least
+constexpr int kMinRun = 3;                 // units of a warp's run at least
 
 template <int D>
 struct Shape {
@@ -506,10 +507,10 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
 }
 
 // Tiles that span warps.  A warp takes one piece of a tile's O (float4 per lane as the attention's lanes held it: channels
-// (D / 8) g + 2 i, + 1 x heads 2 t, 2 t + 1).  Many tiles have few parts each: a thread block per tile, a warp
-// per piece.  Few tiles have many (one sequence: 64): GROUPS warps share a piece, each every GROUPS-th part, and are added up in order.
-constexpr int kMergeGroups = 8;
-
+// (D / 8) g + 2 i, + 1 x heads 2 t, 2 t + 1).  Many tiles have few parts each: a thread block per tile, a warp per piece.  Few tiles have
+// many (one sequence: 86): GROUPS warps share a piece, each every GROUPS-th part, and are added up in order.  A warp alone gets
+// through one instruction in about eight cycles, so what is serial counts: 8 tiles of 4096 tokens, both kernels, 22.7 / 15.8 / 13.1 / 12.7 us
+// with 2 / 4 / 8 / 16 groups; 64 tiles of 32768 tokens 101 / 99 / 99 / 106 us, 108 with one.
 template <typename T, int D, int GROUPS>
 __global__ void __launch_bounds__(GROUPS > 1 ? GROUPS * 32 : D * 2) paged_merge_kernel(const PagedAttnParams p, int warps) {
   using S = Shape<D>;
@@ -610,21 +611,25 @@ int pare_paged_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h, const
                           reinterpret_cast<float*>(workspace), softmax_scale * kLog2e, T, tb->R, H, group, sub,
                           l->block_size == 16 ? 4 : l->block_size == 32 ? 5 : 6, l->num_blocks, tb->max_blocks};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  auto go = [&](auto kern, auto merge, auto merge_few, size_t smem) {
-    if (!ensure_smem_attr(reinterpret_cast<const void*>(kern), (int)smem)) return (int)PARE_ERR_CUDA;
-    int status = launch_pdl(kern, dim3(blocks), dim3(kThreads), smem, st, p);
+  auto by_dim = [&](auto tag, auto dim) {
+    using E = decltype(tag);
+    constexpr int kD = decltype(dim)::value;
+    const auto kern = paged_attn_kernel<E, kD>;
+    if (!ensure_smem_attr(reinterpret_cast<const void*>(kern), (int)Shape<kD>::kSmem)) return (int)PARE_ERR_CUDA;
+    int status = launch_pdl(kern, dim3(blocks), dim3(kThreads), Shape<kD>::kSmem, st, p);
     if (status != PARE_OK) return status;
-    const int jobs = T * H * sub, most = 16 * blocks;
-    status = 2 * jobs <= blocks ? launch_pdl(merge_few, dim3(jobs, D / 16), dim3(kMergeGroups * 32), 0, st, p, blocks * kWarps)
-                            : launch_pdl(merge, dim3(jobs < most ? jobs : most), dim3(D * 2), 0, st, p, blocks * kWarps);
+    const int jobs = T * H * sub, sms = blocks / 2, warps = blocks * kWarps;
+    auto merge = [&](auto kernel, int groups) {
+      return groups > 1 ? launch_pdl(kernel, dim3(jobs, kD / 16), dim3(groups * 32), 0, st, p, warps)
+                        : launch_pdl(kernel, dim3(std::min(jobs, 32 * sms)), dim3(2 * kD), 0, st, p, warps);
+    };
+    if (8 * jobs <= sms) status = merge(paged_merge_kernel<E, kD, 16>, 16);
+    else if (jobs <= sms) status = merge(paged_merge_kernel<E, kD, 8>, 8);
+    else status = merge(paged_merge_kernel<E, kD, 1>, 1);
     return status != PARE_OK ? status : launch_status();
   };
-  auto by_dim = [&](auto tag) {
-    using E = decltype(tag);
-    return D == 64 ? go(paged_attn_kernel<E, 64>, paged_merge_kernel<E, 64, 1>, paged_merge_kernel<E, 64, kMergeGroups>, Shape<64>::kSmem)
-                   : go(paged_attn_kernel<E, 128>, paged_merge_kernel<E, 128, 1>, paged_merge_kernel<E, 128, kMergeGroups>, Shape<128>::kSmem);
-  };
-  return l->dtype == PARE_F16 ? by_dim(__half()) : by_dim(__nv_bfloat16());
+  auto by_type = [&](auto dim) { return l->dtype == PARE_F16 ? by_dim(__half(), dim) : by_dim(__nv_bfloat16(), dim); };
+  return D == 64 ? by_type(std::integral_constant<int, 64>()) : by_type(std::integral_constant<int, 128>());
 }
 
 }  // extern "C"
