@@ -126,6 +126,9 @@ __device__ __forceinline__ int64_t run_units(int64_t total, int warps) {
 template <typename T, int D>
 struct Tile {
   using S = Shape<D>;
+  // Rounding a probability to fp16 is off by 2^-11 of it: nothing beside a bf16 result, as much as the rounding of an fp16 result.
+  // There it is two numbers, the second what the first left (16 x 32768 tokens: 105 us instead of 98).
+  static constexpr bool kTwoTerms = std::is_same<T, __half>::value;
   static constexpr int kJ = D / 64;              // 16-byte chunks of a key row per lane
   static constexpr int kW = D / 32;              // words of four value channels per lane and token: channels (D / 8) g ..
   uint32_t qh[kJ][4][2];                         // query operand, fp16: channels 16 (t + 4 j) + 4 w + {0, 1}, {2, 3} of head g
@@ -246,7 +249,13 @@ struct Tile {
       if (g + 8 >= seen) s[2] = s[3] = -INFINITY;
     }
     softmax(s);
-    const uint32_t p0 = transpose8x8(pack_half2(s[0], s[1])), p1 = transpose8x8(pack_half2(s[2], s[3]));
+    const uint32_t h0 = pack_half2(s[0], s[1]), h1 = pack_half2(s[2], s[3]), p0 = transpose8x8(h0), p1 = transpose8x8(h1);
+    uint32_t r0 = 0, r1 = 0;       // what the rounding left
+    if constexpr (kTwoTerms) {
+      const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h0)), b = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+      r0 = transpose8x8(pack_half2(s[0] - a.x, s[1] - a.y));
+      r1 = transpose8x8(pack_half2(s[2] - b.x, s[3] - b.y));
+    }
     const uint32_t vbase = stage + kUnit * D;
     uint32_t v[4][kW];   // tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 x channels (D / 8) g ..
 #pragma unroll
@@ -265,11 +274,15 @@ struct Tile {
       // the four channels of two neighbouring tokens side by side, then to fp16 pairs (token, next token)
       const uint32_t ab0 = __byte_perm(v[0][w], v[1][w], 0x5140) ^ 0x80808080u, ab1 = __byte_perm(v[0][w], v[1][w], 0x7362) ^ 0x80808080u;
       const uint32_t cd0 = __byte_perm(v[2][w], v[3][w], 0x5140) ^ 0x80808080u, cd1 = __byte_perm(v[2][w], v[3][w], 0x7362) ^ 0x80808080u;
+      const uint32_t a[4] = {codes_to_half2<0x4140>(ab0), codes_to_half2<0x4342>(ab0), codes_to_half2<0x4140>(cd0), codes_to_half2<0x4342>(cd0)};
+      const uint32_t b[4] = {codes_to_half2<0x4140>(ab1), codes_to_half2<0x4342>(ab1), codes_to_half2<0x4140>(cd1), codes_to_half2<0x4342>(cd1)};
       float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-      mma16816<__half>(x, codes_to_half2<0x4140>(ab0), codes_to_half2<0x4342>(ab0), codes_to_half2<0x4140>(cd0),
-                       codes_to_half2<0x4342>(cd0), p0, p1);
-      mma16816<__half>(y, codes_to_half2<0x4140>(ab1), codes_to_half2<0x4342>(ab1), codes_to_half2<0x4140>(cd1),
-                       codes_to_half2<0x4342>(cd1), p0, p1);
+      mma16816<__half>(x, a[0], a[1], a[2], a[3], p0, p1);
+      mma16816<__half>(y, b[0], b[1], b[2], b[3], p0, p1);
+      if constexpr (kTwoTerms) {
+        mma16816<__half>(x, a[0], a[1], a[2], a[3], r0, r1);
+        mma16816<__half>(y, b[0], b[1], b[2], b[3], r0, r1);
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         o[2 * w][i] = fmaf(vs, x[i], o[2 * w][i]);
@@ -279,8 +292,7 @@ struct Tile {
   }
 
   // Up to 16 open tokens in 16 bits: the keys in one stage of the ring, the values in another.  Hidden rows (later tokens,
-  // leftovers) were not loaded, they are zeros: what lies there may be infinite.  bf16 probabilities have too few digits: value +
-  // what its rounding left.
+  // leftovers) were not loaded, they are zeros: what lies there may be infinite.  Probabilities in two terms, in the rows' type.
   __device__ __forceinline__ void open_unit(uint32_t stage_k, uint32_t stage_v, const T* q_row, float scale_log2, int seen, int lane) {
     const int g = lane >> 2, t = lane & 3;
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
@@ -308,10 +320,14 @@ struct Tile {
     if (g >= seen) s[0] = s[1] = -INFINITY;
     if (g + 8 >= seen) s[2] = s[3] = -INFINITY;
     softmax(s);
-    uint32_t p0, p1, r0 = 0, r1 = 0;
+    uint32_t p0, p1, r0, r1;
     if constexpr (std::is_same<T, __half>::value) {
-      p0 = transpose8x8(pack_half2(s[0], s[1]));
-      p1 = transpose8x8(pack_half2(s[2], s[3]));
+      const uint32_t a = pack_half2(s[0], s[1]), b = pack_half2(s[2], s[3]);
+      const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&a)), fb = __half22float2(*reinterpret_cast<const __half2*>(&b));
+      p0 = transpose8x8(a);
+      p1 = transpose8x8(b);
+      r0 = transpose8x8(pack_half2(s[0] - fa.x, s[1] - fa.y));
+      r1 = transpose8x8(pack_half2(s[2] - fb.x, s[3] - fb.y));
     } else {
       const uint32_t a = pack_bf2(s[0], s[1]), b = pack_bf2(s[2], s[3]);
       auto lo = [](uint32_t w) { return __uint_as_float(w << 16); };
@@ -335,7 +351,7 @@ struct Tile {
         const uint32_t a0 = __byte_perm(a[w], b[w], 0x5410), a1 = __byte_perm(a[w], b[w], 0x7632);
         const uint32_t a2 = __byte_perm(d[w], e[w], 0x5410), a3 = __byte_perm(d[w], e[w], 0x7632);
         mma16816<T>(o[4 * c + w], a0, a1, a2, a3, p0, p1);
-        if constexpr (!std::is_same<T, __half>::value) mma16816<T>(o[4 * c + w], a0, a1, a2, a3, r0, r1);
+        mma16816<T>(o[4 * c + w], a0, a1, a2, a3, r0, r1);
       }
     }
   }
@@ -372,13 +388,17 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem + warp * S::kRing);
   Tile<T, D> tile;
 
-  // where this lane's 16-byte chunks of a unit go in a stage (chunk e * 32 + lane of the keys and of the values)
-  uint32_t at_k[S::kChunks], at_v[S::kChunks];
+  // Where this lane's 16-byte chunks of a unit go in a stage: chunk e * 32 + lane of the keys at at_k + 512 e, of the values at
+  // at_v[e & 1] + 512 e (the pattern that spreads rows over banks repeats after two rounds)
+  uint32_t at_k, at_v[2];
+  {
+    const int row = lane / (D / 16), c = lane % (D / 16);
+    at_k = row * D + (D == 128 ? c ^ ((row & 1) << 2) : c) * 16;
 #pragma unroll
-  for (int e = 0; e < S::kChunks; ++e) {
-    const int row = (e * 32 + lane) / (D / 16), c = (e * 32 + lane) % (D / 16);
-    at_k[e] = row * D + (D == 128 ? c ^ ((row & 1) << 2) : c) * 16;
-    at_v[e] = kUnit * D + row * D + (D == 128 ? c ^ (((row >> 1) & 3) << 1) : c ^ ((row >> 1) & 3)) * 16;
+    for (int e = 0; e < 2; ++e) {
+      const int r = row + e * (512 / D);
+      at_v[e] = kUnit * D + row * D + (D == 128 ? c ^ (((r >> 1) & 3) << 1) : c ^ ((r >> 1) & 3)) * 16;
+    }
   }
 
   int first_unit = p.unit_start[t], units = p.unit_start[t + 1] - first_unit;
@@ -421,9 +441,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
         const int8_t* sk = p.k_codes + src + lane * 16;
         const int8_t* sv = p.v_codes + src + lane * 16;
 #pragma unroll
-        for (int e = 0; e < S::kChunks; ++e) cp_async16(dst + at_k[e], sk + e * 512, bytes);
+        for (int e = 0; e < S::kChunks; ++e) cp_async16(dst + at_k + e * 512, sk + e * 512, bytes);
 #pragma unroll
-        for (int e = 0; e < S::kChunks; ++e) cp_async16(dst + at_v[e], sv + e * 512, bytes);
+        for (int e = 0; e < S::kChunks; ++e) cp_async16(dst + at_v[e & 1] + e * 512, sv + e * 512, bytes);
       } else if (i < entries) {
         const int from = (j0 + n8 - nq_units + (i - n8) / 2) * kUnit, seen = pos + 1 - nq - from;   // first row, visible rows
         const bool values = (i - n8) & 1;

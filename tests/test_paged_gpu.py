@@ -76,10 +76,11 @@ class _Model:
         p = torch.softmax(s, -1)
         o = p @ v
         # Error of a score: 2 d + 2 roundings of fp32 sums of |q| |k|, two scale products; doubled for the softmax's numerator and
-        # denominator.  Probabilities: fp16 rounding 2^-11 (bf16 rows: two terms, less), ex2 and the rescales below 2^-19; those
-        # that are subnormal in fp16 lose at most 2^-25 each where the largest is at least 2^4.  Sums of the products: fp32.
+        # denominator.  Probabilities: fp16 rounding 2^-11 for a bf16 result, two terms (2^-16 and less) in fp16 and for open rows;
+        # ex2 and the rescales below 2^-19; those that are subnormal in fp16 lose at most 2^-25 each where the largest is at
+        # least 2^4.  Sums of the products: fp32.
         mag = (qq.abs() @ k.abs().transpose(1, 2)).amax(-1, keepdim=True) * scale
-        rel = 2.0 ** -11 + 2 * ((2 * self.d + 8) * 2.0 ** -24 * mag) + 2.0 ** -18
+        rel = (2.0 ** -11 if self.dtype is torch.bfloat16 else 2.0 ** -16) + 2 * ((2 * self.d + 8) * 2.0 ** -24 * mag) + 2.0 ** -18
         out_step = torch.finfo(self.dtype).eps / 2
         bound = rel * (p @ v.abs()) + seen * 2.0 ** -29 * v.abs().amax(1, keepdim=True) + out_step * o.abs() * 1.01 + 1e-30
         if self.dtype is torch.float16:
