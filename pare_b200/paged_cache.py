@@ -92,14 +92,19 @@ class PagedStep:
 
     __slots__ = ("words", "requests", "tokens", "block_size", "block_table", "device", "lengths", "_at", "_ld", "_struct", "_c")
 
-    def __init__(self, words: Tensor, at: tuple[int, ...], requests: int, tokens: int, block_size: int, block_table: Tensor) -> None:
+    def __init__(self, words: Tensor, at: tuple[int, ...], requests: int, tokens: int, block_size: int, block_table: Tensor, ld: int) -> None:
         self.words, self._at, self.device = words, at, words.device
-        self.requests, self.tokens, self.block_size, self.block_table = requests, tokens, block_size, block_table
+        self.requests, self.tokens, self.block_size, self.block_table, self._ld = requests, tokens, block_size, block_table, ld
         self.lengths: list[tuple[int, int]] | None = None    # (old, new) per request where the host knows them
-        width = block_table.shape[1]
-        self._ld = max(block_table.stride(0), width)
-        self._struct = _lib.PagedTablesStruct(words.data_ptr(), block_table.data_ptr(), self._ld, width, requests, tokens, block_size)
-        self._c = ctypes.addressof(self._struct)
+        self._c = 0
+
+    def _tables(self) -> int:
+        """Address of the step as the C entries take it."""
+        if not self._c:
+            self._struct = _lib.PagedTablesStruct(self.words.data_ptr(), self.block_table.data_ptr(), self._ld, self.block_table.shape[1],
+                                                  self.requests, self.tokens, self.block_size)
+            self._c = ctypes.addressof(self._struct)
+        return self._c
 
     @property
     def query_start(self) -> Tensor:
@@ -173,21 +178,22 @@ def plan_blocks(seq_lens: Tensor, new_lens: Tensor, block_table: Tensor, free_bl
     dev = seq_lens.device
     if dev.type != "cuda":
         raise RuntimeError("plan_blocks runs on CUDA tensors only")
-    n = seq_lens.shape[0] if seq_lens.dim() == 1 else 0
-    per_request, capacity = (n,), free_blocks.numel()
-    _ints(seq_lens, per_request, dev, "seq_lens")
-    _ints(new_lens, per_request, dev, "new_lens")
-    _ints(free_count, (1,), dev, "free_count")
-    _ints(free_blocks, (capacity,), dev, "free_blocks")
-    rows = block_table.shape
-    if (block_table.dtype is not torch.int32 or len(rows) != 2 or rows[0] != n or rows[1] == 0 or block_table.device != dev
-            or not (block_table.is_contiguous() or (block_table.stride(1) == 1 and block_table.stride(0) >= rows[1]))):
-        raise ValueError(f"block_table must be int32 [{n}, blocks per request] with adjacent columns on {dev}")
+    shape, rows, capacity, i32 = seq_lens.shape, block_table.shape, free_blocks.numel(), torch.int32
+    n = shape[0] if len(shape) == 1 else 0
+    for t, want, what in ((seq_lens, (n,), "seq_lens"), (new_lens, (n,), "new_lens"), (free_count, (1,), "free_count"),
+                          (free_blocks, (capacity,), "free_blocks")):
+        if t.dtype is not i32 or t.shape != want or t.device != dev or not t.is_contiguous():
+            _ints(t, want, dev, what)
+    ld = rows[1] if len(rows) == 2 else 0
+    if block_table.dtype is not i32 or ld == 0 or rows[0] != n or block_table.device != dev or not block_table.is_contiguous():
+        if block_table.dtype is not i32 or ld == 0 or rows[0] != n or block_table.device != dev or block_table.stride(1) != 1 or block_table.stride(0) < ld:
+            raise ValueError(f"block_table must be int32 [{n}, blocks per request] with adjacent columns on {dev}")
+        ld = block_table.stride(0)
     nbytes, at = _step_layout(n, tokens, block_size)
     words = seq_lens.new_empty(nbytes // 4)
-    step = PagedStep(words, at, n, tokens, block_size, block_table)
+    step = PagedStep(words, at, n, tokens, block_size, block_table, ld)
     _call(dev, _lib.lib().pare_paged_plan, "pare_paged_plan", seq_lens.data_ptr(), new_lens.data_ptr(), n, block_table.data_ptr(),
-          step._ld, rows[1], free_blocks.data_ptr(), capacity, free_count.data_ptr(), block_size, tokens, words.data_ptr(), nbytes)
+          ld, rows[1], free_blocks.data_ptr(), capacity, free_count.data_ptr(), block_size, tokens, words.data_ptr(), nbytes)
     return step
 
 
@@ -212,7 +218,7 @@ def append_blocks(layer: PagedLayer, step: PagedStep, k: Tensor, v: Tensor) -> N
     k, v = _rows(k, step.tokens, layer.heads, layer, "k"), _rows(v, step.tokens, layer.heads, layer, "v")
     ks, vs = k.stride(), v.stride()
     _call(layer.device, _lib.lib().pare_paged_append, "pare_paged_append", k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1],
-          layer._c, step._c)
+          layer._c, step._tables())
 
 
 def dense_blocks(layer: PagedLayer, step: PagedStep, total: int) -> tuple[Tensor, Tensor]:
@@ -222,7 +228,7 @@ def dense_blocks(layer: PagedLayer, step: PagedStep, total: int) -> tuple[Tensor
     _fits(layer, step)
     k = layer.tail_k.new_empty(total, layer.heads, layer.head_dim)
     v = torch.empty_like(k)
-    _call(layer.device, _lib.lib().pare_paged_dense, "pare_paged_dense", layer._c, step._c, k.data_ptr(), v.data_ptr(), total)
+    _call(layer.device, _lib.lib().pare_paged_dense, "pare_paged_dense", layer._c, step._tables(), k.data_ptr(), v.data_ptr(), total)
     return k, v
 
 
@@ -254,7 +260,7 @@ def attend_blocks(layer: PagedLayer, step: PagedStep, q: Tensor, scale: float | 
             return attend_blocks(layer, step, q, scale, out)
     stream, nbytes, qs, os = _lib.current_stream(dev), _attn_workspace(d, dev.index), q.stride(), out.stride()
     ws = _lib.scratch(dev, nbytes, stream)
-    status = _lib.lib().pare_paged_attn(q.data_ptr(), qs[0], qs[1], layer._c, step._c, hq, out.data_ptr(), os[0], os[1],
+    status = _lib.lib().pare_paged_attn(q.data_ptr(), qs[0], qs[1], layer._c, step._tables(), hq, out.data_ptr(), os[0], os[1],
                                         1.0 / math.sqrt(d) if scale is None else scale, ws.data_ptr(), nbytes, stream)
     if status:
         _lib.check(status, "pare_paged_attn")
