@@ -300,7 +300,7 @@ int pare_rope(const void* x, int64_t stride_b, int64_t stride_h, int64_t stride_
  * themselves are multiplied:
  *   x~ = x, or dtype(x / input_scale);  step = max(max_k |x~|, 1e-6) / 127;  c = round_half_even(x~ / step) in [-127, 127]
  *   y = dtype((sum_k c q - zero sum_k c) * step * scale + bias)
- *   x            [M, ldx]  F16 or BF16; 16-byte aligned with ldx % 8 == 0 if M <= 16 and K % 8 == 0
+ *   x            [M, ldx]  F16 or BF16; 16-byte aligned with ldx % 8 == 0 where no workspace is needed
  *   weight       [N, ldw]  int8, ldw >= K a multiple of 16, 16-byte aligned
  *   scale, zero  [N] float32 (zero may be NULL = 0)
  *   input_scale  optional [K] float32, divides the activations first (the quotient rounded to their dtype)

@@ -718,9 +718,11 @@ __global__ void __launch_bounds__(kThreads, 1) w8a8_pair_kernel(const __grid_con
 // ---- product of up to 16 rows, tokens quantized on the way ---------------------------------------------------------------------------------
 // Streams the weights once, and what counts besides is the number of steps that wait for one another: so one launch, in which the
 // weights are on their way while the tokens become codes.  `splits` thread blocks (a cluster of 1, 2, 4) share a
-// weight tile's K; each quantizes its own columns (row maxima are exchanged through shared memory), keeps their codes there in the
-// order of the MMA's operand for all its tiles, and finishes the sums of its share of the 128 weight rows with what the others send.
+// weight tile's K; each quantizes its own columns (and looks at all of them for the rows' maxima), keeps their codes in shared memory in
+// the order of the MMA's operand for all its tiles, and finishes the sums of its share of the 128 weight rows with what the others send.
 //   warp 0  TMA of weights     warp 1  tcgen05.mma     warp 2  tensor memory     warps 4-11  tokens, then (4-7) the epilogue
+// CODED: the tokens were quantized by a launch before this one (where that is too much to do beside the weights) and their codes
+// come by TMA; what is left is the sums' short way through the cluster.
 constexpr int kFewRows = 16;
 constexpr int kFewThreads = 384;
 constexpr int kFewCodes = 256;                        // threads that quantize
@@ -734,26 +736,27 @@ struct FewParams {
   const void* x;
   int64_t ldx;
   const float* input_scale;
-  int K, tiles, splits;
+  int K, tiles, splits, stages;
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kFewThreads, 1) w8a8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const FewParams fp) {
+template <typename T, bool CODED>
+__global__ void __launch_bounds__(kFewThreads, 1) w8a8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
+                                                                  const FewParams fp) {
   extern __shared__ unsigned char smem_raw[];
   pdl_launch_dependents();
   __shared__ int s_failed;
-  __shared__ uint32_t s_top[4][kFewRows];             // row maxima, from each thread block of the cluster
-  __shared__ int s_sum[4][kFewRows];                  // sums of codes likewise
+  __shared__ uint32_t s_top[kFewRows];                // row maxima
+  __shared__ int s_sum[4][kFewRows];                  // sums of codes, from each thread block of the cluster
   __shared__ float s_step[kFewRows];
   __shared__ int4 s_in[3 * 128 / 4 * 4];              // sums from the others: [sender][4][rows of this share] of four activation rows
   __shared__ uint64_t s_bars[2 * kMaxStages + 8];
   __shared__ uint32_t s_tmem;
   const W8Params& p = fp.w;
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int ku = p.ku, stages = p.stages, M = p.M, splits = fp.splits;
+  const int ku = p.ku, stages = fp.stages, M = p.M, splits = fp.splits;
   const uint32_t w_ring = s_u32(smem), codes = w_ring + stages * kWBytes;
   const uint32_t full = s_u32(s_bars), empty = full + kMaxStages * 8, acc_full = empty + kMaxStages * 8, acc_empty = acc_full + 16,
-                 mma_done = acc_empty + 16, x_ready = mma_done + 8, tops_in = x_ready + 8, sums_in = tops_in + 8;
+                 mma_done = acc_empty + 16, x_ready = mma_done + 8, sums_in = x_ready + 8;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = splits > 1 ? (int)cluster_rank() : 0;
   const int k0 = ku * rank / splits, k1 = ku * (rank + 1) / splits, n_k = k1 - k0;
@@ -772,12 +775,12 @@ __global__ void __launch_bounds__(kFewThreads, 1) w8a8_few_kernel(const __grid_c
       bar_init(acc_empty + i * 8, 4);
     }
     bar_init(mma_done, 1);
-    bar_init(x_ready, kFewCodes / 32);
-    bar_init(tops_in, splits);
+    bar_init(x_ready, CODED ? 1 : kFewCodes / 32);
     bar_init(sums_in, splits > 1 ? (splits - 1) * (4 / splits) : 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (threadIdx.x < 4 * kFewRows) (&s_top[0][0])[threadIdx.x] = 0, (&s_sum[0][0])[threadIdx.x] = 0;
+  if (threadIdx.x < kFewRows) s_top[threadIdx.x] = 0;
+  if (threadIdx.x < 4 * kFewRows) (&s_sum[0][0])[threadIdx.x] = 0;
   if (warp == 2) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_u32(&s_tmem)), "r"(kFewTmem) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -791,7 +794,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) w8a8_few_kernel(const __grid_c
   if (warp == 0) {
     // ================= weights =================
     if (lane == 0) {
-      pdl_wait();      // whoever made the weights may be the kernel before
+      if (!CODED) pdl_wait();      // whoever made the weights may be the kernel before
       const int mine = first < fp.tiles ? (fp.tiles - first + step - 1) / step * n_k : 0;
       int t = first, k = k0, s = 0, i = 0;
       uint32_t par = 1;
@@ -838,77 +841,70 @@ __global__ void __launch_bounds__(kFewThreads, 1) w8a8_few_kernel(const __grid_c
     // ================= tokens =================
     pdl_wait();
     const int tid = threadIdx.x - 4 * 32;
-    int per = kFewCodes;                              // threads per row
-    for (int r = 1; r < M; r <<= 1) per >>= 1;
-    const int m = tid / per, at = tid % per, c0 = k0 * kUnitK, c1 = min(k1 * kUnitK, fp.K);
-    const T* row = reinterpret_cast<const T*>(fp.x) + m * fp.ldx;
-    // all of a row if that is little (then nobody has to ask for a maximum), else this thread block's columns of it
-    const bool whole = splits == 1 || (fp.K / 8 + per - 1) / per <= kFewVecs;
-    const int lo = whole ? 0 : c0, hi = whole ? fp.K : c1;
-    uint4 v[kFewVecs];
-    uint32_t top = 0;
-    if (m < M) {
-#pragma unroll
-      for (int i = 0; i < kFewVecs; ++i) {
-        const int c = lo + (i * per + at) * 8;
-        v[i] = c < hi ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
+    if constexpr (CODED) {
+      if (tid == 0) {
+        bar_expect(x_ready, n_k * kFewUnitBytes);
+        for (int u = 0; u < n_k; ++u) tma_tile(codes + u * kFewUnitBytes, &tm_x, (k0 + u) * kUnitK, 0, x_ready);
       }
-      if (fp.input_scale) {
+      if (tid < M) s_step[tid] = p.step[tid];
+      asm volatile("bar.sync 2, 256;" ::: "memory");
+      if (splits > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    } else {
+      int per = kFewCodes;                              // threads per row, at least sixteen
+      for (int r = 1; r < M; r <<= 1) per >>= 1;
+      const int m = tid / per, at = tid % per, c0 = k0 * kUnitK, c1 = min(k1 * kUnitK, fp.K);
+      const T* row = reinterpret_cast<const T*>(fp.x) + m * fp.ldx;
+      uint4 v[kFewVecs];
+      uint32_t top = 0;
+      if (m < M) {
 #pragma unroll
         for (int i = 0; i < kFewVecs; ++i) {
-          const int c = lo + (i * per + at) * 8;
-          T* e = reinterpret_cast<T*>(&v[i]);
-          if (c < hi) {
+          const int c = (i * per + at) * 8;
+          v[i] = c < fp.K ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
+        }
+        if (fp.input_scale) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) e[j] = smoothed<T>(e[j], fp.input_scale, c + j);
+          for (int i = 0; i < kFewVecs; ++i) {
+            const int c = (i * per + at) * 8;
+            T* e = reinterpret_cast<T*>(&v[i]);
+            if (c < fp.K) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) e[j] = smoothed<T>(e[j], fp.input_scale, c + j);
+            }
           }
         }
+#pragma unroll
+        for (int i = 0; i < kFewVecs; ++i) top = __vmaxu2(top, q8::magnitudes(v[i]));
+        top = max(top & 0xffffu, top >> 16);
       }
 #pragma unroll
-      for (int i = 0; i < kFewVecs; ++i) top = __vmaxu2(top, q8::magnitudes(v[i]));
-      top = max(top & 0xffffu, top >> 16);
-    }
+      for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));      // at least sixteen threads share a row
+      if (m < M && (lane & 15) == 0) atomicMax(&s_top[m], top);
+      asm volatile("bar.sync 2, 256;" ::: "memory");
+      if (splits > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+      if (m < M) {
+        top = s_top[m];
+        const uint16_t bits = (uint16_t)top;
+        const float amax = to_float<T>(*reinterpret_cast<const T*>(&bits));
+        const q8::Grid grid(amax < 1e-6f ? 1e-6f : amax);
+        if (at == 0) s_step[m] = grid.finite ? grid.step : __int_as_float(0x7fffffff);
+        int sum = 0;
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));      // at least sixteen threads share a row
-    if (m < M && (lane & 15) == 0) atomicMax(&s_top[rank][m], top);
-    asm volatile("bar.sync 2, 256;" ::: "memory");
-    if (splits > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-    if (!whole) {      // to everybody, this thread block among them
-      if (tid < kFewRows)
-        for (int q = 0; q < splits; ++q)
-          if (q != rank)
-            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(in_block(s_u32(&s_top[rank][tid]), q)), "r"(s_top[rank][tid]) : "memory");
-      if (warp == 4) {
-        asm volatile("fence.acq_rel.cluster;" ::: "memory");
-        __syncwarp();
-        if (lane < splits) arrive_at(in_block(tops_in, lane));
+        for (int i = 0; i < kFewVecs; ++i) {
+          const int c = (i * per + at) * 8;
+          if (c < c0 || c >= c1) continue;
+          const uint2 o = grid.codes<T>(v[i]);
+          sum = __dp4a((int)o.y, 0x01010101, __dp4a((int)o.x, 0x01010101, sum));
+          const int u = (c - c0) / kUnitK, chunk = (c % kUnitK) / 16;
+          asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(codes + u * kFewUnitBytes + m * kUnitK + ((chunk ^ (m & 7)) << 4) + (c & 8)), "r"(o.x), "r"(o.y)
+                       : "memory");
+        }
+        if (p.zero) atomicAdd(&s_sum[rank][m], sum);
       }
-      bar_wait_cluster(tops_in, 0, status, dead);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      asm volatile("bar.sync 2, 256;" ::: "memory");    // steps and sums are there for the epilogue
+      if (lane == 0) bar_arrive(x_ready);
     }
-    if (m < M) {
-      top = s_top[rank][m];
-      if (!whole)
-        for (int q = 0; q < splits; ++q) top = max(top, s_top[q][m]);
-      const uint16_t bits = (uint16_t)top;
-      const float amax = to_float<T>(*reinterpret_cast<const T*>(&bits));
-      const q8::Grid grid(amax < 1e-6f ? 1e-6f : amax);
-      if (at == 0) s_step[m] = grid.finite ? grid.step : __int_as_float(0x7fffffff);
-      int sum = 0;
-#pragma unroll
-      for (int i = 0; i < kFewVecs; ++i) {
-        const int c = lo + (i * per + at) * 8;
-        if (c < c0 || c >= c1) continue;
-        const uint2 o = grid.codes<T>(v[i]);
-        sum = __dp4a((int)o.y, 0x01010101, __dp4a((int)o.x, 0x01010101, sum));
-        const int u = (c - c0) / kUnitK, chunk = (c % kUnitK) / 16;
-        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(codes + u * kFewUnitBytes + m * kUnitK + ((chunk ^ (m & 7)) << 4) + (c & 8)), "r"(o.x), "r"(o.y)
-                     : "memory");
-      }
-      if (p.zero) atomicAdd(&s_sum[rank][m], sum);
-    }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    asm volatile("bar.sync 2, 256;" ::: "memory");    // steps and sums are there for the epilogue
-    if (lane == 0) bar_arrive(x_ready);
 
     if (warp < 8) {
       // ================= epilogue =================
@@ -937,7 +933,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) w8a8_few_kernel(const __grid_c
               asm volatile("st.shared::cluster.v4.s32 [%0], {%1, %2, %3, %4};" ::"r"(to + (slot(rank, owner) + i * share * 32) * 16), "r"(a[4 * i]),
                            "r"(a[4 * i + 1]), "r"(a[4 * i + 2]), "r"(a[4 * i + 3])
                            : "memory");
-            if (p.zero && q4 % share == 0 && lane < kFewRows)
+            if (!CODED && p.zero && q4 % share == 0 && lane < kFewRows)
               asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(in_block(s_u32(&s_sum[rank][lane]), owner)), "r"(s_sum[rank][lane]) : "memory");
             if (bad && lane == 0)
               asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(in_block(s_u32(&s_failed), owner)), "r"((int)PARE_ERR_TIMEOUT) : "memory");
@@ -959,15 +955,16 @@ __global__ void __launch_bounds__(kFewThreads, 1) w8a8_few_kernel(const __grid_c
               a[4 * i + 3] += v.w;
             }
           }
-          if (p.zero) {        // sums over all of K in this warp's own copy
+          if (!CODED && p.zero) {        // sums over all of K in this warp's own copy
             int all = 0;
             if (lane < kFewRows)
               for (int q = 0; q < splits; ++q) all += s_sum[q][lane];
             epi.row_sum = all;
           }
-        } else if (p.zero) {
+        } else if (!CODED && p.zero) {
           epi.row_sum = lane < kFewRows ? s_sum[0][lane] : 0;
         }
+        if (CODED && p.zero) epi.row_sum = lane < M ? p.sums[lane] : 0;
         epi.bad = bad;
         epi.store16(a, 0, M, s_step);
       }
@@ -1012,21 +1009,22 @@ int resident_clusters(const void* kern, int size, int threads, int smem, int (&c
   return cached[dev] - 1;
 }
 
-// Up to 16 rows: the kernel that quantizes on the way, if a thread block's codes fit beside a ring of weights and its threads have little to
-// quantize: four vectors of eight columns each, or eight if that is whole rows and no maxima are exchanged.  Measured against the
-// two launches: 4096 x 4096, 1 / 4 / 8 / 16 rows 7.9 / 9.0 / 10.6 / 12.9 us (10.7 / 10.7 / 10.9 / 11.8); 28672 x 4096, 1 / 4 rows 22.4 / 25.9
-// (26.2 / 25.2).  K is shared by as many thread blocks (4, 2) as keep every SM to one tile.
+// Up to 16 rows, if a thread block's codes fit beside a ring of weights.  The tokens are quantized on the way where a thread has at most
+// eight vectors of eight columns to look at (4 rows of 4096): one launch, 1 / 2 / 4 rows of 4096 x 4096 8.0 / 8.3 / 9.6 us, 28672 x 4096 21.9 /
+// 22.4 / 24.4; in a launch of their own 8.8 / 8.8 / 8.8 and 23.6 / 23.9 / 24.3, and the same up to 16 rows (8 rows on the way: 11.7).
+// K is shared by as many thread blocks (4, 2) as keep every SM to one tile.
 struct FewPlan {
   int splits, tiles, blocks, stages, units;      // splits 0: not this kernel
+  bool coded;                                    // tokens are quantized by a launch of their own
 };
 constexpr int kFewSmem = 216 * 1024;
 
 FewPlan few_plan(int M, int N, int K) {
   FewPlan f{};
-  if (M > kFewRows || K % 8) return f;
+  if (M > kFewRows) return f;
   const int ku = (K + kUnitK - 1) / kUnitK;
   f.tiles = (N + kRows - 1) / kRows;
-  const void* kern = reinterpret_cast<const void*>(w8a8_few_kernel<__half>);
+  const void* kern = reinterpret_cast<const void*>(w8a8_few_kernel<__half, false>);
   static int cached4[64] = {}, cached2[64] = {};
   int splits = 1;
   if (ku >= 8 && f.tiles <= sm_count() / 2 && ensure_smem_attr(kern, kFewSmem)) {
@@ -1036,8 +1034,8 @@ FewPlan few_plan(int M, int N, int K) {
   f.units = (ku + splits - 1) / splits;
   int per = kFewCodes;      // threads per row
   for (int r = 1; r < M; r <<= 1) per >>= 1;
-  const int whole = (K / 8 + per - 1) / per, share = (f.units * (kUnitK / 8) + per - 1) / per;      // vectors of eight columns per thread
-  if (f.units > kFewMaxUnits || !(share <= kFewVecs / 2 || (splits > 1 && whole <= kFewVecs))) return f;
+  if (f.units > kFewMaxUnits) return f;
+  f.coded = K % 8 || (K / 8 + per - 1) / per > kFewVecs;
   f.splits = splits;
   f.blocks = splits > 1 ? f.tiles * splits : f.tiles < sm_count() ? f.tiles : sm_count();
   f.stages = (kFewSmem - 1024 - f.units * kFewUnitBytes) / kWBytes;
@@ -1140,8 +1138,10 @@ extern "C" {
 using namespace pare;
 
 size_t pare_w8a8_workspace_bytes(int M, int N, int K) {
-  if (M <= 0 || N <= 0 || K <= 0 || K > kMaxK || few_plan(M, N, K).splits) return 0;
-  return W8Space(w8_plan(M, N, K), M, K).bytes;
+  if (M <= 0 || N <= 0 || K <= 0 || K > kMaxK) return 0;
+  const FewPlan f = few_plan(M, N, K);
+  if (f.splits && !f.coded) return 0;
+  return W8Space(f.splits ? W8Plan{} : w8_plan(M, N, K), M, K).bytes;
 }
 
 int pare_w8a8_forward(const void* x, int x_dtype, int64_t ldx, const int8_t* weight, int64_t ldw, const float* scale, const float* zero,
@@ -1155,7 +1155,7 @@ int pare_w8a8_forward(const void* x, int x_dtype, int64_t ldx, const int8_t* wei
   const FewPlan f = few_plan(M, N, K);
   const W8Plan g = f.splits ? W8Plan{} : w8_plan(M, N, K);
   const W8Space sp(g, M, K);
-  if (f.splits) {
+  if (f.splits && !f.coded) {
     PARE_REQUIRE(aligned16(x) && (M == 1 || ldx % 8 == 0), PARE_ERR_ALIGN);
   } else {
     PARE_REQUIRE(g.units + g.run < (int64_t)1 << 31, PARE_ERR_UNSUPPORTED);
@@ -1201,16 +1201,15 @@ int pare_w8a8_forward(const void* x, int x_dtype, int64_t ldx, const int8_t* wei
   p.N = N;
   p.ku = (K + kUnitK - 1) / kUnitK;
 
-  if (f.splits) {
-    p.stages = f.stages;
-    const FewParams fp{p, x, ldx, input_scale, K, f.tiles, f.splits};
-    const size_t smem = 1024 + (size_t)f.stages * kWBytes + (size_t)f.units * kFewUnitBytes;
-    return x_dtype == PARE_F16 ? launch(w8a8_few_kernel<__half>, f.blocks, kFewThreads, smem, f.splits, tw, fp)
-                               : launch(w8a8_few_kernel<__nv_bfloat16>, f.blocks, kFewThreads, smem, f.splits, tw, fp);
-  }
+  const bool half = x_dtype == PARE_F16;
+  const FewParams fp{p, x, ldx, input_scale, K, f.tiles, f.splits, f.stages};
+  const size_t few_smem = 1024 + (size_t)f.stages * kWBytes + (size_t)f.units * kFewUnitBytes;
+  if (f.splits && !f.coded)
+    return half ? launch(w8a8_few_kernel<__half, false>, f.blocks, kFewThreads, few_smem, f.splits, tw, tw, fp)
+                : launch(w8a8_few_kernel<__nv_bfloat16, false>, f.blocks, kFewThreads, few_smem, f.splits, tw, tw, fp);
 
   unsigned char* ws = reinterpret_cast<unsigned char*>(workspace);
-  PARE_REQUIRE(map(&tx, ws + sp.codes, M, sp.ldc, g.splits ? g.mt / 2 : g.mt), PARE_ERR_CUDA);
+  PARE_REQUIRE(map(&tx, ws + sp.codes, M, sp.ldc, f.splits ? kFewRows : g.splits ? g.mt / 2 : g.mt), PARE_ERR_CUDA);
 
   const QuantParams q{x, ldx, input_scale, reinterpret_cast<int8_t*>(ws + sp.codes), sp.ldc, reinterpret_cast<float*>(ws + sp.step),
                       reinterpret_cast<int*>(ws + sp.sums), reinterpret_cast<int*>(ws + sp.counters), g.blocks + 1, K};
@@ -1234,6 +1233,12 @@ int pare_w8a8_forward(const void* x, int x_dtype, int64_t ldx, const int8_t* wei
 
   p.step = q.step;
   p.sums = q.sums;
+  if (f.splits) {
+    FewParams cp = fp;
+    cp.w = p;
+    return half ? launch(w8a8_few_kernel<__half, true>, f.blocks, kFewThreads, few_smem, f.splits, tw, tx, cp)
+                : launch(w8a8_few_kernel<__nv_bfloat16, true>, f.blocks, kFewThreads, few_smem, f.splits, tw, tx, cp);
+  }
   p.mt = g.mt;
   p.mtiles = g.mtiles;
   p.total_units = (int)g.units;
@@ -1242,7 +1247,6 @@ int pare_w8a8_forward(const void* x, int x_dtype, int64_t ldx, const int8_t* wei
   p.partial = reinterpret_cast<int*>(ws + sp.partial);
   p.counters = q.zeroed;
   const size_t smem = 1024 + (size_t)g.stages * (kWBytes + (g.splits ? g.mt / 2 : g.mt) * kUnitK) + 512;
-  const bool half = x_dtype == PARE_F16;
   if (g.splits == 0)
     return half ? launch(w8a8_gemm_kernel<__half>, g.blocks, kThreads, smem, 1, tw, tx, p)
                 : launch(w8a8_gemm_kernel<__nv_bfloat16>, g.blocks, kThreads, smem, 1, tw, tx, p);
