@@ -9,10 +9,9 @@
 // its ring with weights, which the first does not write (and what came before the first has ended); it waits before it touches
 // anything else.  A few rows take one launch (w8a8_few_kernel below).
 //
-// The product: as in w4a16_gemm.cu the 128 rows of a weight tile sit on the MMA's M axis (the TMEM lanes), activation rows on its N
-// axis, one persistent thread block per SM, each with one contiguous run of (weight tile, activation tile, 128-column unit); tiles
-// that span runs are added up by whoever arrives last.  Both operands come by TMA (128-byte rows, 128B swizzle) and are multiplied
-// where they land; the accumulator is double-buffered in tensor memory so a tile's epilogue overlaps the next tile's products.
+// The product: as in w4a16_gemm.cu the rows of a weight tile sit on the MMA's M axis (the TMEM lanes), activation rows on its N axis.
+// Both operands come by TMA (128-byte rows, 128B swizzle) and are multiplied where they land; the accumulator is double-buffered in
+// tensor memory so a tile's epilogue overlaps the next tile's products.
 //   warp 0     TMA of both operands      warp 1  tcgen05.mma      warp 2  tensor memory      warps 4-7  epilogue
 // All waits are bounded; when one runs out the thread block stops waiting and loading, lets its copies and products in flight
 // end, and its outputs become NaN.
@@ -45,8 +44,7 @@ struct QuantParams {
   int64_t ldc;
   float* step;
   int* sums;
-  int* zeroed;      // words the product's thread blocks count in
-  int n_zeroed, K;
+  int K;
 };
 
 template <typename T>
@@ -69,7 +67,6 @@ __global__ void __launch_bounds__(THREADS) w8a8_quantize_kernel(const QuantParam
   const int m = blockIdx.x, tid = threadIdx.x;
   const T* row = reinterpret_cast<const T*>(p.x) + m * p.ldx;
   int8_t* out = p.codes + m * p.ldc;
-  for (int i = m * THREADS + tid; i < p.n_zeroed; i += gridDim.x * THREADS) p.zeroed[i] = 0;
   uint32_t top = 0;
   uint4 x[VECS > 0 ? VECS : 1];
   if constexpr (VECS > 0) {
@@ -144,12 +141,10 @@ struct W8Params {
   void* y;
   int64_t ldy;
   int M, N;
-  int mt;                // activation rows per tile (UMMA N), a multiple of 16
+  int mt;                // activation rows per tile (UMMA N), a multiple of 32
   int mtiles;
   int ku;                // units per tile
-  int total_units, run_units, stages;
-  int* partial;          // [thread block][2][mt / 4][128][4]: a run's first tile (begun by another) and its last (not finished)
-  int* counters;         // [thread block]: arrivals at the tile that it begins and others continue; behind them a word for failures
+  int stages;
 };
 
 // bar_wait for arrivals from another thread block of the cluster
@@ -239,219 +234,14 @@ __device__ __forceinline__ void load16(uint32_t taddr, int (&a)[16]) {
   for (int i = 0; i < 16; ++i) a[i] = (int)v[i];
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 1) w8a8_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
-                                                                const W8Params p) {
-  extern __shared__ unsigned char smem_raw[];
-  __shared__ int s_failed, s_flag;
-  __shared__ float s_step[256];
-  __shared__ int s_sums[256];
-  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int stages = p.stages, ku = p.ku;
-  const uint32_t x_bytes = (uint32_t)p.mt * kUnitK, w_ring = s_u32(smem), x_ring = w_ring + stages * kWBytes;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + stages * (kWBytes + x_bytes));
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kMaxStages + 5);
-  const uint32_t full = s_u32(bars), empty = full + kMaxStages * 8, acc_full = empty + kMaxStages * 8, acc_empty = acc_full + 16,
-                 mma_done = acc_empty + 16;
-  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int u0 = blockIdx.x * p.run_units, u1 = min(u0 + p.run_units, p.total_units);
-  bool dead = false;
-  int* status = &s_failed;
-
-  if (threadIdx.x == 0) {
-    s_failed = 0;
-    for (int i = 0; i < kMaxStages; ++i) {
-      bar_init(full + i * 8, 1);
-      bar_init(empty + i * 8, 1);
-    }
-    bar_init(mma_done, 1);
-    for (int i = 0; i < 2; ++i) {
-      bar_init(acc_full + i * 8, 1);
-      bar_init(acc_empty + i * 8, 4);
-    }
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  if (warp == 2) {  // one thread block per SM (its shared memory sees to that): it takes all of tensor memory
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_u32(tmem_slot)), "r"(kTmemCols) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-
-  if (warp == 0) {
-    // ================= operands =================
-    if (lane == 0) {
-      const int n = u1 - u0;
-      auto load_w = [&](int i, int s) {
-        const int t = (u0 + i) / ku, k = u0 + i - t * ku;
-        bar_expect(full + s * 8, kWBytes + x_bytes);
-        tma_tile(w_ring + s * kWBytes, &tm_w, k * kUnitK, t / p.mtiles * kRows, full + s * 8);
-      };
-      auto load_x = [&](int i, int s) {
-        const int t = (u0 + i) / ku, k = u0 + i - t * ku;
-        tma_tile(x_ring + s * x_bytes, &tm_x, k * kUnitK, t % p.mtiles * p.mt, full + s * 8);
-      };
-      int i = 0;
-      for (; i < min(n, stages); ++i) load_w(i, i);     // weights: nothing that this launch may overlap writes them
-      pdl_wait();
-      for (int j = 0; j < i; ++j) load_x(j, j);
-      int s = 0;
-      uint32_t par = 0;
-      for (; i < n; ++i) {
-        bar_wait(empty + s * 8, par, status, dead);
-        if (dead) break;
-        load_w(i, s);
-        load_x(i, s);
-        if (++s == stages) s = 0, par ^= 1;
-      }
-      bool late = false;
-      for (int j = max(0, i - stages); j < i; ++j) bar_wait(full + (j % stages) * 8, (j / stages) & 1, status, late);
-    }
-    __syncwarp();
-  } else if (warp == 1) {
-    // ================= products =================
-    const uint32_t me = elect_one();
-    const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(p.mt >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
-    const uint64_t w_desc0 = umma_desc(w_ring), x_desc0 = umma_desc(x_ring);
-    int s = 0, seg = 0;
-    uint32_t par = 0;
-    for (int u = u0; u < u1; ++seg) {
-      const int n = min(ku - u % ku, u1 - u), buf = seg & 1;
-      const uint32_t acc = tmem + buf * 256;
-      bar_wait(acc_empty + buf * 8, ((seg >> 1) & 1) ^ 1, status, dead);
-      for (int i = 0; i < n; ++i) {
-        bar_wait(full + s * 8, par, status, dead);
-        __syncwarp();
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint64_t dw = w_desc0 + (uint64_t)(s * (kWBytes >> 4)), dx = x_desc0 + (uint64_t)(s * (x_bytes >> 4));
-#pragma unroll
-        for (int j = 0; j < 4; ++j) umma_i8(acc, dw + 2 * j, dx + 2 * j, idesc, (i | j) != 0, me);
-        umma_commit(empty + s * 8, me);
-        if (++s == stages) s = 0, par ^= 1;
-      }
-      umma_commit(acc_full + buf * 8, me);
-      u += n;
-    }
-    umma_commit(mma_done, me);
-    bool late = false;
-    bar_wait(mma_done, 0, status, late);
-    __syncwarp();
-  } else if (warp >= 4) {
-    // ================= epilogue: tensor memory -> registers -> global =================
-    pdl_wait();
-    const int q4 = warp & 3, te = threadIdx.x - 4 * 32;
-    Epilogue<T> epi(p);
-    auto epi_sync = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
-    int* failures = p.counters + gridDim.x;
-    int seg = 0;
-    for (int u = u0; u < u1; ++seg) {
-      const int t = u / ku, k0 = u - t * ku, len = min(ku - k0, u1 - u);
-      u += len;
-      const int row0 = t / p.mtiles * kRows, m0 = t % p.mtiles * p.mt;
-      const int mrows = min(p.mt, p.M - m0), buf = seg & 1;
-      const uint32_t acc = tmem + buf * 256 + ((uint32_t)(q4 * 32) << 16);
-      epi.column(p, row0 + q4 * 32 + lane);
-      epi_sync();     // the tile before has been written
-      for (int i = te; i < mrows; i += 128) {
-        s_step[i] = p.step[m0 + i];
-        s_sums[i] = p.sums[m0 + i];
-      }
-      epi_sync();
-      auto store16 = [&](const int (&a)[16], int c) { epi.store16(a, m0 + c, m0 + mrows, s_step + c, s_sums + c); };
-      bar_wait(acc_full + buf * 8, (seg >> 1) & 1, status, dead);
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      epi.bad = __any_sync(0xffffffffu, dead || *const_cast<volatile int*>(&s_failed) != 0);
-      if (len == ku) {
-        for (int c = 0; c < mrows; c += 16) {
-          int a[16];
-          load16(acc + c, a);
-          store16(a, c);
-        }
-      } else {
-        // ---- the tile spans the runs of thread blocks first .. last; whoever arrives last adds the parts ----
-        const int first = (int)((int64_t)t * ku / p.run_units), last = (int)(((int64_t)t * ku + ku - 1) / p.run_units), me = blockIdx.x;
-        const size_t slot_ints = (size_t)p.mt * kRows;
-        int* counter = p.counters + first;
-        auto slot_of = [&](int b) {   // [mt / 4][128 n][4 m]: four rows of this thread's column per 16-byte access
-          return reinterpret_cast<int4*>(p.partial + ((size_t)b * 2 + (b == first ? 1 : 0)) * slot_ints) + q4 * 32 + lane;
-        };
-        if (epi.bad && lane == 0) atomicExch(failures, 1);
-        epi_sync();
-        if (te == 0) {
-          int have;
-          asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(have) : "l"(counter) : "memory");
-          s_flag = have == last - first;
-        }
-        epi_sync();
-        const bool in_tmem = s_flag != 0;   // all others are there already: this part need not leave tensor memory
-        bool finish = in_tmem;
-        if (!in_tmem) {
-          int4* dst = slot_of(me);
-          for (int c = 0; c < mrows; c += 16) {
-            int a[16];
-            load16(acc + c, a);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) __stcg(dst + (c / 4 + i) * kRows, make_int4(a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3]));
-          }
-          __threadfence();
-          epi_sync();
-          if (te == 0) s_flag = atomicAdd(counter, 1) == last - first;
-          epi_sync();
-          finish = s_flag != 0;
-        }
-        if (finish) {
-          __threadfence();
-          epi.bad = epi.bad || __ldcg(failures) != 0;
-          for (int c = 0; c < mrows; c += 16) {
-            int a[16];
-            if (in_tmem) {
-              load16(acc + c, a);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) a[i] = 0;
-            }
-#pragma unroll 2
-            for (int b = first; b <= last; ++b) {
-              if (in_tmem && b == me) continue;
-              const int4* src = slot_of(b) + c / 4 * kRows;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int4 v = __ldcg(src + i * kRows);
-                a[4 * i] += v.x;
-                a[4 * i + 1] += v.y;
-                a[4 * i + 2] += v.z;
-                a[4 * i + 3] += v.w;
-              }
-            }
-            store16(a, c);
-          }
-        }
-      }
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) bar_arrive(acc_empty + buf * 8);
-    }
-  }
-
-  // ---- teardown: everyone done with tensor memory, then free it ----
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
-  if (warp == 2) {
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
-  }
-}
-
 // ---- product, two SMs on a tile -------------------------------------------------------------------------------------------------------
-// With one SM per 128 x 256 tile every unit brings 48 KB from L2, and at 87 GB/s and SM (measured: half the MMAs take the same time) that, not the MMAs,
-// sets the pace.  cta_group::2 pairs two SMs on 256 weight rows x mt activation rows: each loads its own 128 weight rows and half of
-// the activation rows, the MMA reads both halves, 32 KB per unit.  The even thread block of a pair issues the MMAs; its `full`
-// barrier counts the bytes of both; commits arrive in both.
+// cta_group::2: two SMs on a tile of 256 weight rows x mt activation rows.  Each loads its own 128 weight rows and half of the
+// activation rows, the MMA reads both halves: 32 KB per SM and unit at mt = 256, where one SM alone with a 128 x 256 tile needs 48 KB, and
+// that set its pace (half the MMAs took the same time: 87 GB/s and SM from L2; 28672 x 4096, 2048 rows 260 us against 167, 2880 Top/s).  The
+// even thread block of a pair issues the MMAs; its `full` barrier counts the bytes of both; commits arrive in both.
 //
-// A cluster is one pair, walking over tiles, or (few tiles) 2 or 4 pairs that split K of one tile: then each of them adds up a
-// share of the activation rows, which the others send to its shared memory.
+// A cluster is one pair, walking over tiles, or (few tiles, long K) two pairs that split K of one tile: then each of them adds up
+// half of the activation rows, which the other sends to its shared memory.
 struct PairParams {
   W8Params w;
   int tiles, splits;
@@ -1044,44 +834,19 @@ FewPlan few_plan(int M, int N, int K) {
 }
 
 struct W8Plan {
-  int mt, mtiles, ku, run, blocks, stages;
-  int splits;        // 0: one SM per tile (runs of units); 1, 2: pairs of SMs
+  int mt, mtiles, ku, blocks, stages, splits;
   int tiles;         // weight tiles x activation tiles
   int64_t units;
 };
 
-// Heights of the activation tiles (equal, multiples of 16) and runs by an estimate in microseconds.
+// Height of the activation tiles (equal, a multiple of 32) and whether two pairs of SMs split K, by an estimate in microseconds: rounds of
+// all pairs x units x what a unit of that height takes (0.21 at 32 rows, 0.36 at 256), the weights' way from memory as a lower
+// bound, and what a split adds.  Within a few per cent of the best of 8 heights x 2 splits for 23 shapes of 17 - 3000 rows.
 W8Plan w8_plan(int M, int N, int K) {
   W8Plan best{};
   double least = 1e30;
   const int sms = sm_count(), ku = (K + kUnitK - 1) / kUnitK;
-  const double stream_us = (double)N * K / 6.0e6;       // the weights from memory
-  int seen = 0;
-  for (int target : {256, 192, 128, 96, 64, 32, 16}) {
-    W8Plan g{};
-    g.mtiles = (M + target - 1) / target;
-    g.mt = ((M + g.mtiles - 1) / g.mtiles + 15) / 16 * 16;
-    g.mtiles = (M + g.mt - 1) / g.mt;
-    if (g.mt == seen) continue;
-    seen = g.mt;
-    g.ku = ku;
-    g.tiles = (N + kRows - 1) / kRows * g.mtiles;
-    g.units = (int64_t)g.tiles * g.ku;
-    const double unit_us = 0.19 + 0.0013 * g.mt;
-    auto consider = [&](int64_t run) {
-      if (run < 1 || (g.units + run - 1) / run > sms) return;
-      double cost = std::max(run * unit_us, stream_us) + 0.01 * g.mt;
-      if (run % g.ku) cost += 2.5 + 0.02 * g.mt * ((g.ku + run - 1) / run + (g.ku % run != 0));
-      if (cost < least - 1e-9) {
-        least = cost;
-        g.run = (int)run;
-        best = g;
-      }
-    };
-    consider((int64_t)(g.tiles + sms - 1) / sms * g.ku);
-    consider((g.units + sms - 1) / sms);
-    for (int parts = 2; parts <= 16; ++parts) consider((g.ku + parts - 1) / parts);
-  }
+  const double stream_us = (double)N * K / 6.0e6;
   for (int target : {256, 192, 160, 128, 96, 64, 32}) {
     for (int splits : {1, 2}) {
       W8Plan g{};
@@ -1090,43 +855,37 @@ W8Plan w8_plan(int M, int N, int K) {
       g.mtiles = (M + g.mt - 1) / g.mt;
       g.ku = ku;
       g.splits = splits;
-      g.tiles = (N + 2 * kRows - 1) / (2 * kRows) * g.mtiles;
-      g.units = (int64_t)g.tiles * g.ku;
-      if (g.mt > 256 || splits > ku) continue;
+      g.units = (int64_t)((N + 2 * kRows - 1) / (2 * kRows)) * g.mtiles;
+      if (g.mt > 256 || splits > ku || g.units * ku >= (int64_t)1 << 31) continue;
+      g.tiles = (int)g.units;
+      g.units *= ku;
       const int clusters = sms / (2 * splits), rounds = (g.tiles + clusters - 1) / clusters;
       if (splits > 1 && rounds > 1) continue;
-      const double cost = std::max((double)rounds * ((ku + splits - 1) / splits) * (0.2 + 0.00055 * g.mt), stream_us) + 0.01 * g.mt + 1.5 * (splits > 1);
+      const double cost = std::max((double)rounds * ((ku + splits - 1) / splits) * (0.2 + 0.00055 * g.mt), stream_us) + 0.01 * g.mt +
+                          (splits > 1 ? 2.0 + 0.015 * g.mt : 0.0);
       if (cost < least - 1e-9) {
         least = cost;
         best = g;
       }
     }
   }
-  if (best.splits) {
-    const int clusters = sms / (2 * best.splits);
-    best.run = ku;
-    best.blocks = 2 * best.splits * (best.splits > 1 || best.tiles < clusters ? best.tiles : clusters);
-    best.stages = kRingBytes / (kWBytes + best.mt / 2 * kUnitK);
-  } else {
-    best.blocks = (int)((best.units + best.run - 1) / best.run);
-    best.stages = kRingBytes / (kWBytes + best.mt * kUnitK);
-  }
-  if (best.stages > kMaxStages) best.stages = kMaxStages;
+  if (best.splits == 0) return best;
+  const int clusters = sms / (2 * best.splits);
+  best.blocks = 2 * best.splits * (best.splits > 1 || best.tiles < clusters ? best.tiles : clusters);
+  best.stages = std::min(kRingBytes / (kWBytes + best.mt / 2 * kUnitK), kMaxStages);
   return best;
 }
 
 struct W8Space {
-  size_t codes, step, sums, counters, partial, bytes;
+  size_t codes, step, sums, bytes;
   int64_t ldc;
-  W8Space(const W8Plan& g, int M, int K) {
+  W8Space(int M, int K) {
     auto up = [](size_t b) { return (b + 255) / 256 * 256; };
     ldc = (K + 15) / 16 * 16;
     codes = 0;
     step = up((size_t)M * ldc);
     sums = step + up((size_t)M * 4);
-    counters = sums + up((size_t)M * 4);
-    partial = counters + up(((size_t)g.blocks + 1) * 4);
-    bytes = partial + (g.ku && g.run % g.ku ? (size_t)g.blocks * 2 * g.mt * kRows * 4 : 0);
+    bytes = sums + up((size_t)M * 4);
   }
 };
 
@@ -1141,7 +900,7 @@ size_t pare_w8a8_workspace_bytes(int M, int N, int K) {
   if (M <= 0 || N <= 0 || K <= 0 || K > kMaxK) return 0;
   const FewPlan f = few_plan(M, N, K);
   if (f.splits && !f.coded) return 0;
-  return W8Space(f.splits ? W8Plan{} : w8_plan(M, N, K), M, K).bytes;
+  return f.splits || w8_plan(M, N, K).splits ? W8Space(M, K).bytes : 0;
 }
 
 int pare_w8a8_forward(const void* x, int x_dtype, int64_t ldx, const int8_t* weight, int64_t ldw, const float* scale, const float* zero,
@@ -1154,11 +913,11 @@ int pare_w8a8_forward(const void* x, int x_dtype, int64_t ldx, const int8_t* wei
   PARE_REQUIRE(aligned16(weight) && ldw % 16 == 0 && aligned16(workspace), PARE_ERR_ALIGN);
   const FewPlan f = few_plan(M, N, K);
   const W8Plan g = f.splits ? W8Plan{} : w8_plan(M, N, K);
-  const W8Space sp(g, M, K);
+  const W8Space sp(M, K);
   if (f.splits && !f.coded) {
     PARE_REQUIRE(aligned16(x) && (M == 1 || ldx % 8 == 0), PARE_ERR_ALIGN);
   } else {
-    PARE_REQUIRE(g.units + g.run < (int64_t)1 << 31, PARE_ERR_UNSUPPORTED);
+    PARE_REQUIRE(f.splits || g.splits, PARE_ERR_UNSUPPORTED);
     PARE_REQUIRE(workspace && workspace_bytes >= sp.bytes, PARE_ERR_WORKSPACE);
   }
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
@@ -1209,10 +968,10 @@ int pare_w8a8_forward(const void* x, int x_dtype, int64_t ldx, const int8_t* wei
                 : launch(w8a8_few_kernel<__nv_bfloat16, false>, f.blocks, kFewThreads, few_smem, f.splits, tw, tw, fp);
 
   unsigned char* ws = reinterpret_cast<unsigned char*>(workspace);
-  PARE_REQUIRE(map(&tx, ws + sp.codes, M, sp.ldc, f.splits ? kFewRows : g.splits ? g.mt / 2 : g.mt), PARE_ERR_CUDA);
+  PARE_REQUIRE(map(&tx, ws + sp.codes, M, sp.ldc, f.splits ? kFewRows : g.mt / 2), PARE_ERR_CUDA);
 
   const QuantParams q{x, ldx, input_scale, reinterpret_cast<int8_t*>(ws + sp.codes), sp.ldc, reinterpret_cast<float*>(ws + sp.step),
-                      reinterpret_cast<int*>(ws + sp.sums), reinterpret_cast<int*>(ws + sp.counters), g.blocks + 1, K};
+                      reinterpret_cast<int*>(ws + sp.sums), K};
   const bool vec = aligned16(x) && (M == 1 || ldx % 8 == 0) && K % 8 == 0 && (!input_scale || aligned16(input_scale));
   // Many rows: few threads with several vectors in flight each, so that all rows are resident at once; few rows: many threads.
   auto quantize = [&](auto tag) {
@@ -1241,15 +1000,8 @@ int pare_w8a8_forward(const void* x, int x_dtype, int64_t ldx, const int8_t* wei
   }
   p.mt = g.mt;
   p.mtiles = g.mtiles;
-  p.total_units = (int)g.units;
-  p.run_units = g.run;
   p.stages = g.stages;
-  p.partial = reinterpret_cast<int*>(ws + sp.partial);
-  p.counters = q.zeroed;
-  const size_t smem = 1024 + (size_t)g.stages * (kWBytes + (g.splits ? g.mt / 2 : g.mt) * kUnitK) + 512;
-  if (g.splits == 0)
-    return half ? launch(w8a8_gemm_kernel<__half>, g.blocks, kThreads, smem, 1, tw, tx, p)
-                : launch(w8a8_gemm_kernel<__nv_bfloat16>, g.blocks, kThreads, smem, 1, tw, tx, p);
+  const size_t smem = 1024 + (size_t)g.stages * (kWBytes + g.mt / 2 * kUnitK) + 512;
   const PairParams pp{p, g.tiles, g.splits};
   return half ? launch(w8a8_pair_kernel<__half>, g.blocks, kThreads, smem, 2 * g.splits, tw, tx, pp)
               : launch(w8a8_pair_kernel<__nv_bfloat16>, g.blocks, kThreads, smem, 2 * g.splits, tw, tx, pp);
