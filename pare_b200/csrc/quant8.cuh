@@ -27,20 +27,23 @@ struct Grid {
     if (!finite || step == 0.f) return 0;
     return (int)fminf(fmaxf(rintf(__fdiv_rn(x, step)), -127.f), 127.f);
   }
-  // Eight of them.  x * inv + 1.5 * 2^23 has the code in its low byte, rounded half to even; it is what the quotient rounds to
-  // except next to a border between two codes (x * inv is off by less than 1e-5), where the quotient itself is taken.
+  // Eight of them.  x * inv + 1.5 * 2^23 has the code in its low byte, rounded half to even; x * inv is off by less than 2^-22 of itself, so
+  // where slightly smaller and slightly larger reciprocals give the same, that is what the quotient rounds to.  Where they do not
+  // (next to a border between two codes) the quotient itself is taken.
   template <typename T>
   __device__ __forceinline__ uint2 codes(const uint4& w) const {
     constexpr float kMagic = 12582912.f;
     const T* v = reinterpret_cast<const T*>(&w);
-    float r[8], off = 0.f;
+    const float less = inv * (1.f - 0x1p-21f), more = inv * (1.f + 0x1p-21f);
+    float r[8];
+    uint32_t differ = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float x = to_float<T>(v[j]);
-      r[j] = fmaf(x, inv, kMagic);
-      off = fmaxf(off, fabsf(fmaf(x, inv, kMagic - r[j])));
+      r[j] = fmaf(x, more, kMagic);
+      differ |= __float_as_uint(r[j]) ^ __float_as_uint(fmaf(x, less, kMagic));
     }
-    if (off > 0.4999f || tiny || !finite) {
+    if (differ || tiny || !finite) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) r[j] = (float)code(to_float<T>(v[j])) + kMagic;
     }

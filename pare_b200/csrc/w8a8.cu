@@ -43,7 +43,7 @@ struct QuantParams {
   int8_t* codes;
   int64_t ldc;
   float* step;
-  int* sums;
+  int* sums;        // NULL: nobody asks for them
   int K;
 };
 
@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(THREADS) w8a8_quantize_kernel(const QuantParam
       const int k = (i * THREADS + tid) * 8;
       if (k >= p.K) break;
       const uint2 o = grid.codes<T>(x[i]);
-      sum = __dp4a((int)o.y, 0x01010101, __dp4a((int)o.x, 0x01010101, sum));
+      if (p.sums) sum = __dp4a((int)o.y, 0x01010101, __dp4a((int)o.x, 0x01010101, sum));
       *reinterpret_cast<uint2*>(out + k) = o;
     }
   } else {
@@ -119,6 +119,8 @@ __global__ void __launch_bounds__(THREADS) w8a8_quantize_kernel(const QuantParam
       out[k] = (int8_t)c;
     }
   }
+  if (tid == 0) p.step[m] = grid.finite ? grid.step : __int_as_float(0x7fffffff);
+  if (!p.sums) return;
   sum = __reduce_add_sync(0xffffffffu, sum);
   if ((tid & 31) == 0) s_sum[tid >> 5] = sum;
   __syncthreads();
@@ -126,7 +128,6 @@ __global__ void __launch_bounds__(THREADS) w8a8_quantize_kernel(const QuantParam
     int all = 0;
 #pragma unroll
     for (int w = 0; w < kW; ++w) all += s_sum[w];
-    p.step[m] = grid.finite ? grid.step : __int_as_float(0x7fffffff);
     p.sums[m] = all;
   }
 }
@@ -415,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, 1) w8a8_pair_kernel(const __grid_con
       asm volatile("bar.sync 1, 128;" ::: "memory");
       for (int i = te; i < mrows; i += 128) {
         s_step[i] = p.step[m0 + i];
-        s_sums[i] = p.sums[m0 + i];
+        s_sums[i] = p.zero ? p.sums[m0 + i] : 0;
       }
       asm volatile("bar.sync 1, 128;" ::: "memory");
       bar_wait(acc_full + buf * 8, (seg >> 1) & 1, status, dead);
@@ -474,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1) w8a8_pair_kernel(const __grid_con
       epi.bad = *const_cast<volatile int*>(&s_failed) != 0;
       for (int i = te; i < to - from; i += 128) {
         s_step[i] = p.step[m0 + from + i];
-        s_sums[i] = p.sums[m0 + from + i];
+        s_sums[i] = p.zero ? p.sums[m0 + from + i] : 0;
       }
       asm volatile("bar.sync 1, 128;" ::: "memory");
       for (int c = 0; c < to - from; c += 16) {
@@ -971,7 +972,7 @@ int pare_w8a8_forward(const void* x, int x_dtype, int64_t ldx, const int8_t* wei
   PARE_REQUIRE(map(&tx, ws + sp.codes, M, sp.ldc, f.splits ? kFewRows : g.mt / 2), PARE_ERR_CUDA);
 
   const QuantParams q{x, ldx, input_scale, reinterpret_cast<int8_t*>(ws + sp.codes), sp.ldc, reinterpret_cast<float*>(ws + sp.step),
-                      reinterpret_cast<int*>(ws + sp.sums), K};
+                      zero ? reinterpret_cast<int*>(ws + sp.sums) : nullptr, K};
   const bool vec = aligned16(x) && (M == 1 || ldx % 8 == 0) && K % 8 == 0 && (!input_scale || aligned16(input_scale));
   // Many rows: few threads with several vectors in flight each, so that all rows are resident at once; few rows: many threads.
   auto quantize = [&](auto tag) {
