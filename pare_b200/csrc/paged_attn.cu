@@ -32,6 +32,7 @@ constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kBias = 4.f, kSlack = 11.f;
+constexpr float kLowest = -1e30f;          // a reference below every score, and finite
 constexpr int kMinRun = 3;                 // units of a warp's run at least
 
 template <int D>
@@ -105,6 +106,12 @@ __device__ __forceinline__ uint32_t pack_bf2(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+// A product that begins a sum (mma16816 adds to one)
+__device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 // Largest over the eight lanes that hold the same heads (lane = 4 g + t: over g)
 __device__ __forceinline__ float max_over_g(float v) {
 #pragma unroll
@@ -139,7 +146,7 @@ struct Tile {
   __device__ __forceinline__ void reset() {
 #pragma unroll
     for (int i = 0; i < 2 * kW; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    m0 = m1 = -INFINITY;
+    m0 = m1 = kLowest;
     l0 = l1 = 0.f;
   }
 
@@ -192,11 +199,22 @@ struct Tile {
     f1 = __shfl_sync(0xffffffffu, back, 8 * t + 4) * scale_log2;
   }
 
-  // Scores (already in base 2; hidden ones -inf) of tokens g, g + 8 x heads 2 t, 2 t + 1 -> probabilities in place
-  __device__ __forceinline__ void softmax(float (&s)[4]) {
-    const bool passed = s[0] > m0 + kSlack || s[2] > m0 + kSlack || s[1] > m1 + kSlack || s[3] > m1 + kSlack;
-    if (__any_sync(0xffffffffu, passed)) {
-      const float n0 = fmaxf(m0, max_over_g(fmaxf(s[0], s[2]))), n1 = fmaxf(m1, max_over_g(fmaxf(s[1], s[3])));
+  // Sums of products of tokens g, g + 8 x heads 2 t, 2 t + 1, their factors to scores in base 2, and how many of the tokens are visible
+  // -> probabilities in place
+  __device__ __forceinline__ void softmax(float (&s)[4], float s0, float s1, int seen, int g) {
+    float x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = fmaf(s[i], (i & 1) ? s1 : s0, (i & 1) ? kBias - m1 : kBias - m0);
+    if (seen < kUnit) {
+      if (g >= seen) x[0] = x[1] = -INFINITY;
+      if (g + 8 >= seen) x[2] = x[3] = -INFINITY;
+    }
+    if (__any_sync(0xffffffffu, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) > kBias + kSlack)) {
+      // the reference moves up to the largest score
+      float t[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t[i] = x[i] == -INFINITY ? -INFINITY : s[i] * ((i & 1) ? s1 : s0);
+      const float n0 = fmaxf(m0, max_over_g(fmaxf(t[0], t[2]))), n1 = fmaxf(m1, max_over_g(fmaxf(t[1], t[3])));
       const float a0 = n0 == m0 ? 1.f : ex2(m0 - n0), a1 = n1 == m1 ? 1.f : ex2(m1 - n1);
       m0 = n0;
       m1 = n1;
@@ -209,12 +227,12 @@ struct Tile {
         o[i][2] *= a0;
         o[i][3] *= a1;
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (x[i] != -INFINITY) x[i] = fmaf(s[i], (i & 1) ? s1 : s0, (i & 1) ? kBias - m1 : kBias - m0);
     }
-    const float b0 = m0 == -INFINITY ? 0.f : m0 - kBias, b1 = m1 == -INFINITY ? 0.f : m1 - kBias;
-    s[0] = ex2(s[0] - b0);
-    s[1] = ex2(s[1] - b1);
-    s[2] = ex2(s[2] - b0);
-    s[3] = ex2(s[3] - b1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = ex2(x[i]);
     l0 += s[0] + s[2];
     l1 += s[1] + s[3];
   }
@@ -225,30 +243,21 @@ struct Tile {
     float acc[kJ][4];
 #pragma unroll
     for (int j = 0; j < kJ; ++j) {
-      acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
       const int chunk = D == 128 ? (t + 4 * j) ^ ((g & 1) << 2) : t;
       const uint4 lo = lds128(stage + g * D + chunk * 16), hi = lds128(stage + (g + 8) * D + chunk * 16);
       const uint32_t a[4] = {lo.x, lo.y, lo.z, lo.w}, b[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const uint32_t ua = a[w] ^ 0x80808080u, ub = b[w] ^ 0x80808080u;
-        mma16816<__half>(acc[j], codes_to_half2<0x4140>(ua), codes_to_half2<0x4140>(ub), codes_to_half2<0x4342>(ua),
-                         codes_to_half2<0x4342>(ub), qh[j][w][0], qh[j][w][1]);
+        const uint32_t c0 = codes_to_half2<0x4140>(ua), c1 = codes_to_half2<0x4140>(ub), c2 = codes_to_half2<0x4342>(ua), c3 = codes_to_half2<0x4342>(ub);
+        if (w == 0) mma16816_first(acc[j], c0, c1, c2, c3, qh[j][w][0], qh[j][w][1]);
+        else mma16816<__half>(acc[j], c0, c1, c2, c3, qh[j][w][0], qh[j][w][1]);
       }
     }
-    const float s0 = ks * f0, s1 = ks * f1;
     float s[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float x = acc[0][i];
-      if (kJ == 2) x += acc[kJ - 1][i];
-      s[i] = x * ((i & 1) ? s1 : s0);
-    }
-    if (seen < kUnit) {
-      if (g >= seen) s[0] = s[1] = -INFINITY;
-      if (g + 8 >= seen) s[2] = s[3] = -INFINITY;
-    }
-    softmax(s);
+    for (int i = 0; i < 4; ++i) s[i] = kJ == 2 ? acc[0][i] + acc[kJ - 1][i] : acc[0][i];
+    softmax(s, ks * f0, ks * f1, seen, g);
     const uint32_t h0 = pack_half2(s[0], s[1]), h1 = pack_half2(s[2], s[3]), p0 = transpose8x8(h0), p1 = transpose8x8(h1);
     uint32_t r0 = 0, r1 = 0;       // what the rounding left
     if constexpr (kTwoTerms) {
@@ -276,9 +285,9 @@ struct Tile {
       const uint32_t cd0 = __byte_perm(v[2][w], v[3][w], 0x5140) ^ 0x80808080u, cd1 = __byte_perm(v[2][w], v[3][w], 0x7362) ^ 0x80808080u;
       const uint32_t a[4] = {codes_to_half2<0x4140>(ab0), codes_to_half2<0x4342>(ab0), codes_to_half2<0x4140>(cd0), codes_to_half2<0x4342>(cd0)};
       const uint32_t b[4] = {codes_to_half2<0x4140>(ab1), codes_to_half2<0x4342>(ab1), codes_to_half2<0x4140>(cd1), codes_to_half2<0x4342>(cd1)};
-      float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-      mma16816<__half>(x, a[0], a[1], a[2], a[3], p0, p1);
-      mma16816<__half>(y, b[0], b[1], b[2], b[3], p0, p1);
+      float x[4], y[4];
+      mma16816_first(x, a[0], a[1], a[2], a[3], p0, p1);
+      mma16816_first(y, b[0], b[1], b[2], b[3], p0, p1);
       if constexpr (kTwoTerms) {
         mma16816<__half>(x, a[0], a[1], a[2], a[3], r0, r1);
         mma16816<__half>(y, b[0], b[1], b[2], b[3], r0, r1);
@@ -314,12 +323,8 @@ struct Tile {
 #pragma unroll
       for (int w = 0; w < 4; ++w) mma16816<T>(acc, wa[2 * w], wb[2 * w], wa[2 * w + 1], wb[2 * w + 1], wq[2 * w], wq[2 * w + 1]);
     }
-    float s[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = acc[i] * scale_log2;
-    if (g >= seen) s[0] = s[1] = -INFINITY;
-    if (g + 8 >= seen) s[2] = s[3] = -INFINITY;
-    softmax(s);
+    float s[4] = {acc[0], acc[1], acc[2], acc[3]};
+    softmax(s, scale_log2, scale_log2, seen, g);
     uint32_t p0, p1, r0, r1;
     if constexpr (std::is_same<T, __half>::value) {
       const uint32_t a = pack_half2(s[0], s[1]), b = pack_half2(s[2], s[3]);
