@@ -51,6 +51,8 @@ _FP8 = (QuantDtype.FP8_E4M3, QuantDtype.FP8_E5M2)
 
 
 class QuantizedLinear(nn.Module):
+    int8_kernel = False
+
     def __init__(
         self,
         q_weight: Tensor,
@@ -91,7 +93,6 @@ class QuantizedLinear(nn.Module):
         self.quantize_inputs = quantize_inputs
         self.use_kernel = use_kernel
         self.kernel_meta_fp16 = False
-        self.int8_kernel = False
 
     def _register_optional(self, g_idx: Tensor | None, input_scale: Tensor | None) -> None:
         self.register_buffer("g_idx", None if g_idx is None else g_idx.to(torch.int32))
@@ -210,10 +211,24 @@ class QuantizedLinear(nn.Module):
             raise ValueError("int8_kernel needs an INT8 layer with quantize_inputs and without g_idx")
         if scale.numel() not in (1, n) or zero.numel() not in (1, n):
             raise ValueError("int8_kernel needs one scale per output channel or per tensor (granularity per_channel or per_tensor)")
-        zero = zero.reshape(-1).expand(n).contiguous()
-        self.register_buffer("_q_weight_int8", aligned_rows(self.q_weight), persistent=False)
-        self.register_buffer("_scale_int8", scale.reshape(-1).expand(n).contiguous(), persistent=False)
+        zero = zero.float().reshape(-1).expand(n).contiguous()
+        self.register_buffer("_scale_int8", scale.float().reshape(-1).expand(n).contiguous(), persistent=False)
         self.register_buffer("_zero_int8", zero if bool(zero.any()) else None, persistent=False)
+        self.register_buffer("_q_weight_int8", aligned_rows(self.q_weight), persistent=False)
+
+    def _drop_int8_buffers(self) -> None:
+        for name in ("_q_weight_int8", "_scale_int8", "_zero_int8"):
+            if name in self._buffers:
+                delattr(self, name)
+
+    # Both may change what the derived tensors were made from (moving them would also lose their rows' alignment).
+    def _load_from_state_dict(self, *args, **kwargs) -> None:
+        self._drop_int8_buffers()
+        super()._load_from_state_dict(*args, **kwargs)
+
+    def _apply(self, *args, **kwargs):
+        self._drop_int8_buffers()
+        return super()._apply(*args, **kwargs)
 
     def supports_prepared(self, rows: int) -> bool:
         """True if :meth:`forward_prepared` can serve ``rows`` activation rows of this layer."""

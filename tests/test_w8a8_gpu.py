@@ -1,5 +1,7 @@
 """W8A8 linear on the GPU against the definition: codes in the float32 arithmetic it names, sums in 64-bit integers, the rest in float64."""
 
+import copy
+
 import pytest
 import torch
 import torch.nn as nn
@@ -161,6 +163,29 @@ def test_layer_takes_the_integer_path_when_asked(cuda_lib):
         layer.input_scale = torch.rand(500, device=DEV) + 0.5
         _check(layer(x).reshape(14, n), x.reshape(14, 500), layer.q_weight, layer.scale.reshape(-1).expand(n), layer.zero.reshape(-1).expand(n),
                layer.bias, layer.input_scale)
+
+
+@pytest.mark.parametrize("granularity", ["per_channel", "per_tensor"])
+def test_layer_follows_loaded_states_and_moves(granularity, cuda_lib):
+    def layer(seed, sym):
+        torch.manual_seed(seed)
+        cfg = QuantConfig(bits=8, scheme="smoothquant", granularity=granularity, sym=sym)
+        one = QuantizedLinear.from_linear(nn.Linear(500, 300), cfg).cuda()
+        one.quantize_inputs, one.use_kernel, one.int8_kernel = True, True, True
+        return one
+
+    x = torch.randn(5, 500, device=DEV, dtype=torch.float16)
+    first, other = layer(0, True), layer(1, False)
+    first(x)
+    first.load_state_dict(other.state_dict())                               # a zero-point where there was none
+    want = other(x)
+    assert torch.equal(first(x), want)
+    moved = first.cpu().cuda()
+    assert torch.equal(moved(x), want) and moved._buffers["_q_weight_int8"].stride(0) == 512
+    assert torch.equal(copy.deepcopy(first)(x), want)
+    half = other.half()                                                     # rounds its scales, which the product then has in float32
+    n = half.out_features
+    _check(half(x), x, half.q_weight, half.scale.float().reshape(-1).expand(n), half.zero.float().reshape(-1).expand(n), half.bias)
 
 
 def test_layer_refuses_what_the_integers_cannot_do(cuda_lib):
