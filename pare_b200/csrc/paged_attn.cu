@@ -32,7 +32,7 @@ constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kBias = 4.f, kSlack = 11.f;
-constexpr float kLowest = -1e30f;          // a reference below every score, and finite
+constexpr float kLowest = -3e38f;          // a reference below every score, and finite
 constexpr int kMinRun = 3;                 // units of a warp's run at least
 
 template <int D>
@@ -629,6 +629,8 @@ int pare_paged_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h, const
   PARE_REQUIRE(workspace && workspace_bytes >= workspace_of(D, blocks), PARE_ERR_WORKSPACE);
   const int group = Hq / H, sub = (group + kHeads - 1) / kHeads;
   PARE_REQUIRE((int64_t)T * H * sub < (int64_t)1 << 31, PARE_ERR_UNSUPPORTED);
+  // the step counts its units in 32 bits
+  PARE_REQUIRE(T * ((int64_t)tb->max_blocks * l->block_size / kUnit + 2) < (int64_t)1 << 31, PARE_ERR_UNSUPPORTED);
   const StepLayout s(tb->R, T, l->block_size);
   const int* w = reinterpret_cast<const int*>(tb->step);
   const PagedAttnParams p{q, q_stride_t, q_stride_h, out, out_stride_t, out_stride_h, reinterpret_cast<const int4*>(w + s.info),

@@ -7,6 +7,7 @@
 // Until then its tokens stay in the input type in the request's open rows (tail_k / tail_v), so every code is the result of one
 // rounding and tokens fed in pieces give what the same tokens fed at once give (the property of the reference's residual window,
 // pare/kv_cache.py:231-244).
+#include <climits>
 #include <type_traits>
 
 #include "paged.cuh"
@@ -218,9 +219,11 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
 }
 
 // Blocks of the requests marked in `release` go back to the stack, in request order, oldest block first; their lengths become 0.
+// One thread block: blocks before a request by a prefix sum, then the blocks of all requests are spread over the threads.
 __global__ void __launch_bounds__(kPlanThreads) paged_release_kernel(const int* release, int* seq_lens, const int* table, int64_t ld_table,
                                                                      int* free_blocks, int free_capacity, int* free_count, int R, int bs_log2,
                                                                      int max_blocks) {
+  extern __shared__ int s_start[];      // [R] blocks given back by the requests before
   __shared__ long long s_sums[1][kPlanWarps];
   const int per = (R + kPlanThreads - 1) / kPlanThreads, r0 = min(R, (int)threadIdx.x * per), r1 = min(R, r0 + per);
   auto blocks_of = [&](int r) {
@@ -231,15 +234,20 @@ __global__ void __launch_bounds__(kPlanThreads) paged_release_kernel(const int* 
   for (int r = r0; r < r1; ++r) n[0] += blocks_of(r);
   const int count = max(0, *free_count);
   block_scan<1>(n, before, all, s_sums);
-  long long at = count + before[0];
+  const int room = max(0, free_capacity - count), given = (int)min((long long)room, all[0]);      // a pool has no more blocks than its stack
+  long long at = before[0];
   for (int r = r0; r < r1; ++r) {
-    const int nb = blocks_of(r);
-    for (int b = 0; b < nb; ++b, ++at)
-      if (at < free_capacity) free_blocks[at] = table[r * ld_table + b];
-    if (release[r] != 0) seq_lens[r] = 0;
+    s_start[r] = (int)min(at, (long long)INT_MAX);
+    at += blocks_of(r);
   }
   __syncthreads();
-  if (threadIdx.x == 0) *free_count = (int)min((long long)free_capacity, count + all[0]);
+  for (int r = r0; r < r1; ++r)
+    if (release[r] != 0) seq_lens[r] = 0;
+  for (int i = threadIdx.x; i < given; i += kPlanThreads) {
+    const int r = last_at_most(s_start, R, i);
+    free_blocks[count + i] = table[r * ld_table + i - s_start[r]];
+  }
+  if (threadIdx.x == 0) *free_count = count + given;
 }
 
 // ---- append -----------------------------------------------------------------------------------------------------------------------
@@ -477,7 +485,7 @@ int pare_paged_release(const int32_t* release, int32_t* seq_lens, int R, const i
   PARE_REQUIRE(release && seq_lens && block_table && free_blocks && free_count, PARE_ERR_SHAPE);
   PARE_REQUIRE(R > 0 && R <= kMaxRequests && max_blocks > 0 && ld_table >= max_blocks && free_capacity >= 0, PARE_ERR_SHAPE);
   PARE_REQUIRE(block_size_ok(block_size), PARE_ERR_UNSUPPORTED);
-  paged_release_kernel<<<1, kPlanThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+  paged_release_kernel<<<1, kPlanThreads, R * sizeof(int), reinterpret_cast<cudaStream_t>(stream)>>>(
       release, seq_lens, block_table, ld_table, free_blocks, free_capacity, free_count, R, log2_of(block_size), max_blocks);
   return launch_status();
 }

@@ -113,6 +113,8 @@ def test_c_entries_refuse():
     assert attend(q=None) == attend(Hq=7) == attend(Hq=0) == SHAPE and attend(t=ctypes.addressof(many)) == UNSUPPORTED
     assert attend(size=16) == attend(ws=None) == SPACE and attend(q=p + 4) == attend(sh=130) == attend(ws=p + 8) == ALIGN
     assert attend(t=ctypes.addressof(none)) == OK
+    wide = tables(T=256, ld=1 << 23, width=1 << 23)          # more units than 32 bits count
+    assert attend(t=ctypes.addressof(wide)) == UNSUPPORTED
     assert L.pare_paged_attn_workspace_bytes(96) == 0
 
     def linear(M=2, N=4, K=32, ldw=32, ldx=32, ldy=4, dtype=0, x=p, w=p, ws=p, size=need):
