@@ -5,7 +5,7 @@ sequences all have the same length.  A server's requests start and end at their 
 tokens is shared by up to ``max_requests`` of them through a block table.  A block holds int8 codes with one scale per head for its
 keys and one for its values; it is quantized once, when its last token arrives.  Until then the tokens stay in the input type
 (``tail_k`` / ``tail_v``), so what is stored does not depend on how the tokens were cut into calls, as with the reference's
-residual window.
+residual window.  An infinity or NaN in a block makes that head's whole block NaN once it is quantized.
 
 Three functions work on plain tensors, and :class:`PagedKVCache` keeps those tensors for all layers of a model:
 
@@ -23,6 +23,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import threading
 from dataclasses import dataclass
 from typing import NamedTuple, Sequence
 
@@ -76,6 +77,17 @@ class PagedLayer(_LayerTensors):
         self._c = ctypes.addressof(self._struct)
         return self
 
+    # Copies and other tensors in a layer's place are layers of their own, with their own addresses.
+    @classmethod
+    def _make(cls, tensors) -> "PagedLayer":
+        return cls(*tensors)
+
+    def __reduce__(self):
+        return PagedLayer, tuple(self)
+
+
+_first_use = threading.Lock()
+
 
 @functools.lru_cache(maxsize=4096)
 def _step_layout(requests: int, tokens: int, block_size: int) -> tuple[int, tuple[int, ...]]:
@@ -101,9 +113,11 @@ class PagedStep:
     def _tables(self) -> int:
         """Address of the step as the C entries take it."""
         if not self._c:
-            self._struct = _lib.PagedTablesStruct(self.words.data_ptr(), self.block_table.data_ptr(), self._ld, self.block_table.shape[1],
-                                                  self.requests, self.tokens, self.block_size)
-            self._c = ctypes.addressof(self._struct)
+            with _first_use:       # threads may share a step
+                if not self._c:
+                    self._struct = _lib.PagedTablesStruct(self.words.data_ptr(), self.block_table.data_ptr(), self._ld, self.block_table.shape[1],
+                                                          self.requests, self.tokens, self.block_size)
+                    self._c = ctypes.addressof(self._struct)
         return self._c
 
     @property
@@ -241,7 +255,8 @@ def _attn_workspace(d: int, index: int) -> int:
 def attend_blocks(layer: PagedLayer, step: PagedStep, q: Tensor, scale: float | None = None, out: Tensor | None = None) -> Tensor:
     """``softmax(q K^T * scale) V`` of the step's queries ``q [tokens, Hq, D]`` over their request's tokens up to and with their own
     (the step's keys and values have been appended).  ``Hq`` is a multiple of the KV heads; default scale ``1 / sqrt(D)``.  At most
-    4096 rows: longer prompts go through :meth:`PagedKVCache.prefill`.  Rows that belong to nobody are left as they were in
+    4096 rows: longer prompts go through :meth:`PagedKVCache.prefill` (and rows times tokens of a full row of the block table stay
+    below 2^35).  Rows that belong to nobody are left as they were in
     ``out`` (``[tokens, Hq, D]``, channels adjacent, not overlapping ``q``; a new tensor if not given)."""
     _fits(layer, step)
     tokens, d, dev = step.tokens, layer.head_dim, layer.device
@@ -308,6 +323,7 @@ class PagedKVCache:
         self._state = torch.zeros(c.max_requests + 1, dtype=torch.int32, device=device)    # lengths, then the number of free blocks
         self.seq_lens, self.free_count = self._state[:-1], self._state[-1:]
         self.free_blocks = torch.empty(c.num_blocks, dtype=torch.int32, device=device)
+        self._captured = False      # a graph changes the lengths: the host cannot follow them any more
         self.reset()
 
     def reset(self) -> None:
@@ -316,7 +332,7 @@ class PagedKVCache:
         self.free_blocks.copy_(torch.arange(c.num_blocks - 1, -1, -1, dtype=torch.int32))
         self._state.zero_()
         self._state[-1] = c.num_blocks
-        self._lens: list[int] | None = [0] * c.max_requests       # None once lengths are known to the GPU alone
+        self._lens: list[int] | None = None if self._captured else [0] * c.max_requests       # None: lengths are known to the GPU alone
 
     # ------------------------------------------------------------------ lengths
     def _blocks(self, n: int) -> int:
@@ -338,6 +354,7 @@ class PagedKVCache:
         if isinstance(new_lens, Tensor):
             if tokens is None:
                 raise ValueError("plan: the number of rows is needed when lengths are on the GPU")
+            self._captured |= torch.cuda.is_current_stream_capturing()
         else:
             if isinstance(new_lens, dict):
                 if any(not 0 <= r < c.max_requests for r in new_lens):
@@ -374,6 +391,7 @@ class PagedKVCache:
         if isinstance(requests, Tensor):
             mask = requests
             _ints(mask, (c.max_requests,), self.device, "release")
+            self._captured |= torch.cuda.is_current_stream_capturing()
             self._lens = None
         else:
             ending = set(requests)
@@ -407,6 +425,7 @@ class PagedKVCache:
         layer = self.layers[layer_idx]
         if layer.head_dim != 128:
             raise ValueError("prefill needs head_dim 128: use attend")
+        q = _rows(q, step.tokens, q.shape[1] if q.dim() == 3 else 0, layer, "q")
         if step.lengths is None:
             step.check()
             start, end = step.query_start.tolist(), step.seq_lens.tolist()

@@ -2,6 +2,7 @@
 
 Tables, codes and scales have to be equal.  Attention is held to a bound that is derived per output element (``_bound``)."""
 
+import copy
 import math
 import random
 
@@ -309,6 +310,21 @@ def test_attend_peaked_and_flat_scores(cuda_lib):
     _check_attend(model, step, [1] * 3, q, out, scale=1.0)
 
 
+@pytest.mark.parametrize("tokens", [5, 16, 100])
+def test_attend_scores_far_below_zero(tokens, cuda_lib):
+    cache, model = _cache(1, 1, 64, 16, torch.bfloat16), _Model(1, 1, 64, 16, torch.bfloat16)
+    k = torch.full((tokens, 1, 64), 2.0 ** 54, dtype=torch.bfloat16, device=DEV)
+    k[3] *= 0.25                                                       # all scores below -1e32, this one by far the largest
+    v = _rand(k.shape, 1, torch.bfloat16)
+    step = cache.plan([tokens])
+    cache.append(0, step, k, v)
+    model.add(0, k, v)
+    out = pc.attend_blocks(cache.layers[0], step, torch.full((tokens, 1, 64), -(2.0 ** 53), dtype=torch.bfloat16, device=DEV))
+    want = model.dense(model.v[0])[0, 3]
+    # one probability is 1 and the others vanish: the result's rounding is below 2^-8 / (1 + 2^-8), those of an fp32 product and quotient below 2^-22
+    assert bool(((out[3:, 0].double() - want).abs() <= 2.0 ** -8 * want.abs()).all())
+
+
 @pytest.mark.parametrize("big", [3e4, 1e-6])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_attend_query_magnitudes(big, dtype, cuda_lib):
@@ -435,6 +451,40 @@ def test_requests_come_and_go(cuda_lib):
         _check_attend(model, step, new, q, pc.attend_blocks(cache.layers[0], step, q))
 
 
+def test_release_of_many_blocks(cuda_lib):
+    """More requests than threads and a long one among them: the stack holds their blocks in request order, each once."""
+    requests, bs = 700, 16
+    cache = _cache(requests, 1, 64, bs, torch.float16, blocks=3000, max_len=20000)
+    new = [(17 * r) % 40 for r in range(requests)]
+    new[5] = 15000
+    cache.plan(new)
+    table, free = cache.block_table.tolist(), cache.free_blocks.tolist()
+    count = cache.free_block_count()
+    assert count == int(cache.free_count) == 3000 - sum(-(-n // bs) for n in new)
+    ending = [r for r in range(requests) if r % 3 or r == 699]
+    cache.release(ending + ending[:7])
+    back = [b for r in ending for b in table[r][: -(-new[r] // bs)]]
+    assert cache.free_blocks.tolist() == free[:count] + back + free[count + len(back):]
+    assert cache.free_block_count() == int(cache.free_count) == count + len(back)
+    assert cache.seq_lens.tolist() == [0 if r in set(ending) else n for r, n in enumerate(new)]
+    cache.release(ending)
+    assert int(cache.free_count) == count + len(back)
+
+
+def test_copies_of_a_cache_are_caches_of_their_own(cuda_lib):
+    cache, model = _cache(2, 2, 64, 16, torch.float16), _Model(2, 2, 64, 16, torch.float16)
+    _feed(cache, model, [40, 9], 1)
+    twin = copy.deepcopy(cache)
+    layer = pc.PagedLayer._make(cache.layers[0])
+    assert twin.layers[0]._c != cache.layers[0]._c != layer._c and layer._replace(tail_k=twin.layers[0].tail_k).tail_k is twin.layers[0].tail_k
+    before = [t.clone() for t in (*twin.layers[0], twin.seq_lens, twin.block_table, twin.free_blocks, twin.free_count)]
+    _feed(cache, model, [30, 30], 5)
+    assert all(torch.equal(a, b) for a, b in zip(before, (*twin.layers[0], twin.seq_lens, twin.block_table, twin.free_blocks, twin.free_count)))
+    step = twin.plan([0, 1])
+    twin.append(0, step, *(_rand((1, 2, 64), i, torch.float16) for i in (8, 9)))
+    assert twin.seq_lens.tolist() == [40, 10] and cache.seq_lens.tolist() == [70, 39]
+
+
 def test_prefill_then_decode(cuda_lib):
     h, group, d = 2, 4, 128
     cache, model = _cache(3, h, d, 32, torch.bfloat16, layers=2), _Model(3, h, d, 32, torch.bfloat16)
@@ -507,6 +557,29 @@ def test_captured_steps_replay(cuda_lib):
                 model.add(r, k[r:r + 1], v[r:r + 1])
             step.check()
             _check_attend(model, step, [1] * requests, q, out)
+
+
+def test_a_captured_plan_takes_the_lengths_from_the_host(cuda_lib):
+    """A replay moves lengths that the host had counted: after it was captured the host asks the GPU, a reset included."""
+    cache, model = _cache(2, 1, 128, 16, torch.float16), _Model(2, 1, 128, 16, torch.float16)
+    new = _i32([20, 3])
+    q, k, v = (_rand((23, n, 128), 7 + n, torch.float16) for n in (2, 1, 1))
+    cache.attend(0, cache.plan(new, tokens=23), q, k, v)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.append(0, cache.plan(new, tokens=23), k, v)
+    cache.reset()
+    assert cache.seq_len(0) == 0 and cache.free_block_count() == 200
+    graph.replay()
+    assert cache.seq_len(0) == 20 and cache.free_block_count() == 197
+    for r, rows in enumerate((slice(0, 20), slice(20, 23))):
+        model.add(r, k[rows], v[rows])
+    step = cache.plan([0, 1])
+    q1, k1, v1 = (_rand((1, n, 128), 70 + n, torch.float16) for n in (2, 1, 1))
+    out = cache.prefill(0, step, q1, k1, v1)
+    model.add(1, k1, v1)
+    want, bound = model.attend(1, q1[0], 4, 128 ** -0.5)
+    assert bool(((out[0].double() - want).abs() <= bound + 2.0 ** -11 * want.abs()).all())       # four open rows: nothing is in 8 bits
 
 
 def test_two_streams_at_once(cuda_lib):

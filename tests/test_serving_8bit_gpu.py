@@ -195,6 +195,11 @@ def test_refusals(cuda_lib):
     for bs, rows in ((8, 2), (128, 2), (16, -1)):
         with pytest.raises(ValueError):
             pc.plan_blocks(*lens, bs, rows)
+    long = PagedKVCache(1, 2, 128, PagedKVConfig(10, 16, 3, 100), dtype=torch.float16, device=DEV)
+    step, rows = long.plan([3, 0, 0]), torch.zeros(3, 2, 128, dtype=torch.float16, device=DEV)
+    for bad in (rows[:2], rows[0], rows.float(), rows.cpu()):
+        with pytest.raises((ValueError, IndexError)):
+            long.prefill(0, step, bad, rows, rows)
     many = PagedKVCache(1, 1, 64, PagedKVConfig(300, 16, 1, 4800), dtype=torch.float16, device=DEV)
     step = many.plan([4097])
     with pytest.raises(ValueError, match="at most 4096"):
