@@ -10,7 +10,12 @@ constexpr int kMaxRequests = 4096;
 constexpr int kMaxQueryTokens = 4096;      // tokens of a step that attention is planned for
 constexpr int kMaxTokens = 1 << 22;
 constexpr int kUnit = 16;                  // tokens per unit of attention work
+constexpr int kPacks = 4;                  // attention tiles of 1, 2, 4, 8 tokens of a request: a table of units for each
 constexpr int kItemInts = 8;               // request, block id, first row, offset in the block, tokens, block index, length before, length after
+
+// Whether tokens of a request share tiles: where there are more rows than requests, some request has several new tokens.  (8 requests x
+// 8 tokens over 2000, 16 query and KV heads: 191 -> 86 us for two layers.)
+__host__ __device__ inline bool packs_tokens(int R, int T) { return T > R; }
 
 inline bool block_size_ok(int bs) { return bs == 16 || bs == 32 || bs == 64; }
 
@@ -22,7 +27,7 @@ inline int max_items(int R, int T, int bs) {
 
 // A step: one buffer of 32-bit words, every array on a 16-byte boundary.
 struct StepLayout {
-  int64_t status, query_start, seq_lens, context_start, token_request, positions, slots, unit_start, info, items, words;
+  int64_t status, query_start, seq_lens, context_start, token_request, positions, slots, unit_start, unit_stride, info, items, words;
   int n_items;
   bool units;
   __host__ StepLayout(int R, int T, int bs) {
@@ -37,7 +42,8 @@ struct StepLayout {
     token_request = slots + up(2 * (int64_t)T);
     positions = token_request + up(T);
     unit_start = positions + up(T);
-    info = unit_start + up(units ? T + 1 : 0);     // [T] request, position, length after the step, 0
+    unit_stride = up((int64_t)T + 1);
+    info = unit_start + (units ? kPacks * unit_stride : 0);     // [T] request, position, length after the step, number in the request's rows
     items = info + (units ? 4 * (int64_t)T : 0);
     words = items + (int64_t)n_items * kItemInts;
   }

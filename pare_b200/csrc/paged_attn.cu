@@ -50,8 +50,8 @@ struct PagedAttnParams {
   int64_t q_st, q_sh;
   void* out;
   int64_t o_st, o_sh;
-  const int4* info;          // [T] request, position, length after the step
-  const int* unit_start;     // [T + 1]
+  const int4* info;          // [T] request, position, length after the step, number in the request's rows
+  const int* unit_start;     // [T + 1], of tiles of `pack` tokens
   const int* table;
   int64_t ld_table;
   const int8_t* k_codes;
@@ -63,6 +63,7 @@ struct PagedAttnParams {
   float* parts;              // [warp][2]: of a tile that warps before it began, of one that it begins
   float scale_log2;
   int T, R, H, group, sub, bs_log2, num_blocks, max_blocks;   // sub: tiles of eight heads per KV head
+  int pack, per_group;       // tokens of a tile at most, 256 / group rounded up
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
@@ -124,13 +125,28 @@ __device__ __forceinline__ float sum_over_g(float v) {
   return v;
 }
 
+// Which of a tile's tokens a column belongs to: c / group for the groups that share tiles
+template <bool PACKED>
+__device__ __forceinline__ int token_of(const PagedAttnParams& p, int c) {
+  return PACKED ? c * p.per_group >> 8 : 0;
+}
+
+// Where a column of a tile goes, nullptr if it is nobody's.  A tile's columns are the `heads` heads of its first token, of the next, ..;
+// `earlier` tokens before the last one, which is token t.
+template <typename T, bool PACKED>
+__device__ __forceinline__ T* column_out(const PagedAttnParams& p, int t, int c, int earlier, int head0, int heads) {
+  const int token = token_of<PACKED>(p, c), head = c - token * p.group;
+  return token <= earlier && head < heads ? reinterpret_cast<T*>(p.out) + (int64_t)(t - earlier + token) * p.o_st + (int64_t)(head0 + head) * p.o_sh
+                                          : nullptr;
+}
+
 // Units of a run: equal shares, but not so few that the parts outweigh the work.
 __device__ __forceinline__ int64_t run_units(int64_t total, int warps) {
   const int64_t each = (total + warps - 1) / warps;
   return each < kMinRun ? kMinRun : each;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool PACKED>
 struct Tile {
   using S = Shape<D>;
   // Rounding a probability to fp16 is off by 2^-11 of it: nothing beside a bf16 result, as much as the rounding of an fp16 result.
@@ -199,15 +215,17 @@ struct Tile {
     f1 = __shfl_sync(0xffffffffu, back, 8 * t + 4) * scale_log2;
   }
 
-  // Sums of products of tokens g, g + 8 x heads 2 t, 2 t + 1, their factors to scores in base 2, and how many of the tokens are visible
-  // -> probabilities in place
-  __device__ __forceinline__ void softmax(float (&s)[4], float s0, float s1, int seen, int g) {
+  // Sums of products of tokens g, g + 8 x heads 2 t, 2 t + 1, their factors to scores in base 2, and how many of the tokens are visible to
+  // those heads (`least`: to any) -> probabilities in place
+  __device__ __forceinline__ void softmax(float (&s)[4], float s0, float s1, int least, int seen0, int seen1, int g) {
     float x[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = fmaf(s[i], (i & 1) ? s1 : s0, (i & 1) ? kBias - m1 : kBias - m0);
-    if (seen < kUnit) {
-      if (g >= seen) x[0] = x[1] = -INFINITY;
-      if (g + 8 >= seen) x[2] = x[3] = -INFINITY;
+    if (least < kUnit) {
+      if (g >= seen0) x[0] = -INFINITY;
+      if (g >= seen1) x[1] = -INFINITY;
+      if (g + 8 >= seen0) x[2] = -INFINITY;
+      if (g + 8 >= seen1) x[3] = -INFINITY;
     }
     if (__any_sync(0xffffffffu, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) > kBias + kSlack)) {
       // the reference moves up to the largest score
@@ -237,8 +255,8 @@ struct Tile {
     l1 += s[1] + s[3];
   }
 
-  // 16 tokens in 8 bits from a stage of the ring; `seen`: how many of them are visible
-  __device__ __forceinline__ void quantized_unit(uint32_t stage, float ks, float vs, int seen, int lane) {
+  // 16 tokens in 8 bits from a stage of the ring; `least`, `seen0`, `seen1`: how many of them are visible
+  __device__ __forceinline__ void quantized_unit(uint32_t stage, float ks, float vs, int least, int seen0, int seen1, int lane) {
     const int g = lane >> 2, t = lane & 3;
     float acc[kJ][4];
 #pragma unroll
@@ -257,7 +275,9 @@ struct Tile {
     float s[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) s[i] = kJ == 2 ? acc[0][i] + acc[kJ - 1][i] : acc[0][i];
-    softmax(s, ks * f0, ks * f1, seen, g);
+    softmax(s, ks * f0, ks * f1, least, seen0, seen1, g);
+    // a block that a head does not see at all may have a scale that is not finite
+    const float vs0 = PACKED && seen0 <= 0 ? 0.f : vs, vs1 = PACKED && seen1 <= 0 ? 0.f : vs;
     const uint32_t h0 = pack_half2(s[0], s[1]), h1 = pack_half2(s[2], s[3]), p0 = transpose8x8(h0), p1 = transpose8x8(h1);
     uint32_t r0 = 0, r1 = 0;       // what the rounding left
     if constexpr (kTwoTerms) {
@@ -294,15 +314,17 @@ struct Tile {
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        o[2 * w][i] = fmaf(vs, x[i], o[2 * w][i]);
-        o[2 * w + 1][i] = fmaf(vs, y[i], o[2 * w + 1][i]);
+        o[2 * w][i] = fmaf((i & 1) ? vs1 : vs0, x[i], o[2 * w][i]);
+        o[2 * w + 1][i] = fmaf((i & 1) ? vs1 : vs0, y[i], o[2 * w + 1][i]);
       }
     }
   }
 
-  // Up to 16 open tokens in 16 bits: the keys in one stage of the ring, the values in another.  Hidden rows (later tokens,
-  // leftovers) were not loaded, they are zeros: what lies there may be infinite.  Probabilities in two terms, in the rows' type.
-  __device__ __forceinline__ void open_unit(uint32_t stage_k, uint32_t stage_v, const T* q_row, float scale_log2, int seen, int lane) {
+  // Up to 16 open tokens in 16 bits: the keys in one stage of the ring, the values in another.  Rows that are hidden to a head (later
+  // tokens, leftovers) were not loaded, they are zeros: what lies there may be infinite.  Values that some of the heads see (`most`
+  // rows are visible to any, `least` to all; v_rows: where they are) are added one by one.  Probabilities in two terms, in the rows' type.
+  __device__ __forceinline__ void open_unit(uint32_t stage_k, uint32_t stage_v, const T* q_row, const T* v_rows, float scale_log2, int least, int most,
+                                            int seen0, int seen1, int lane) {
     const int g = lane >> 2, t = lane & 3;
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -324,7 +346,19 @@ struct Tile {
       for (int w = 0; w < 4; ++w) mma16816<T>(acc, wa[2 * w], wb[2 * w], wa[2 * w + 1], wb[2 * w + 1], wq[2 * w], wq[2 * w + 1]);
     }
     float s[4] = {acc[0], acc[1], acc[2], acc[3]};
-    softmax(s, scale_log2, scale_log2, seen, g);
+    softmax(s, scale_log2, scale_log2, least, seen0, seen1, g);
+#pragma unroll 1
+    for (int row = PACKED ? max(least, 0) : kUnit; row < min(most, kUnit); ++row) {
+      const float y0 = __shfl_sync(0xffffffffu, row < 8 ? s[0] : s[2], 4 * (row & 7) + t), y1 = __shfl_sync(0xffffffffu, row < 8 ? s[1] : s[3], 4 * (row & 7) + t);
+      const T* v = v_rows + row * D + (D / 8) * g;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        const uint32_t two = *reinterpret_cast<const uint32_t*>(v + 2 * i);
+        const T* e = reinterpret_cast<const T*>(&two);
+        if (row < seen0) o[i][0] = fmaf(y0, to_float<T>(e[0]), o[i][0]), o[i][2] = fmaf(y0, to_float<T>(e[1]), o[i][2]);
+        if (row < seen1) o[i][1] = fmaf(y1, to_float<T>(e[0]), o[i][1]), o[i][3] = fmaf(y1, to_float<T>(e[1]), o[i][3]);
+      }
+    }
     uint32_t p0, p1, r0, r1;
     if constexpr (std::is_same<T, __half>::value) {
       const uint32_t a = pack_half2(s[0], s[1]), b = pack_half2(s[2], s[3]);
@@ -366,7 +400,7 @@ struct Tile {
   __device__ static __forceinline__ int open_value_swizzle(int t) { return D == 128 ? (t & 1) | ((t >> 1) << 2) : 2 * t; }
 };
 
-template <typename T, int D>
+template <typename T, int D, bool PACKED>
 __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttnParams p) {
   using S = Shape<D>;
   extern __shared__ __align__(128) unsigned char smem[];
@@ -391,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
   }
 
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem + warp * S::kRing);
-  Tile<T, D> tile;
+  Tile<T, D, PACKED> tile;
 
   // Where this lane's 16-byte chunks of a unit go in a stage: chunk e * 32 + lane of the keys at at_k + 512 e, of the values at
   // at_v[e & 1] + 512 e (the pattern that spreads rows over banks repeats after two rounds)
@@ -415,7 +449,12 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
     const int r = info.x, pos = info.y, end = info.z;
     const int held = end >> p.bs_log2 << p.bs_log2, nq = min(pos + 1, held), nq_units = (nq + kUnit - 1) / kUnit;
     const int hk = h / p.sub, head0 = hk * p.group + (h - hk * p.sub) * kHeads, heads = min(kHeads, (hk + 1) * p.group - head0);
-    const T* q_row = g < heads ? reinterpret_cast<const T*>(p.q) + t * p.q_st + (head0 + g) * p.q_sh : nullptr;
+    const int earlier = PACKED ? info.w & (p.pack - 1) : 0;                // tokens of the tile before its last one, t
+    const int g_token = token_of<PACKED>(p, g), g_head = g - g_token * p.group;
+    // how many tokens the columns 2 t4, 2 t4 + 1 see less than that one
+    const int behind0 = PACKED ? earlier - token_of<PACKED>(p, 2 * t4) : 0, behind1 = PACKED ? earlier - token_of<PACKED>(p, 2 * t4 + 1) : 0;
+    const T* q_row = g_token <= earlier && g_head < heads
+                         ? reinterpret_cast<const T*>(p.q) + (t - earlier + g_token) * p.q_st + (head0 + g_head) * p.q_sh : nullptr;
     const int* row_table = p.table + r * p.ld_table;
     const int n8 = max(0, min(n, nq_units - j0));             // units in 8 bits, then units of open rows: two entries of the ring each
     const int entries = n8 + 2 * (n - n8);
@@ -450,14 +489,15 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
 #pragma unroll
         for (int e = 0; e < S::kChunks; ++e) cp_async16(dst + at_v[e & 1] + e * 512, sv + e * 512, bytes);
       } else if (i < entries) {
-        const int from = (j0 + n8 - nq_units + (i - n8) / 2) * kUnit, seen = pos + 1 - nq - from;   // first row, visible rows
+        const int from = (j0 + n8 - nq_units + (i - n8) / 2) * kUnit;      // first row
         const bool values = (i - n8) & 1;
+        const int seen = pos + 1 - nq - from - (values ? earlier : 0);     // rows visible to any head (keys), to all (values)
         const T* src = reinterpret_cast<const T*>(values ? p.tail_v : p.tail_k) + ((((int64_t)r * p.H + hk) << p.bs_log2) + from) * D;
         const uint32_t dst = ring + slot_in * S::kStageBytes;
 #pragma unroll 1
         for (int e = 0; e < 2 * S::kChunks; ++e) {
           const int row = (e * 32 + lane) / (D / 8), c = (e * 32 + lane) % (D / 8);
-          const int to = c ^ (values ? Tile<T, D>::open_value_swizzle((row >> 1) & 3) : row & 1);
+          const int to = c ^ (values ? Tile<T, D, PACKED>::open_value_swizzle((row >> 1) & 3) : row & 1);
           const bool there = row < seen;
           cp_async16(dst + row * 2 * D + to * 16, there ? src + row * D + c * 8 : src, there ? 16 : 0);
         }
@@ -477,7 +517,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
       const float ks = __shfl_sync(0xffffffffu, kss, i & 31), vs = __shfl_sync(0xffffffffu, vss, i & 31);
       asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
       __syncwarp();
-      tile.quantized_unit(ring + slot * S::kStageBytes, ks, vs, nq - (j0 + i) * kUnit, lane);
+      const int seen = pos + 1 - (j0 + i) * kUnit;
+      tile.quantized_unit(ring + slot * S::kStageBytes, ks, vs, seen - earlier, seen - behind0, seen - behind1, lane);
       if (++slot == S::kStages) slot = 0;
       __syncwarp();
       issue(i + S::kStages - 1);
@@ -487,8 +528,10 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
       asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 3) : "memory");
       __syncwarp();
       const int next = slot + 1 == S::kStages ? 0 : slot + 1;
-      tile.open_unit(ring + slot * S::kStageBytes, ring + next * S::kStageBytes, q_row, p.scale_log2,
-                     pos + 1 - nq - (j0 + n8 - nq_units + (i - n8) / 2) * kUnit, lane);
+      const int from = (j0 + n8 - nq_units + (i - n8) / 2) * kUnit, seen = pos + 1 - nq - from;
+      tile.open_unit(ring + slot * S::kStageBytes, ring + next * S::kStageBytes, q_row,
+                     reinterpret_cast<const T*>(p.tail_v) + ((((int64_t)r * p.H + hk) << p.bs_log2) + from) * D, p.scale_log2, seen - earlier, seen,
+                     seen - behind0, seen - behind1, lane);
       slot = next + 1 == S::kStages ? 0 : next + 1;
       __syncwarp();
       issue(i + S::kStages - 1);
@@ -500,12 +543,13 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
     const float l0 = sum_over_g(tile.l0), l1 = sum_over_g(tile.l1);
     if (n == units) {
       const float y0 = 1.f / l0, y1 = 1.f / l1;
-      T* out = reinterpret_cast<T*>(p.out) + t * p.o_st + (int64_t)(head0 + 2 * t4) * p.o_sh;
+      T* out0 = column_out<T, PACKED>(p, t, 2 * t4, earlier, head0, heads);
+      T* out1 = column_out<T, PACKED>(p, t, 2 * t4 + 1, earlier, head0, heads);
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
         const int c = (D / 8) * g + 2 * i;
-        if (2 * t4 < heads) out[c] = from_float<T>(tile.o[i][0] * y0), out[c + 1] = from_float<T>(tile.o[i][2] * y0);
-        if (2 * t4 + 1 < heads) out[p.o_sh + c] = from_float<T>(tile.o[i][1] * y1), out[p.o_sh + c + 1] = from_float<T>(tile.o[i][3] * y1);
+        if (out0) out0[c] = from_float<T>(tile.o[i][0] * y0), out0[c + 1] = from_float<T>(tile.o[i][2] * y0);
+        if (out1) out1[c] = from_float<T>(tile.o[i][1] * y1), out1[c + 1] = from_float<T>(tile.o[i][3] * y1);
       }
     } else {
       float* part = p.parts + ((int64_t)me * 2 + (j0 == 0 ? 1 : 0)) * S::kPartFloats;
@@ -536,14 +580,14 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
 // many (one sequence: 86): GROUPS warps share a piece, each every GROUPS-th part, and are added up in order.  A warp alone gets
 // through one instruction in about eight cycles, so what is serial counts: 8 tiles of 4096 tokens, both kernels, 22.7 / 15.8 / 13.1 / 12.7 us
 // with 2 / 4 / 8 / 16 groups; 64 tiles of 32768 tokens 101 / 99 / 99 / 106 us, 108 with one.
-template <typename T, int D, int GROUPS>
+template <typename T, int D, int GROUPS, bool PACKED>
 __global__ void __launch_bounds__(GROUPS > 1 ? GROUPS * 32 : D * 2) paged_merge_kernel(const PagedAttnParams p, int warps) {
   using S = Shape<D>;
   constexpr int kFlight = 4;     // parts in flight per warp
   __shared__ float4 s_o[GROUPS][32], s_ml[GROUPS][32];
-  pdl_wait();
   const int tiles = p.H * p.sub, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   const int group = GROUPS > 1 ? warp : 0, piece = GROUPS > 1 ? blockIdx.y : warp;
+  pdl_wait();
   const int64_t total = (int64_t)p.unit_start[p.T] * tiles, run = run_units(total, warps);
   auto run_of = [&](int64_t u) { return total >> 32 ? (int)(u / run) : (int)((uint32_t)u / (uint32_t)run); };
   for (int job = blockIdx.x; job < p.T * tiles; job += gridDim.x) {
@@ -592,9 +636,18 @@ __global__ void __launch_bounds__(GROUPS > 1 ? GROUPS * 32 : D * 2) paged_merge_
       }
     }
     const int hk = h / p.sub, head0 = hk * p.group + (h - hk * p.sub) * kHeads, heads = min(kHeads, (hk + 1) * p.group - head0);
-    T* out = reinterpret_cast<T*>(p.out) + t * p.o_st + (int64_t)(head0 + 2 * t4) * p.o_sh + (D / 8) * g + 2 * piece;
-    if (2 * t4 < heads) out[0] = from_float<T>(o.x / l.x), out[1] = from_float<T>(o.z / l.x);
-    if (2 * t4 + 1 < heads) out[p.o_sh] = from_float<T>(o.y / l.y), out[p.o_sh + 1] = from_float<T>(o.w / l.y);
+    const int earlier = PACKED ? p.info[t].w & (p.pack - 1) : 0, c = (D / 8) * g + 2 * piece;
+    T *out0, *out1;
+    if constexpr (PACKED) {
+      out0 = column_out<T, PACKED>(p, t, 2 * t4, earlier, head0, heads);
+      out1 = column_out<T, PACKED>(p, t, 2 * t4 + 1, earlier, head0, heads);
+    } else {
+      out0 = reinterpret_cast<T*>(p.out) + t * p.o_st + (int64_t)(head0 + 2 * t4) * p.o_sh;
+      out1 = 2 * t4 + 1 < heads ? out0 + p.o_sh : nullptr;
+      if (2 * t4 >= heads) out0 = nullptr;
+    }
+    if (out0) out0[c] = from_float<T>(o.x / l.x), out0[c + 1] = from_float<T>(o.z / l.x);
+    if (out1) out1[c] = from_float<T>(o.y / l.y), out1[c + 1] = from_float<T>(o.w / l.y);
   }
 }
 
@@ -627,21 +680,23 @@ int pare_paged_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h, const
   PARE_REQUIRE(aligned16(q) && (q_stride_t | q_stride_h) % 8 == 0 && aligned16(workspace), PARE_ERR_ALIGN);
   const int blocks = attn_blocks();
   PARE_REQUIRE(workspace && workspace_bytes >= workspace_of(D, blocks), PARE_ERR_WORKSPACE);
-  const int group = Hq / H, sub = (group + kHeads - 1) / kHeads;
+  const int group = Hq / H, sub = (group + kHeads - 1) / kHeads, packs = !packs_tokens(tb->R, T) || group > 4 ? 0 : group == 1 ? 3 : group == 2 ? 2 : 1;
   PARE_REQUIRE((int64_t)T * H * sub < (int64_t)1 << 31, PARE_ERR_UNSUPPORTED);
   // the step counts its units in 32 bits
   PARE_REQUIRE(T * ((int64_t)tb->max_blocks * l->block_size / kUnit + 2) < (int64_t)1 << 31, PARE_ERR_UNSUPPORTED);
   const StepLayout s(tb->R, T, l->block_size);
   const int* w = reinterpret_cast<const int*>(tb->step);
   const PagedAttnParams p{q, q_stride_t, q_stride_h, out, out_stride_t, out_stride_h, reinterpret_cast<const int4*>(w + s.info),
-                          w + s.unit_start, tb->block_table, tb->ld_table, l->k_codes, l->v_codes, l->k_scale, l->v_scale, l->tail_k, l->tail_v,
+                          w + s.unit_start + packs * s.unit_stride, tb->block_table, tb->ld_table, l->k_codes, l->v_codes, l->k_scale, l->v_scale, l->tail_k, l->tail_v,
                           reinterpret_cast<float*>(workspace), softmax_scale * kLog2e, T, tb->R, H, group, sub,
-                          l->block_size == 16 ? 4 : l->block_size == 32 ? 5 : 6, l->num_blocks, tb->max_blocks};
+                          l->block_size == 16 ? 4 : l->block_size == 32 ? 5 : 6, l->num_blocks, tb->max_blocks,
+                          1 << packs, (256 + group - 1) / group};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  auto by_dim = [&](auto tag, auto dim) {
+  auto go = [&](auto tag, auto dim, auto packed) {
     using E = decltype(tag);
     constexpr int kD = decltype(dim)::value;
-    const auto kern = paged_attn_kernel<E, kD>;
+    constexpr bool kPacked = decltype(packed)::value;
+    const auto kern = paged_attn_kernel<E, kD, kPacked>;
     if (!ensure_smem_attr(reinterpret_cast<const void*>(kern), (int)Shape<kD>::kSmem)) return (int)PARE_ERR_CUDA;
     int status = launch_pdl(kern, dim3(blocks), dim3(kThreads), Shape<kD>::kSmem, st, p);
     if (status != PARE_OK) return status;
@@ -650,11 +705,12 @@ int pare_paged_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h, const
       return groups > 1 ? launch_pdl(kernel, dim3(jobs, kD / 16), dim3(groups * 32), 0, st, p, warps)
                         : launch_pdl(kernel, dim3(std::min(jobs, 32 * sms)), dim3(2 * kD), 0, st, p, warps);
     };
-    if (8 * jobs <= sms) status = merge(paged_merge_kernel<E, kD, 16>, 16);
-    else if (jobs <= sms) status = merge(paged_merge_kernel<E, kD, 8>, 8);
-    else status = merge(paged_merge_kernel<E, kD, 1>, 1);
+    if (8 * jobs <= sms) status = merge(paged_merge_kernel<E, kD, 16, kPacked>, 16);
+    else if (jobs <= sms) status = merge(paged_merge_kernel<E, kD, 8, kPacked>, 8);
+    else status = merge(paged_merge_kernel<E, kD, 1, kPacked>, 1);
     return status != PARE_OK ? status : launch_status();
   };
+  auto by_dim = [&](auto tag, auto dim) { return packs ? go(tag, dim, std::true_type()) : go(tag, dim, std::false_type()); };
   auto by_type = [&](auto dim) { return l->dtype == PARE_F16 ? by_dim(__half(), dim) : by_dim(__nv_bfloat16(), dim); };
   return D == 64 ? by_type(std::integral_constant<int, 64>()) : by_type(std::integral_constant<int, 128>());
 }

@@ -34,22 +34,22 @@ struct PlanParams {
   const int* free_blocks;
   const int* free_count;
   int* step;
-  int64_t o_query_start, o_seq_lens, o_context, o_slots, o_request, o_positions, o_units, o_info, o_items;
+  int64_t o_query_start, o_seq_lens, o_context, o_slots, o_request, o_positions, o_units, unit_stride, o_info, o_items;
   int R, T, bs_log2, max_blocks, free_capacity, n_items, units;
 };
 
 // Exclusive prefix sums of N values per thread, and their totals.  All threads call it.
-template <int N>
-__device__ __forceinline__ void block_scan(const long long (&v)[N], long long (&before)[N], long long (&total)[N], long long (*sums)[kPlanWarps]) {
+template <int N, typename V>
+__device__ __forceinline__ void block_scan(const V (&v)[N], V (&before)[N], V (&total)[N], long long (*sums)[kPlanWarps]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long x[N];
+  V x[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) x[i] = v[i];
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const long long y = __shfl_up_sync(0xffffffffu, x[i], o);
+      const V y = __shfl_up_sync(0xffffffffu, x[i], o);
       if (lane >= o) x[i] += y;
     }
   }
@@ -62,7 +62,7 @@ __device__ __forceinline__ void block_scan(const long long (&v)[N], long long (&
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     // the warps' sums, one per lane
-    long long s = lane < kPlanWarps ? sums[i][lane] : 0, mine = lane < warp ? s : 0;
+    V s = lane < kPlanWarps ? (V)sums[i][lane] : 0, mine = lane < warp ? s : 0;
 #pragma unroll
     for (int o = kPlanWarps / 2; o > 0; o >>= 1) {
       s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
     }
   }
   if (count < 0 || count > p.free_capacity) bad |= PARE_PAGED_BLOCKS;
-  block_scan<4>(sum, before, total, s_sums);
+  block_scan(sum, before, total, s_sums);
   if (total[0] > p.T) bad |= PARE_PAGED_ROWS;
   if (total[1] > count) bad |= PARE_PAGED_BLOCKS;
   if (bad) atomicOr(&s_bad, bad);
@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
     }
     if (p.units) {
       const int end = r < 0 ? 0 : s_len[r] + (r + 1 < R ? s_start[r + 1] : (int)t_new) - s_start[r];
-      *reinterpret_cast<int4*>(p.step + p.o_info + 4 * (int64_t)i) = make_int4(r, pos, end, 0);
+      *reinterpret_cast<int4*>(p.step + p.o_info + 4 * (int64_t)i) = make_int4(r, pos, end, r < 0 ? 0 : i - s_start[r]);
     }
     p.step[p.o_request + i] = r;
     p.step[p.o_positions + i] = pos;
@@ -196,25 +196,46 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
     const int r = last_at_most(s_take, R, i);
     p.table[r * p.ld_table + ((s_len[r] + bs - 1) >> p.bs_log2) + i - s_take[r]] = p.free_blocks[count - 1 - i];
   }
-  if (lead && p.units) {   // units of attention work before each token: quantized tokens, then open rows, in pieces of kUnit
+  if (lead && p.units) {
+    // Units of attention work before each token: quantized tokens, then open rows, in pieces of kUnit.  Where 2^i tokens of a request
+    // share a tile, its last token has its units and the others have none.
     const int each = (p.T + kPlanThreads - 1) / kPlanThreads;
     const int t0 = min(p.T, (int)threadIdx.x * each), t1 = min(p.T, t0 + each);
-    auto units_of = [&](int t) {
-      if (t >= t_new) return 0;
-      const int r = last_at_most(s_start, R, t), seen = s_len[r] + t - s_start[r] + 1;
-      const int end = s_len[r] + (r + 1 < R ? s_start[r + 1] : (int)t_new) - s_start[r];
-      const int held = end >> p.bs_log2 << p.bs_log2, nq = min(seen, held);
-      return (nq + kUnit - 1) / kUnit + (seen - nq + kUnit - 1) / kUnit;
+    auto tables = [&](auto packs) {
+      constexpr int kN = decltype(packs)::value;
+      auto units_of = [&](int t, int (&n)[kN]) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) n[i] = 0;
+        if (t >= t_new) return;
+        const int r = last_at_most(s_start, R, t), mine = t - s_start[r], seen = s_len[r] + mine + 1;
+        const int end = s_len[r] + (r + 1 < R ? s_start[r + 1] : (int)t_new) - s_start[r];
+        const int held = end >> p.bs_log2 << p.bs_log2, nq = min(seen, held);
+        const int units = (nq + kUnit - 1) / kUnit + (seen - nq + kUnit - 1) / kUnit;
+#pragma unroll
+        for (int i = 0; i < kN; ++i) n[i] = seen == end || (mine + 1) % (1 << i) == 0 ? units : 0;
+      };
+      int sums[kN] = {}, first[kN], all[kN], n[kN];
+      for (int t = t0; t < t1; ++t) {
+        units_of(t, n);
+#pragma unroll
+        for (int i = 0; i < kN; ++i) sums[i] += n[i];
+      }
+      block_scan(sums, first, all, s_sums);
+      for (int t = t0; t < t1; ++t) {
+        units_of(t, n);
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+          p.step[p.o_units + i * p.unit_stride + t] = first[i];
+          first[i] += n[i];
+        }
+      }
+      if (threadIdx.x == 0) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) p.step[p.o_units + i * p.unit_stride + p.T] = all[i];
+      }
     };
-    long long n[1] = {0}, first[1], all[1];
-    for (int t = t0; t < t1; ++t) n[0] += units_of(t);
-    block_scan<1>(n, first, all, s_sums);
-    int at = (int)first[0];
-    for (int t = t0; t < t1; ++t) {
-      p.step[p.o_units + t] = at;
-      at += units_of(t);
-    }
-    if (threadIdx.x == 0) p.step[p.o_units + p.T] = (int)all[0];
+    if (packs_tokens(p.R, p.T)) tables(std::integral_constant<int, kPacks>());
+    else tables(std::integral_constant<int, 1>());
   }
 }
 
@@ -233,7 +254,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_release_kernel(const int* 
   long long n[1] = {0}, before[1], all[1];
   for (int r = r0; r < r1; ++r) n[0] += blocks_of(r);
   const int count = max(0, *free_count);
-  block_scan<1>(n, before, all, s_sums);
+  block_scan(n, before, all, s_sums);
   const int room = max(0, free_capacity - count), given = (int)min((long long)room, all[0]);      // a pool has no more blocks than its stack
   long long at = before[0];
   for (int r = r0; r < r1; ++r) {
@@ -470,7 +491,7 @@ int pare_paged_plan(const int32_t* seq_lens, const int32_t* new_lens, int R, int
   PARE_REQUIRE(step_bytes >= (size_t)s.words * 4, PARE_ERR_WORKSPACE);
   PARE_REQUIRE(aligned16(step), PARE_ERR_ALIGN);
   PlanParams p{seq_lens, new_lens, block_table, ld_table, free_blocks, free_count, reinterpret_cast<int*>(step),
-               s.query_start, s.seq_lens, s.context_start, s.slots, s.token_request, s.positions, s.unit_start, s.info, s.items,
+               s.query_start, s.seq_lens, s.context_start, s.slots, s.token_request, s.positions, s.unit_start, s.unit_stride, s.info, s.items,
                R, T, log2_of(block_size), max_blocks, free_capacity, s.n_items, s.units ? 1 : 0};
   const size_t smem = (size_t)R * 4 * sizeof(int);
   if (!ensure_smem_attr(reinterpret_cast<const void*>(paged_plan_kernel), kMaxRequests * 4 * (int)sizeof(int))) return PARE_ERR_CUDA;

@@ -259,7 +259,8 @@ def test_codes_at_ties_zeros_and_non_finite_blocks(dtype, cuda_lib):
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("h,group,d,bs", [(1, 1, 64, 16), (2, 4, 128, 16), (8, 4, 128, 32), (4, 7, 128, 64), (2, 8, 64, 32), (1, 9, 128, 32),
-                                          (2, 16, 128, 16), (1, 28, 64, 64)])
+                                          (2, 16, 128, 16), (1, 28, 64, 64),
+                                          (2, 1, 128, 16), (1, 2, 64, 32), (2, 3, 128, 32), (3, 5, 64, 16), (4, 2, 128, 64)])
 def test_attend_ragged_steps(h, group, d, bs, dtype, cuda_lib):
     requests = 6
     cache, model = _cache(requests, h, d, bs, dtype, blocks=400), _Model(requests, h, d, bs, dtype)
@@ -362,6 +363,27 @@ def test_hidden_rows_do_not_reach_a_query(cuda_lib):
                 assert bool(((out[row + i].double() - want).abs() <= bound).all()), (r, i)
             row += 9
         assert out[8].isnan().all() and out[47:].isnan().any(dim=-1).all()
+
+
+@pytest.mark.parametrize("group", [1, 2, 4])
+def test_blocks_that_fill_up_with_nan_do_not_reach_earlier_tokens(group, cuda_lib):
+    """Tokens of a step that share a tile, on both sides of a block's border: the first ones do not see the block behind it."""
+    for dtype, d in ((torch.float16, 128), (torch.bfloat16, 64)):
+        cache, model = _cache(1, 2, d, 32, dtype), _Model(1, 2, d, 32, dtype)
+        _feed(cache, model, [2 if group > 1 else 3], 5)
+        n, old = 70, model.k[0].shape[1]
+        step = cache.plan([n])
+        k, v, q = _rand((n, 2, d), 1, dtype), _rand((n, 2, d), 2, dtype), _rand((n, 2 * group, d), 3, dtype)
+        k[40], v[40] = float("nan"), float("inf")                      # in the second block, all of which has no scale any more
+        cache.append(0, step, k, v)
+        model.add(0, k, v)
+        out = pc.attend_blocks(cache.layers[0], step, q)
+        first = _Model(1, 2, d, 32, dtype)
+        first.k[0], first.v[0] = model.k[0][:, :32], model.v[0][:, :32]
+        for i in range(32 - old):
+            want, bound = first.attend(0, q[i], old + i + 1, 1 / math.sqrt(d))
+            assert bool(((out[i].double() - want).abs() <= bound).all()), i
+        assert out[32 - old:].isnan().all()
 
 
 def test_padded_rows_stay_and_strided_inputs(cuda_lib):
