@@ -217,22 +217,30 @@ def _fits(layer: PagedLayer, step: PagedStep) -> None:
                          f"{step.block_size}, {step.device}) do not belong together")
 
 
-def _rows(t: Tensor, tokens: int, heads: int, layer: PagedLayer, what: str) -> Tensor:
-    """A step's rows as the kernels take them: channels adjacent, 16-byte aligned rows."""
+def _rows(t: Tensor, tokens: int, heads: int, layer: PagedLayer, what: str) -> tuple[Tensor, int, int, int]:
+    """A step's rows as the kernels take them (channels adjacent, 16-byte aligned rows), their address and strides."""
     if t.shape != (tokens, heads, layer.head_dim) or t.dtype is not layer.dtype or t.device != layer.device:
         raise ValueError(f"{what} must be {layer.dtype} {[tokens, heads, layer.head_dim]} on {layer.device}, got {t.dtype} {list(t.shape)} on {t.device}")
-    a, b, c = t.stride()
-    return t if c == 1 and (a | b) % 8 == 0 and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+    (a, b, c), p = t.stride(), t.data_ptr()
+    if c == 1 and not (a | b) & 7 and not p & 15:
+        return t, p, a, b
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.data_ptr(), t.stride(0), t.stride(1)
 
 
 def append_blocks(layer: PagedLayer, step: PagedStep, k: Tensor, v: Tensor) -> None:
     """Store the step's new keys and values ``[tokens, H, D]`` in one layer: blocks that fill up are quantized into the pool, the
     rest goes to the open rows."""
     _fits(layer, step)
-    k, v = _rows(k, step.tokens, layer.heads, layer, "k"), _rows(v, step.tokens, layer.heads, layer, "v")
-    ks, vs = k.stride(), v.stride()
-    _call(layer.device, _lib.lib().pare_paged_append, "pare_paged_append", k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1],
-          layer._c, step._tables())
+    tokens, heads, dev = step.tokens, layer.heads, layer.device
+    k, kp, kt, kh = _rows(k, tokens, heads, layer, "k")
+    v, vp, vt, vh = _rows(v, tokens, heads, layer, "v")
+    if dev.index != _lib.current_device():
+        with torch.cuda.device(dev):
+            return append_blocks(layer, step, k, v)
+    status = _lib.lib().pare_paged_append(kp, vp, kt, kh, vt, vh, layer._c, step._c or step._tables(), _lib.current_stream(dev))
+    if status:
+        _lib.check(status, "pare_paged_append")
 
 
 def dense_blocks(layer: PagedLayer, step: PagedStep, total: int) -> tuple[Tensor, Tensor]:
@@ -260,22 +268,25 @@ def attend_blocks(layer: PagedLayer, step: PagedStep, q: Tensor, scale: float | 
     ``out`` (``[tokens, Hq, D]``, channels adjacent, not overlapping ``q``; a new tensor if not given)."""
     _fits(layer, step)
     tokens, d, dev = step.tokens, layer.head_dim, layer.device
-    hq = q.shape[1] if q.dim() == 3 else 0
+    hq = q.size(1) if q.dim() == 3 else 0
     if hq == 0 or hq % layer.heads:
         raise ValueError(f"attend_blocks: q [tokens, heads, {d}] with a multiple of {layer.heads} heads, got {list(q.shape)}")
     if tokens > MAX_QUERY_TOKENS:
         raise ValueError(f"attend_blocks takes at most {MAX_QUERY_TOKENS} rows, got {tokens}")
-    q = _rows(q, tokens, hq, layer, "q")
+    q, qp, qt, qh = _rows(q, tokens, hq, layer, "q")
     if out is None:
         out = q.new_empty(tokens, hq, d)
+        ot, oh = hq * d, d
     elif out.shape != q.shape or out.dtype is not q.dtype or out.device != dev or out.stride(2) != 1:
         raise ValueError(f"out must be {q.dtype} {list(q.shape)} on {dev} with adjacent channels")
+    else:
+        ot, oh, _ = out.stride()
     if dev.index != _lib.current_device():
         with torch.cuda.device(dev):
             return attend_blocks(layer, step, q, scale, out)
-    stream, nbytes, qs, os = _lib.current_stream(dev), _attn_workspace(d, dev.index), q.stride(), out.stride()
+    stream, nbytes = _lib.current_stream(dev), _attn_workspace(d, dev.index)
     ws = _lib.scratch(dev, nbytes, stream)
-    status = _lib.lib().pare_paged_attn(q.data_ptr(), qs[0], qs[1], layer._c, step._tables(), hq, out.data_ptr(), os[0], os[1],
+    status = _lib.lib().pare_paged_attn(qp, qt, qh, layer._c, step._c or step._tables(), hq, out.data_ptr(), ot, oh,
                                         1.0 / math.sqrt(d) if scale is None else scale, ws.data_ptr(), nbytes, stream)
     if status:
         _lib.check(status, "pare_paged_attn")
@@ -425,7 +436,7 @@ class PagedKVCache:
         layer = self.layers[layer_idx]
         if layer.head_dim != 128:
             raise ValueError("prefill needs head_dim 128: use attend")
-        q = _rows(q, step.tokens, q.shape[1] if q.dim() == 3 else 0, layer, "q")
+        q = _rows(q, step.tokens, q.shape[1] if q.dim() == 3 else 0, layer, "q")[0]
         if step.lengths is None:
             step.check()
             start, end = step.query_start.tolist(), step.seq_lens.tolist()
