@@ -12,7 +12,7 @@
 // The product: as in w4a16_gemm.cu the rows of a weight tile sit on the MMA's M axis (the TMEM lanes), activation rows on its N axis.
 // Both operands come by TMA (128-byte rows, 128B swizzle) and are multiplied where they land; the accumulator is double-buffered in
 // tensor memory so a tile's epilogue overlaps the next tile's products.
-//   warp 0     TMA of both operands      warp 1  tcgen05.mma      warp 2  tensor memory      warps 4-7  epilogue
+//   warp 0     TMA of both operands      warp 1  tcgen05.mma      warp 2  tensor memory      warps 4-11  epilogue
 // All waits are bounded; when one runs out the thread block stops waiting and loading, lets its copies and products in flight
 // end, and its outputs become NaN.
 #include <algorithm>
@@ -29,7 +29,8 @@ constexpr int kRows = 128;               // weight rows per tile (UMMA M)
 constexpr int kUnitK = 128;              // columns per unit: one 128-byte swizzle row, four MMAs
 constexpr int kWBytes = kRows * kUnitK;
 constexpr int kMaxStages = 12;
-constexpr int kThreads = 256;
+constexpr int kThreads = 384;
+constexpr int kEpiThreads = 256;         // eight warps: two per quarter of the tensor memory's lanes, every other 16 activation rows each
 constexpr uint32_t kTmemCols = 512;      // two accumulators of up to 256 columns
 constexpr int kMaxSmem = 224 * 1024;    // beside 2 KB of static shared memory
 constexpr int kRingBytes = kMaxSmem - 1024 - 512;
@@ -241,8 +242,8 @@ __device__ __forceinline__ void load16(uint32_t taddr, int (&a)[16]) {
 // that set its pace (half the MMAs took the same time: 87 GB/s and SM from L2; 28672 x 4096, 2048 rows 260 us against 167, 2880 Top/s).  The
 // even thread block of a pair issues the MMAs; its `full` barrier counts the bytes of both; commits arrive in both.
 //
-// A cluster is one pair, walking over tiles, or (few tiles, long K) two pairs that split K of one tile: then each of them adds up
-// half of the activation rows, which the other sends to its shared memory.
+// A cluster is one pair, walking over tiles, or (few tiles, long K) two or four pairs that split K of one tile: then each of them adds up
+// its share of the activation rows, which the others send to its shared memory.
 struct PairParams {
   W8Params w;
   int tiles, splits;
@@ -321,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, 1) w8a8_pair_kernel(const __grid_con
     bar_init(mma_done, 1);
     for (int i = 0; i < 2; ++i) {
       bar_init(acc_full + i * 8, 1);
-      bar_init(acc_empty + i * 8, 8);       // the epilogue warps of both thread blocks
+      bar_init(acc_empty + i * 8, 2 * kEpiThreads / 32);       // the epilogue warps of both thread blocks
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -405,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1) w8a8_pair_kernel(const __grid_con
   } else if (warp >= 4 && splits == 1) {
     // ================= epilogue: tensor memory -> registers -> global =================
     pdl_wait();
-    const int q4 = warp & 3, te = threadIdx.x - 4 * 32;
+    const int q4 = warp & 3, c0 = (warp - 4) / 4 * 16, te = threadIdx.x - 4 * 32;
     const uint32_t empty_at = in_block(acc_empty, leader);
     Epilogue<T> epi(p);
     int seg = 0;
@@ -413,16 +414,16 @@ __global__ void __launch_bounds__(kThreads, 1) w8a8_pair_kernel(const __grid_con
       const int m0 = t % p.mtiles * p.mt, mrows = min(p.mt, p.M - m0), buf = seg & 1;
       const uint32_t acc = tmem + buf * 256 + ((uint32_t)(q4 * 32) << 16);
       epi.column(p, t / p.mtiles * 2 * kRows + odd * kRows + q4 * 32 + lane);
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      for (int i = te; i < mrows; i += 128) {
+      asm volatile("bar.sync 1, %0;" ::"n"(kEpiThreads) : "memory");
+      for (int i = te; i < mrows; i += kEpiThreads) {
         s_step[i] = p.step[m0 + i];
         s_sums[i] = p.zero ? p.sums[m0 + i] : 0;
       }
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      asm volatile("bar.sync 1, %0;" ::"n"(kEpiThreads) : "memory");
       bar_wait(acc_full + buf * 8, (seg >> 1) & 1, status, dead);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       epi.bad = __any_sync(0xffffffffu, dead || *const_cast<volatile int*>(&s_failed) != 0);
-      for (int c = 0; c < mrows; c += 16) {
+      for (int c = c0; c < mrows; c += 32) {
         int a[16];
         load16(acc + c, a);
         epi.store16(a, m0 + c, m0 + mrows, s_step + c, s_sums + c);
@@ -435,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1) w8a8_pair_kernel(const __grid_con
 
   if (splits > 1) {
     // ================= one tile: its sums meet in the cluster =================
-    const int q4 = warp & 3, te = threadIdx.x - 4 * 32;
+    const int q4 = warp & 3, c0 = (warp - 4) / 4 * 16, te = threadIdx.x - 4 * 32;
     const int m0 = first % p.mtiles * p.mt, mrows = min(p.mt, p.M - m0), share = p.mt / splits;
     const uint32_t acc = tmem + ((uint32_t)(q4 * 32) << 16), row = (uint32_t)(q4 * 32 + lane);
     if (warp >= 4) {
@@ -450,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1) w8a8_pair_kernel(const __grid_con
       for (int q = 0; q < splits; ++q) {
         if (q == split || q * share >= mrows) continue;
         const uint32_t to = in_block(w_ring + (split < q ? split : split - 1) * slot_bytes, 2 * q + odd);
-        for (int c = 0; c < share; c += 16) {
+        for (int c = c0; c < share; c += 32) {
           int a[16];
           load16(acc + q * share + c, a);
 #pragma unroll
@@ -473,12 +474,12 @@ __global__ void __launch_bounds__(kThreads, 1) w8a8_pair_kernel(const __grid_con
       Epilogue<T> epi(p);
       epi.column(p, first / p.mtiles * 2 * kRows + odd * kRows + (int)row);
       epi.bad = *const_cast<volatile int*>(&s_failed) != 0;
-      for (int i = te; i < to - from; i += 128) {
+      for (int i = te; i < to - from; i += kEpiThreads) {
         s_step[i] = p.step[m0 + from + i];
         s_sums[i] = p.zero ? p.sums[m0 + from + i] : 0;
       }
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      for (int c = 0; c < to - from; c += 16) {
+      asm volatile("bar.sync 1, %0;" ::"n"(kEpiThreads) : "memory");
+      for (int c = c0; c < to - from; c += 32) {
         int a[16];
         load16(acc + from + c, a);
         for (int e = 0; e < splits - 1; ++e) {
@@ -840,19 +841,24 @@ struct W8Plan {
   int64_t units;
 };
 
-// Height of the activation tiles (equal, a multiple of 32) and whether two pairs of SMs split K, by an estimate in microseconds: rounds of
+// Height of the activation tiles (equal, a multiple of 32) and whether two or four pairs of SMs split K, by an estimate in microseconds: rounds of
 // all pairs x units x what a unit of that height takes (0.21 at 32 rows, 0.36 at 256), the weights' way from memory as a lower
-// bound, and what a split adds.  Within a few per cent of the best of 8 heights x 2 splits for 23 shapes of 17 - 3000 rows.
+// bound, and what a split adds.  Within a few per cent of the best of 8 heights x 2 splits for 23 shapes of 17 - 3000 rows; four pairs, where
+// all their clusters fit the device at once (not 16 of them): 17 rows of 512 x 18944 16.3 us against 22.7, of 3584 x 18944 19.1 against 24.1.
 W8Plan w8_plan(int M, int N, int K) {
   W8Plan best{};
   double least = 1e30;
   const int sms = sm_count(), ku = (K + kUnitK - 1) / kUnitK;
   const double stream_us = (double)N * K / 6.0e6;
+  const void* kern = reinterpret_cast<const void*>(w8a8_pair_kernel<__half>);
+  static int cached[64] = {};
+  const int eights = ku >= 8 && ensure_smem_attr(kern, kMaxSmem) ? resident_clusters(kern, 8, kThreads, kMaxSmem, cached) : 0;
   for (int target : {256, 192, 160, 128, 96, 64, 32}) {
-    for (int splits : {1, 2}) {
+    for (int splits : {1, 2, 4}) {
       W8Plan g{};
+      const int step = splits == 4 ? 64 : 32;        // a pair's share of a split tile is a multiple of 16
       g.mtiles = (M + target - 1) / target;
-      g.mt = ((M + g.mtiles - 1) / g.mtiles + 31) / 32 * 32;
+      g.mt = ((M + g.mtiles - 1) / g.mtiles + step - 1) / step * step;
       g.mtiles = (M + g.mt - 1) / g.mt;
       g.ku = ku;
       g.splits = splits;
@@ -860,10 +866,10 @@ W8Plan w8_plan(int M, int N, int K) {
       if (g.mt > 256 || splits > ku || g.units * ku >= (int64_t)1 << 31) continue;
       g.tiles = (int)g.units;
       g.units *= ku;
-      const int clusters = sms / (2 * splits), rounds = (g.tiles + clusters - 1) / clusters;
-      if (splits > 1 && rounds > 1) continue;
+      const int clusters = splits == 4 ? eights : sms / (2 * splits), rounds = splits > 1 ? 1 : (g.tiles + clusters - 1) / clusters;
+      if (splits > 1 && g.tiles > clusters) continue;
       const double cost = std::max((double)rounds * ((ku + splits - 1) / splits) * (0.2 + 0.00055 * g.mt), stream_us) + 0.01 * g.mt +
-                          (splits > 1 ? 2.0 + 0.015 * g.mt : 0.0);
+                          (splits == 4 ? 2.4 + 0.02 * g.mt : splits == 2 ? 2.0 + 0.015 * g.mt : 0.0);
       if (cost < least - 1e-9) {
         least = cost;
         best = g;
@@ -935,8 +941,8 @@ int pare_w8a8_forward(const void* x, int x_dtype, int64_t ldx, const int8_t* wei
   CUtensorMap tw, tx;
   PARE_REQUIRE(map(&tw, weight, N, ldw, kRows), PARE_ERR_CUDA);
   // with programmatic launch, and in clusters
-  auto launch = [&](auto kern, int blocks, int threads, size_t smem, int cluster, auto... args) -> int {
-    if (!ensure_smem_attr(reinterpret_cast<const void*>(kern), threads == kFewThreads ? kFewSmem : kMaxSmem)) return PARE_ERR_CUDA;
+  auto launch = [&](auto kern, int blocks, int threads, int most_smem, size_t smem, int cluster, auto... args) -> int {
+    if (!ensure_smem_attr(reinterpret_cast<const void*>(kern), most_smem)) return PARE_ERR_CUDA;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(blocks);
     cfg.blockDim = dim3(threads);
@@ -965,8 +971,8 @@ int pare_w8a8_forward(const void* x, int x_dtype, int64_t ldx, const int8_t* wei
   const FewParams fp{p, x, ldx, input_scale, K, f.tiles, f.splits, f.stages};
   const size_t few_smem = 1024 + (size_t)f.stages * kWBytes + (size_t)f.units * kFewUnitBytes;
   if (f.splits && !f.coded)
-    return half ? launch(w8a8_few_kernel<__half, false>, f.blocks, kFewThreads, few_smem, f.splits, tw, tw, fp)
-                : launch(w8a8_few_kernel<__nv_bfloat16, false>, f.blocks, kFewThreads, few_smem, f.splits, tw, tw, fp);
+    return half ? launch(w8a8_few_kernel<__half, false>, f.blocks, kFewThreads, kFewSmem, few_smem, f.splits, tw, tw, fp)
+                : launch(w8a8_few_kernel<__nv_bfloat16, false>, f.blocks, kFewThreads, kFewSmem, few_smem, f.splits, tw, tw, fp);
 
   unsigned char* ws = reinterpret_cast<unsigned char*>(workspace);
   PARE_REQUIRE(map(&tx, ws + sp.codes, M, sp.ldc, f.splits ? kFewRows : g.mt / 2), PARE_ERR_CUDA);
@@ -996,16 +1002,16 @@ int pare_w8a8_forward(const void* x, int x_dtype, int64_t ldx, const int8_t* wei
   if (f.splits) {
     FewParams cp = fp;
     cp.w = p;
-    return half ? launch(w8a8_few_kernel<__half, true>, f.blocks, kFewThreads, few_smem, f.splits, tw, tx, cp)
-                : launch(w8a8_few_kernel<__nv_bfloat16, true>, f.blocks, kFewThreads, few_smem, f.splits, tw, tx, cp);
+    return half ? launch(w8a8_few_kernel<__half, true>, f.blocks, kFewThreads, kFewSmem, few_smem, f.splits, tw, tx, cp)
+                : launch(w8a8_few_kernel<__nv_bfloat16, true>, f.blocks, kFewThreads, kFewSmem, few_smem, f.splits, tw, tx, cp);
   }
   p.mt = g.mt;
   p.mtiles = g.mtiles;
   p.stages = g.stages;
   const size_t smem = 1024 + (size_t)g.stages * (kWBytes + g.mt / 2 * kUnitK) + 512;
   const PairParams pp{p, g.tiles, g.splits};
-  return half ? launch(w8a8_pair_kernel<__half>, g.blocks, kThreads, smem, 2 * g.splits, tw, tx, pp)
-              : launch(w8a8_pair_kernel<__nv_bfloat16>, g.blocks, kThreads, smem, 2 * g.splits, tw, tx, pp);
+  return half ? launch(w8a8_pair_kernel<__half>, g.blocks, kThreads, kMaxSmem, smem, 2 * g.splits, tw, tx, pp)
+              : launch(w8a8_pair_kernel<__nv_bfloat16>, g.blocks, kThreads, kMaxSmem, smem, 2 * g.splits, tw, tx, pp);
 }
 
 }  // extern "C"

@@ -56,7 +56,8 @@ def _data(m, n, k, seed, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 128, 16), (2, 129, 100), (15, 257, 130), (16, 512, 4096), (17, 300, 1000), (63, 128, 128),
-                                   (129, 1000, 2064), (255, 130, 384), (257, 384, 1111), (333, 3584, 2368), (600, 640, 5000)])
+                                   (129, 1000, 2064), (255, 130, 384), (257, 384, 1111), (333, 3584, 2368), (600, 640, 5000),
+                                   (20, 300, 8200), (65, 1500, 16384), (250, 200, 8192), (513, 300, 9000)])
 def test_sizes(m, n, k, dtype, cuda_lib):
     x, w, scale, g = _data(m, n, k, m + n + k, dtype)
     _check(w8a8_forward(x, w, scale), x, w, scale)
@@ -66,7 +67,7 @@ def test_sizes(m, n, k, dtype, cuda_lib):
     _check(w8a8_forward(x, w, scale, zero, bias=bias, input_scale=ins), x, w, scale, zero, bias, ins)
 
 
-@pytest.mark.parametrize("m", [1, 16, 40])
+@pytest.mark.parametrize("m", [1, 16, 40, 130])
 def test_long_rows_and_split_sums(m, cuda_lib):
     """One or two weight tiles over a long K: every thread block has a part of the same tile."""
     x, w, scale, _ = _data(m, 200, 18944, m, torch.bfloat16)
