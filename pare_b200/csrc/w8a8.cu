@@ -57,39 +57,38 @@ __device__ __forceinline__ uint32_t magnitude(T v) {   // orders like |v|, infin
   return *reinterpret_cast<const uint16_t*>(&v) & 0x7fffu;
 }
 
-// VECS > 0: rows of at most VECS * THREADS vectors of eight stay in registers between the maximum and the codes (and are divided by
-// input_scale once); 0: rows of any length and alignment, read twice.
-template <typename T, int THREADS, int VECS>
-__global__ void __launch_bounds__(THREADS) w8a8_quantize_kernel(const QuantParams p) {
-  pdl_launch_dependents();
+// A row per thread block; where rows allow 16-byte pieces (VEC) it waits in shared memory between the maximum and the codes (and is divided
+// by input_scale once), all of it on its way at the same time and no registers held, so that as many rows as possible are resident.
+// Others are read twice.
+template <typename T, int THREADS, bool VEC>
+__global__ void __launch_bounds__(THREADS, 2048 / THREADS) w8a8_quantize_kernel(const QuantParams p) {
+  pdl_wait();
+  pdl_launch_dependents();      // only now: the product reads weights before it waits
   constexpr int kW = THREADS / 32;
+  extern __shared__ uint4 s_row[];
   __shared__ uint32_t s_top[kW];
   __shared__ int s_sum[kW];
-  const int m = blockIdx.x, tid = threadIdx.x;
+  const int m = blockIdx.x, tid = threadIdx.x, n8 = p.K / 8;
   const T* row = reinterpret_cast<const T*>(p.x) + m * p.ldx;
   int8_t* out = p.codes + m * p.ldc;
   uint32_t top = 0;
-  uint4 x[VECS > 0 ? VECS : 1];
-  if constexpr (VECS > 0) {
-#pragma unroll
-    for (int i = 0; i < VECS; ++i) {
-      const int k = (i * THREADS + tid) * 8;
-      x[i] = k < p.K ? *reinterpret_cast<const uint4*>(row + k) : make_uint4(0, 0, 0, 0);
-    }
-    if (p.input_scale) {
-#pragma unroll
-      for (int i = 0; i < VECS; ++i) {
-        const int k = (i * THREADS + tid) * 8;
-        if (k >= p.K) break;
-        const float4 a = __ldg(reinterpret_cast<const float4*>(p.input_scale + k)), b = __ldg(reinterpret_cast<const float4*>(p.input_scale + k + 4));
+  if constexpr (VEC) {
+    const uint32_t at = s_u32(s_row);
+    for (int i = tid; i < n8; i += THREADS)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + i * 16), "l"(row + i * 8) : "memory");
+    asm volatile("cp.async.wait_all;" ::: "memory");       // a thread reads what it loaded itself
+    for (int i = tid; i < n8; i += THREADS) {
+      uint4 x = s_row[i];
+      if (p.input_scale) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(p.input_scale) + 2 * i), b = __ldg(reinterpret_cast<const float4*>(p.input_scale) + 2 * i + 1);
         const float d[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-        T* v = reinterpret_cast<T*>(&x[i]);
+        T* v = reinterpret_cast<T*>(&x);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = from_float<T>(__fdiv_rn(to_float<T>(v[j]), d[j]));
+        s_row[i] = x;
       }
+      top = __vmaxu2(top, q8::magnitudes(x));
     }
-#pragma unroll
-    for (int i = 0; i < VECS; ++i) top = __vmaxu2(top, q8::magnitudes(x[i]));
     top = max(top & 0xffffu, top >> 16);
   } else {
     for (int k = tid; k < p.K; k += THREADS) top = max(top, magnitude(smoothed<T>(row[k], p.input_scale, k)));
@@ -104,14 +103,12 @@ __global__ void __launch_bounds__(THREADS) w8a8_quantize_kernel(const QuantParam
   // a row with an infinity or NaN has a step that is not finite, so its outputs are NaN
   const q8::Grid grid(amax < 1e-6f ? 1e-6f : amax);
   int sum = 0;
-  if constexpr (VECS > 0) {
-#pragma unroll
-    for (int i = 0; i < VECS; ++i) {
-      const int k = (i * THREADS + tid) * 8;
-      if (k >= p.K) break;
-      const uint2 o = grid.codes<T>(x[i]);
-      if (p.sums) sum = __dp4a((int)o.y, 0x01010101, __dp4a((int)o.x, 0x01010101, sum));
-      *reinterpret_cast<uint2*>(out + k) = o;
+  if constexpr (VEC) {
+#pragma unroll 1
+    for (int i = tid; i < n8; i += THREADS) {
+      const uint2 o = grid.codes<T>(s_row[i]);
+      sum = __dp4a((int)o.y, 0x01010101, __dp4a((int)o.x, 0x01010101, sum));
+      *reinterpret_cast<uint2*>(out + i * 8) = o;
     }
   } else {
     for (int k = tid; k < p.K; k += THREADS) {
@@ -980,22 +977,23 @@ int pare_w8a8_forward(const void* x, int x_dtype, int64_t ldx, const int8_t* wei
   const QuantParams q{x, ldx, input_scale, reinterpret_cast<int8_t*>(ws + sp.codes), sp.ldc, reinterpret_cast<float*>(ws + sp.step),
                       zero ? reinterpret_cast<int*>(ws + sp.sums) : nullptr, K};
   const bool vec = aligned16(x) && (M == 1 || ldx % 8 == 0) && K % 8 == 0 && (!input_scale || aligned16(input_scale));
-  // Many rows: few threads with several vectors in flight each, so that all rows are resident at once; few rows: many threads.
-  auto quantize = [&](auto tag) {
+  // As many threads per row as still leave all rows resident at once.
+  auto quantize = [&](auto tag) -> int {
     using E = decltype(tag);
-    auto go = [&](auto kern, int threads) { kern<<<M, threads, 0, st>>>(q); };
-    const bool many = M > 2 * sm_count();
-    if (!vec || K > 32768) go(w8a8_quantize_kernel<E, 512, 0>, 512);
-    else if (many && K <= 4096) go(w8a8_quantize_kernel<E, 128, 4>, 128);
-    else if (K <= 4096) go(w8a8_quantize_kernel<E, 512, 1>, 512);
-    else if (many && K <= 8192) go(w8a8_quantize_kernel<E, 256, 4>, 256);
-    else if (K <= 16384) go(w8a8_quantize_kernel<E, 512, 4>, 512);
-    else if (K <= 20480) go(w8a8_quantize_kernel<E, 512, 5>, 512);
-    else go(w8a8_quantize_kernel<E, 512, 8>, 512);
+    auto go = [&](auto kern, int threads) -> int {
+      const size_t row = vec ? (size_t)K * 2 : 0;
+      if (row > 48 * 1024 && !ensure_smem_attr(reinterpret_cast<const void*>(kern), kMaxK * 2)) return PARE_ERR_CUDA;
+      return launch_pdl(kern, dim3(M), dim3(threads), row, st, q);
+    };
+    if (!vec) return go(w8a8_quantize_kernel<E, 512, false>, 512);
+    const int per_sm = (M + sm_count() - 1) / sm_count();
+    if (per_sm <= 2 && K > 8192) return go(w8a8_quantize_kernel<E, 1024, true>, 1024);
+    if (per_sm <= 4) return go(w8a8_quantize_kernel<E, 512, true>, 512);
+    if (per_sm <= 8) return go(w8a8_quantize_kernel<E, 256, true>, 256);
+    return go(w8a8_quantize_kernel<E, 128, true>, 128);
   };
-  if (x_dtype == PARE_F16) quantize(__half());
-  else quantize(__nv_bfloat16());
-  if (cudaGetLastError() != cudaSuccess) return PARE_ERR_CUDA;
+  const int rc = half ? quantize(__half()) : quantize(__nv_bfloat16());
+  if (rc != PARE_OK) return rc;
 
   p.step = q.step;
   p.sums = q.sums;
