@@ -16,6 +16,7 @@
 // All waits are bounded; when one runs out the thread block stops waiting and loading, lets its copies and products in flight
 // end, and its outputs become NaN.
 #include <algorithm>
+#include <type_traits>
 
 #include "quant8.cuh"
 #include "tcgen05.cuh"
@@ -58,10 +59,11 @@ __device__ __forceinline__ uint32_t magnitude(T v) {   // orders like |v|, infin
 }
 
 // A row per thread block; where rows allow 16-byte pieces (VEC) it waits in shared memory between the maximum and the codes (and is divided
-// by input_scale once), all of it on its way at the same time and no registers held, so that as many rows as possible are resident.
-// Others are read twice.
-template <typename T, int THREADS, bool VEC>
-__global__ void __launch_bounds__(THREADS, 2048 / THREADS) w8a8_quantize_kernel(const QuantParams p) {
+// by input_scale once: SCALED), all of it on its way at the same time and no registers held, so that as many rows as possible are
+// resident.  Others are read twice.  Bound: the codes' arithmetic.  2048 rows of 4096 6.8 us (bytes: 3.8), 1024 of 14336 9.1 (6.7), 333 of 18944
+// 5.9 and with input_scale 10.4 (2.9; rows held in registers, fewer of them at once: 12 and 18).
+template <typename T, int THREADS, bool VEC, bool SCALED>
+__global__ void __launch_bounds__(THREADS, (SCALED ? 1536 : 2048) / THREADS) w8a8_quantize_kernel(const QuantParams p) {
   pdl_wait();
   pdl_launch_dependents();      // only now: the product reads weights before it waits
   constexpr int kW = THREADS / 32;
@@ -76,18 +78,25 @@ __global__ void __launch_bounds__(THREADS, 2048 / THREADS) w8a8_quantize_kernel(
     const uint32_t at = s_u32(s_row);
     for (int i = tid; i < n8; i += THREADS)
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + i * 16), "l"(row + i * 8) : "memory");
-    asm volatile("cp.async.wait_all;" ::: "memory");       // a thread reads what it loaded itself
-    for (int i = tid; i < n8; i += THREADS) {
-      uint4 x = s_row[i];
-      if (p.input_scale) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(p.input_scale) + 2 * i), b = __ldg(reinterpret_cast<const float4*>(p.input_scale) + 2 * i + 1);
-        const float d[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    if constexpr (SCALED) {
+      const float4* d = reinterpret_cast<const float4*>(p.input_scale);
+      float4 a, b, a2, b2;      // of this vector and of the next
+      if (tid < n8) a = __ldg(d + 2 * tid), b = __ldg(d + 2 * tid + 1);
+      asm volatile("cp.async.wait_all;" ::: "memory");       // a thread reads what it loaded itself
+#pragma unroll 1
+      for (int i = tid; i < n8; i += THREADS, a = a2, b = b2) {
+        if (i + THREADS < n8) a2 = __ldg(d + 2 * (i + THREADS)), b2 = __ldg(d + 2 * (i + THREADS) + 1);
+        uint4 x = s_row[i];
+        const float by[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
         T* v = reinterpret_cast<T*>(&x);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = from_float<T>(__fdiv_rn(to_float<T>(v[j]), d[j]));
+        for (int j = 0; j < 8; ++j) v[j] = from_float<T>(__fdiv_rn(to_float<T>(v[j]), by[j]));
         s_row[i] = x;
+        top = __vmaxu2(top, q8::magnitudes(x));
       }
-      top = __vmaxu2(top, q8::magnitudes(x));
+    } else {
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      for (int i = tid; i < n8; i += THREADS) top = __vmaxu2(top, q8::magnitudes(s_row[i]));
     }
     top = max(top & 0xffffu, top >> 16);
   } else {
@@ -236,7 +245,7 @@ __device__ __forceinline__ void load16(uint32_t taddr, int (&a)[16]) {
 // ---- product, two SMs on a tile -------------------------------------------------------------------------------------------------------
 // cta_group::2: two SMs on a tile of 256 weight rows x mt activation rows.  Each loads its own 128 weight rows and half of the
 // activation rows, the MMA reads both halves: 32 KB per SM and unit at mt = 256, where one SM alone with a 128 x 256 tile needs 48 KB, and
-// that set its pace (half the MMAs took the same time: 87 GB/s and SM from L2; 28672 x 4096, 2048 rows 260 us against 167, 2880 Top/s).  The
+// that set its pace (half the MMAs took the same time: 87 GB/s and SM from L2; 28672 x 4096, 2048 rows 260 us against 164, 2940 Top/s).  The
 // even thread block of a pair issues the MMAs; its `full` barrier counts the bytes of both; commits arrive in both.
 //
 // A cluster is one pair, walking over tiles, or (few tiles, long K) two or four pairs that split K of one tile: then each of them adds up
@@ -799,9 +808,9 @@ int resident_clusters(const void* kern, int size, int threads, int smem, int (&c
 }
 
 // Up to 16 rows, if a thread block's codes fit beside a ring of weights.  The tokens are quantized on the way where a thread has at most
-// eight vectors of eight columns to look at (4 rows of 4096): one launch, 1 / 2 / 4 rows of 4096 x 4096 8.0 / 8.3 / 9.6 us, 28672 x 4096 21.9 /
-// 22.4 / 24.4; in a launch of their own 8.8 / 8.8 / 8.8 and 23.6 / 23.9 / 24.3, and the same up to 16 rows (8 rows on the way: 11.7).
-// K is shared by as many thread blocks (4, 2) as keep every SM to one tile.
+// eight vectors of eight columns to look at (4 rows of 4096): one launch, 1 / 2 / 4 rows of 4096 x 4096 7.4 / 7.5 / 8.1 us, 28672 x 4096 20.7 /
+// 20.6 / 21.9 (0.86 of the copy rate); more rows in a launch of their own, 8 / 16 rows 8.4 / 8.4 and 23.0 / 23.4 (on the way 8 rows of 4096 x 4096
+// cost 2.9 us more).  K is shared by as many thread blocks (4, 2) as keep every SM to one tile.
 struct FewPlan {
   int splits, tiles, blocks, stages, units;      // splits 0: not this kernel
   bool coded;                                    // tokens are quantized by a launch of their own
@@ -978,21 +987,25 @@ int pare_w8a8_forward(const void* x, int x_dtype, int64_t ldx, const int8_t* wei
                       zero ? reinterpret_cast<int*>(ws + sp.sums) : nullptr, K};
   const bool vec = aligned16(x) && (M == 1 || ldx % 8 == 0) && K % 8 == 0 && (!input_scale || aligned16(input_scale));
   // As many threads per row as still leave all rows resident at once.
-  auto quantize = [&](auto tag) -> int {
+  auto quantize = [&](auto tag, auto scaled) -> int {
     using E = decltype(tag);
+    constexpr bool kS = decltype(scaled)::value;
     auto go = [&](auto kern, int threads) -> int {
       const size_t row = vec ? (size_t)K * 2 : 0;
       if (row > 48 * 1024 && !ensure_smem_attr(reinterpret_cast<const void*>(kern), kMaxK * 2)) return PARE_ERR_CUDA;
       return launch_pdl(kern, dim3(M), dim3(threads), row, st, q);
     };
-    if (!vec) return go(w8a8_quantize_kernel<E, 512, false>, 512);
+    if (!vec) return go(w8a8_quantize_kernel<E, 512, false, kS>, 512);
     const int per_sm = (M + sm_count() - 1) / sm_count();
-    if (per_sm <= 2 && K > 8192) return go(w8a8_quantize_kernel<E, 1024, true>, 1024);
-    if (per_sm <= 4) return go(w8a8_quantize_kernel<E, 512, true>, 512);
-    if (per_sm <= 8) return go(w8a8_quantize_kernel<E, 256, true>, 256);
-    return go(w8a8_quantize_kernel<E, 128, true>, 128);
+    if (per_sm <= 2 && K > 8192) return go(w8a8_quantize_kernel<E, 1024, true, kS>, 1024);
+    if (per_sm <= 2) return go(w8a8_quantize_kernel<E, 512, true, kS>, 512);
+    if (per_sm <= 8) return go(w8a8_quantize_kernel<E, 256, true, kS>, 256);
+    return go(w8a8_quantize_kernel<E, 128, true, kS>, 128);
   };
-  const int rc = half ? quantize(__half()) : quantize(__nv_bfloat16());
+  const std::true_type yes;
+  const std::false_type no;
+  const int rc = half ? (input_scale ? quantize(__half(), yes) : quantize(__half(), no))
+                      : (input_scale ? quantize(__nv_bfloat16(), yes) : quantize(__nv_bfloat16(), no));
   if (rc != PARE_OK) return rc;
 
   p.step = q.step;

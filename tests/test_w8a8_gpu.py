@@ -93,6 +93,25 @@ def test_zero_points_of_any_value(cuda_lib):
     _check(w8a8_forward(x, w, scale, zero), x, w, scale, zero)
 
 
+@pytest.mark.parametrize("m", [3, 40, 700])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_smoothing_divides_exactly(dtype, m, cuda_lib):
+    """Every code by itself (the weights are 127 times the identity): scales of any size, powers of two and their neighbours, signs."""
+    k, span = 512, 6 if dtype is torch.float16 else 100
+    g = torch.Generator(device=DEV).manual_seed(m)
+    e = torch.randint(-span, span + 1, (k,), device=DEV, generator=g).double()
+    u = 0.5 + torch.rand(k, device=DEV, generator=g).double()
+    u[::7], u[1::7], u[2::7], u[3::7] = 1.0, 1.0 + 2.0 ** -23, 1.0 - 2.0 ** -24, -1.5
+    ins = (u * 2.0 ** e).float()
+    x = (torch.randn(m, k, device=DEV, generator=g).double().clamp(-3, 3) * 2.0 ** e).to(dtype)
+    x[0, ::5], x[1, 7] = 0.0, float("inf")
+    w = 127 * torch.eye(k, dtype=torch.int8, device=DEV)
+    got = w8a8_forward(x, w, torch.ones(k, device=DEV), input_scale=ins)
+    assert got[1].isnan().all()
+    keep = [i for i in range(m) if i != 1]
+    _check(got[keep], x[keep], w, torch.ones(k, device=DEV), None, None, ins)
+
+
 def test_ties_tiny_and_non_finite_rows(cuda_lib):
     for dtype in (torch.float16, torch.bfloat16):
         x, w, scale, g = _data(8, 128, 256, 2, dtype)
