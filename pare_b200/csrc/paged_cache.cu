@@ -22,8 +22,9 @@ using namespace paged;
 // One prefix sum over the requests gives everything: first row of a request's new tokens, blocks taken from the free stack before
 // it, touched blocks before it.  A thread block holds the sums of all requests in shared memory (every thread block computes them
 // for itself: no order between thread blocks), then tokens, fresh blocks and touched blocks are spread over all threads, each
-// finding its request by bisection.  Bound by latency (two dependent reads and a scan): one request 3.8 us, 64 requests with a token each
-// 5.3, prompts of thousands of tokens 6.3; bytes would take 0.2.
+// finding its request by bisection; one thread block does nothing but count attention's units.  Bound by latency (two dependent reads and
+// a scan or two): one request 3.3 us, 64 requests with a token each 4.1, 256 prompts of 64000 tokens 5.5, 2056 tokens in chunks 7.6;
+// bytes would take 0.2.
 constexpr int kPlanThreads = 512;
 constexpr int kPlanWarps = kPlanThreads / 32;
 
@@ -157,7 +158,9 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
   }
   __syncthreads();
 
-  const int g = blockIdx.x * kPlanThreads + threadIdx.x, stride = gridDim.x * kPlanThreads;
+  // the last thread block counts units of attention, the others share what else there is
+  const bool counts = p.units && blockIdx.x == gridDim.x - 1;
+  const int g = counts ? INT_MAX : blockIdx.x * kPlanThreads + threadIdx.x, stride = (gridDim.x - (p.units ? 1 : 0)) * kPlanThreads;
   // block `blk` of request r, taken in this step or before
   auto block_id = [&](int r, int blk) {
     const int have = (s_len[r] + bs - 1) >> p.bs_log2;
@@ -197,37 +200,42 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
     const int r = last_at_most(s_take, R, i);
     p.table[r * p.ld_table + ((s_len[r] + bs - 1) >> p.bs_log2) + i - s_take[r]] = p.free_blocks[count - 1 - i];
   }
-  if (lead && p.units) {
+  if (counts) {
     // Units of attention work before each token: quantized tokens, then open rows, in pieces of kUnit.  Where 2^i tokens of a request
     // share a tile, its last token has its units and the others have none.
     const int each = (p.T + kPlanThreads - 1) / kPlanThreads;
     const int t0 = min(p.T, (int)threadIdx.x * each), t1 = min(p.T, t0 + each);
+    constexpr int kEach = kMaxQueryTokens / kPlanThreads;
+    int units[kEach], pack[kEach];      // of tokens t0 ..; bit i of pack: the last one of a tile of 2^i
+    int r = t0 < t_new ? last_at_most(s_start, R, t0) : 0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int t = t0 + e;
+      units[e] = pack[e] = 0;
+      if (t >= t1 || t >= t_new) continue;
+      while (r + 1 < R && s_start[r + 1] <= t) ++r;
+      const int mine = t - s_start[r], seen = s_len[r] + mine + 1, end = s_len[r] + (r + 1 < R ? s_start[r + 1] : (int)t_new) - s_start[r];
+      const int held = end >> p.bs_log2 << p.bs_log2, nq = min(seen, held);
+      units[e] = (nq + kUnit - 1) / kUnit + (seen - nq + kUnit - 1) / kUnit;
+#pragma unroll
+      for (int i = 0; i < kPacks; ++i) pack[e] |= seen == end || (mine + 1) % (1 << i) == 0 ? 1 << i : 0;
+    }
     auto tables = [&](auto packs) {
       constexpr int kN = decltype(packs)::value;
-      auto units_of = [&](int t, int (&n)[kN]) {
+      int sums[kN] = {}, first[kN], all[kN];
 #pragma unroll
-        for (int i = 0; i < kN; ++i) n[i] = 0;
-        if (t >= t_new) return;
-        const int r = last_at_most(s_start, R, t), mine = t - s_start[r], seen = s_len[r] + mine + 1;
-        const int end = s_len[r] + (r + 1 < R ? s_start[r + 1] : (int)t_new) - s_start[r];
-        const int held = end >> p.bs_log2 << p.bs_log2, nq = min(seen, held);
-        const int units = (nq + kUnit - 1) / kUnit + (seen - nq + kUnit - 1) / kUnit;
+      for (int e = 0; e < kEach; ++e) {
 #pragma unroll
-        for (int i = 0; i < kN; ++i) n[i] = seen == end || (mine + 1) % (1 << i) == 0 ? units : 0;
-      };
-      int sums[kN] = {}, first[kN], all[kN], n[kN];
-      for (int t = t0; t < t1; ++t) {
-        units_of(t, n);
-#pragma unroll
-        for (int i = 0; i < kN; ++i) sums[i] += n[i];
+        for (int i = 0; i < kN; ++i) sums[i] += pack[e] >> i & 1 ? units[e] : 0;
       }
       block_scan(sums, first, all, s_sums);
-      for (int t = t0; t < t1; ++t) {
-        units_of(t, n);
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        if (t0 + e >= t1) break;
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
-          p.step[p.o_units + i * p.unit_stride + t] = first[i];
-          first[i] += n[i];
+          p.step[p.o_units + i * p.unit_stride + t0 + e] = first[i];
+          first[i] += pack[e] >> i & 1 ? units[e] : 0;
         }
       }
       if (threadIdx.x == 0) {
@@ -499,7 +507,7 @@ int pare_paged_plan(const int32_t* seq_lens, const int32_t* new_lens, int R, int
   if (!ensure_smem_attr(reinterpret_cast<const void*>(paged_plan_kernel), kMaxRequests * 4 * (int)sizeof(int))) return PARE_ERR_CUDA;
   int blocks = (T + kPlanThreads - 1) / kPlanThreads;
   blocks = blocks < 1 ? 1 : blocks > sm_count() ? sm_count() : blocks;
-  const int rc = launch_pdl(paged_plan_kernel, dim3(blocks), dim3(kPlanThreads), smem, reinterpret_cast<cudaStream_t>(stream), p);
+  const int rc = launch_pdl(paged_plan_kernel, dim3(blocks + (s.units ? 1 : 0)), dim3(kPlanThreads), smem, reinterpret_cast<cudaStream_t>(stream), p);
   return rc != PARE_OK ? rc : launch_status();
 }
 
