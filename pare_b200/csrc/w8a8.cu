@@ -33,7 +33,7 @@ constexpr int kMaxStages = 12;
 constexpr int kThreads = 384;
 constexpr int kEpiThreads = 256;         // eight warps: two per quarter of the tensor memory's lanes, every other 16 activation rows each
 constexpr uint32_t kTmemCols = 512;      // two accumulators of up to 256 columns
-constexpr int kMaxSmem = 224 * 1024;    // beside 2 KB of static shared memory
+constexpr int kMaxSmem = 222 * 1024;    // beside 4.1 KB of static shared memory
 constexpr int kRingBytes = kMaxSmem - 1024 - 512;
 constexpr int kMaxK = 65536;             // 65536 * 127 * (128 + 128) < 2^31
 
@@ -199,11 +199,18 @@ struct Epilogue {
         pair_out((reinterpret_cast<uintptr_t>(p.y) & 3u) == 0 && (p.ldy & 1) == 0 && (p.N & 1) == 0), bad(false) {}
   // The zero-point's whole part is taken off in integers, exactly; what is left (0 for the zero-points of quantizers, or a value
   // beyond any code) in fp32.
-  __device__ __forceinline__ void column(const W8Params& p, int col) {
+  __device__ __forceinline__ void column(const W8Params& p, int col) { column(col, fetch(p, col)); }
+  // its scale, zero-point and bias
+  __device__ __forceinline__ float3 fetch(const W8Params& p, int col) const {
+    const bool there = col < N;
+    return make_float3(there ? p.scale[col] : 0.f, p.zero && there ? p.zero[col] : 0.f,
+                       p.bias && there ? to_float<T>(reinterpret_cast<const T*>(p.bias)[col]) : 0.f);
+  }
+  __device__ __forceinline__ void column(int col, const float3& of) {
     n = col;
-    bias = (p.bias && n < N) ? to_float<T>(reinterpret_cast<const T*>(p.bias)[n]) : 0.f;
-    scale = n < N ? p.scale[n] : 0.f;
-    const float z = (p.zero && n < N) ? p.zero[n] : 0.f;
+    scale = of.x;
+    bias = of.z;
+    const float z = of.y;
     zi = fabsf(z) <= 128.f ? __float2int_rn(z) : 0;
     zf = z - (float)zi;
   }
@@ -300,8 +307,8 @@ __global__ void __launch_bounds__(kThreads, 1) w8a8_pair_kernel(const __grid_con
                                                                 const PairParams pp) {
   extern __shared__ unsigned char smem_raw[];
   __shared__ int s_failed;
-  __shared__ float s_step[256];
-  __shared__ int s_sums[256];
+  __shared__ float s_step[2][256];
+  __shared__ int s_sums[2][256];
   const W8Params& p = pp.w;
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int ku = p.ku, stages = p.stages;
@@ -415,24 +422,38 @@ __global__ void __launch_bounds__(kThreads, 1) w8a8_pair_kernel(const __grid_con
     const int q4 = warp & 3, c0 = (warp - 4) / 4 * 16, te = threadIdx.x - 4 * 32;
     const uint32_t empty_at = in_block(acc_empty, leader);
     Epilogue<T> epi(p);
+    // A tile's scales and steps are read while the tile before it is stored (2048 rows of 28672 x 256 @@).
+    static_assert(kEpiThreads >= 256, "a thread per activation row of a tile");
+    float3 of, of_next;
+    float mine = 0.f;
+    int mine_sum = 0;
+    auto column_of = [&](int t) { return t / p.mtiles * 2 * kRows + (int)(odd * kRows) + q4 * 32 + lane; };
+    auto ahead = [&](int t) {
+      const int m = t % p.mtiles * p.mt + te;
+      of_next = epi.fetch(p, column_of(t));
+      if (te < p.mt && m < p.M) {
+        mine = p.step[m];
+        mine_sum = p.zero ? p.sums[m] : 0;
+      }
+    };
+    if (first < pp.tiles) ahead(first);
     int seg = 0;
     for (int t = first; t < pp.tiles; t += step, ++seg) {
       const int m0 = t % p.mtiles * p.mt, mrows = min(p.mt, p.M - m0), buf = seg & 1;
       const uint32_t acc = tmem + buf * 256 + ((uint32_t)(q4 * 32) << 16);
-      epi.column(p, t / p.mtiles * 2 * kRows + odd * kRows + q4 * 32 + lane);
+      of = of_next;
+      epi.column(column_of(t), of);
+      s_step[buf][te] = mine;
+      s_sums[buf][te] = mine_sum;
       asm volatile("bar.sync 1, %0;" ::"n"(kEpiThreads) : "memory");
-      for (int i = te; i < mrows; i += kEpiThreads) {
-        s_step[i] = p.step[m0 + i];
-        s_sums[i] = p.zero ? p.sums[m0 + i] : 0;
-      }
-      asm volatile("bar.sync 1, %0;" ::"n"(kEpiThreads) : "memory");
+      if (t + step < pp.tiles) ahead(t + step);
       bar_wait(acc_full + buf * 8, (seg >> 1) & 1, status, dead);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       epi.bad = __any_sync(0xffffffffu, dead || *const_cast<volatile int*>(&s_failed) != 0);
       for (int c = c0; c < mrows; c += 32) {
         int a[16];
         load16(acc + c, a);
-        epi.store16(a, m0 + c, m0 + mrows, s_step + c, s_sums + c);
+        epi.store16(a, m0 + c, m0 + mrows, s_step[buf] + c, s_sums[buf] + c);
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
@@ -481,8 +502,8 @@ __global__ void __launch_bounds__(kThreads, 1) w8a8_pair_kernel(const __grid_con
       epi.column(p, first / p.mtiles * 2 * kRows + odd * kRows + (int)row);
       epi.bad = *const_cast<volatile int*>(&s_failed) != 0;
       for (int i = te; i < to - from; i += kEpiThreads) {
-        s_step[i] = p.step[m0 + from + i];
-        s_sums[i] = p.zero ? p.sums[m0 + from + i] : 0;
+        s_step[0][i] = p.step[m0 + from + i];
+        s_sums[0][i] = p.zero ? p.sums[m0 + from + i] : 0;
       }
       asm volatile("bar.sync 1, %0;" ::"n"(kEpiThreads) : "memory");
       for (int c = c0; c < to - from; c += 32) {
@@ -498,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, 1) w8a8_pair_kernel(const __grid_con
             a[4 * i + 3] += (int)v.w;
           }
         }
-        epi.store16(a, m0 + from + c, m0 + to, s_step + c, s_sums + c);
+        epi.store16(a, m0 + from + c, m0 + to, s_step[0] + c, s_sums[0] + c);
       }
     }
   }
