@@ -33,7 +33,7 @@ constexpr int kMaxStages = 12;
 constexpr int kThreads = 384;
 constexpr int kEpiThreads = 256;         // eight warps: two per quarter of the tensor memory's lanes, every other 16 activation rows each
 constexpr uint32_t kTmemCols = 512;      // two accumulators of up to 256 columns
-constexpr int kMaxSmem = 222 * 1024;    // beside 4.1 KB of static shared memory
+constexpr int kMaxSmem = 214 * 1024;    // beside 12.1 KB of static shared memory
 constexpr int kRingBytes = kMaxSmem - 1024 - 512;
 constexpr int kMaxK = 65536;             // 65536 * 127 * (128 + 128) < 2^31
 
@@ -191,12 +191,13 @@ struct Epilogue {
   int64_t ldy;
   int M, N, n, zi;
   float bias, scale, zf;
-  bool has_zero, pair_out, bad;
+  bool has_zero, pair_out, wide_out, bad;
   int row_sum = 0;       // where no array of sums is given: of row `lane`
 
   __device__ __forceinline__ Epilogue(const W8Params& p)
       : y(reinterpret_cast<T*>(p.y)), ldy(p.ldy), M(p.M), N(p.N), has_zero(p.zero != nullptr),
-        pair_out((reinterpret_cast<uintptr_t>(p.y) & 3u) == 0 && (p.ldy & 1) == 0 && (p.N & 1) == 0), bad(false) {}
+        pair_out((reinterpret_cast<uintptr_t>(p.y) & 3u) == 0 && (p.ldy & 1) == 0 && (p.N & 1) == 0),
+        wide_out((reinterpret_cast<uintptr_t>(p.y) & 15u) == 0 && (p.ldy & 7) == 0 && (p.N & 7) == 0), bad(false) {}
   // The zero-point's whole part is taken off in integers, exactly; what is left (0 for the zero-points of quantizers, or a value
   // beyond any code) in fp32.
   __device__ __forceinline__ void column(const W8Params& p, int col) { column(col, fetch(p, col)); }
@@ -241,6 +242,36 @@ struct Epilogue {
     }
   }
 };
+
+// The same where rows allow 16-byte pieces: through `stage`, 1 KB of shared memory of this warp's own.
+template <typename T>
+__device__ __forceinline__ void store16_wide(const Epilogue<T>& e, const int (&a)[16], int m0, int end, const float* steps, const int* sums, uint4* stage) {
+  const int lane = threadIdx.x & 31;
+  T* to = reinterpret_cast<T*>(stage) + lane;
+  const float scale = e.bad ? __int_as_float(0x7fffffff) : e.scale;
+#pragma unroll
+  for (int i = 0; i < 16; i += 4) {
+    const float4 s4 = *reinterpret_cast<const float4*>(steps + i);
+    const float s[4] = {s4.x, s4.y, s4.z, s4.w};
+    if (e.has_zero) {
+      const int4 x4 = *reinterpret_cast<const int4*>(sums + i);
+      const int xs[4] = {x4.x, x4.y, x4.z, x4.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) to[(i + j) * 32] = from_float<T>(fmaf(fmaf(-e.zf, (float)xs[j], (float)(a[i + j] - e.zi * xs[j])), s[j] * scale, e.bias));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) to[(i + j) * 32] = from_float<T>(fmaf((float)a[i + j], s[j] * scale, e.bias));
+    }
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 16; i += 8) {
+    const int m = m0 + i + lane / 4, n = e.n - lane + lane % 4 * 8;
+    const uint4 w = stage[(i + lane / 4) * 4 + lane % 4];
+    if (m < end && n < e.N) *reinterpret_cast<uint4*>(e.y + (int64_t)m * e.ldy + n) = w;
+  }
+  __syncwarp();
+}
 
 __device__ __forceinline__ void load16(uint32_t taddr, int (&a)[16]) {
   uint32_t v[16];
@@ -307,8 +338,9 @@ __global__ void __launch_bounds__(kThreads, 1) w8a8_pair_kernel(const __grid_con
                                                                 const PairParams pp) {
   extern __shared__ unsigned char smem_raw[];
   __shared__ int s_failed;
-  __shared__ float s_step[2][256];
-  __shared__ int s_sums[2][256];
+  __shared__ __align__(16) float s_step[2][256];
+  __shared__ __align__(16) int s_sums[2][256];
+  __shared__ uint4 s_stage[kEpiThreads / 32][64];
   const W8Params& p = pp.w;
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int ku = p.ku, stages = p.stages;
@@ -453,7 +485,8 @@ __global__ void __launch_bounds__(kThreads, 1) w8a8_pair_kernel(const __grid_con
       for (int c = c0; c < mrows; c += 32) {
         int a[16];
         load16(acc + c, a);
-        epi.store16(a, m0 + c, m0 + mrows, s_step[buf] + c, s_sums[buf] + c);
+        if (epi.wide_out) store16_wide<T>(epi, a, m0 + c, m0 + mrows, s_step[buf] + c, s_sums[buf] + c, s_stage[warp - 4]);
+        else epi.store16(a, m0 + c, m0 + mrows, s_step[buf] + c, s_sums[buf] + c);
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
@@ -519,7 +552,8 @@ __global__ void __launch_bounds__(kThreads, 1) w8a8_pair_kernel(const __grid_con
             a[4 * i + 3] += (int)v.w;
           }
         }
-        epi.store16(a, m0 + from + c, m0 + to, s_step[0] + c, s_sums[0] + c);
+        if (epi.wide_out) store16_wide<T>(epi, a, m0 + from + c, m0 + to, s_step[0] + c, s_sums[0] + c, s_stage[warp - 4]);
+        else epi.store16(a, m0 + from + c, m0 + to, s_step[0] + c, s_sums[0] + c);
       }
     }
   }
