@@ -243,32 +243,41 @@ struct Epilogue {
   }
 };
 
-// The same where rows allow 16-byte pieces: through `stage`, 1 KB of shared memory of this warp's own.
+// The same where rows allow 16-byte pieces: through `stage`, 1 KB of shared memory of this warp's own, a word for two rows of a column.
+// (2048 rows of 28672 x 256, bound by this: 53 us; with a 16-bit store per output there 57, with shuffles and 4-byte pieces 63.)
 template <typename T>
 __device__ __forceinline__ void store16_wide(const Epilogue<T>& e, const int (&a)[16], int m0, int end, const float* steps, const int* sums, uint4* stage) {
   const int lane = threadIdx.x & 31;
-  T* to = reinterpret_cast<T*>(stage) + lane;
+  uint32_t* to = reinterpret_cast<uint32_t*>(stage) + lane;
   const float scale = e.bad ? __int_as_float(0x7fffffff) : e.scale;
 #pragma unroll
   for (int i = 0; i < 16; i += 4) {
     const float4 s4 = *reinterpret_cast<const float4*>(steps + i);
     const float s[4] = {s4.x, s4.y, s4.z, s4.w};
+    float f[4];
     if (e.has_zero) {
       const int4 x4 = *reinterpret_cast<const int4*>(sums + i);
       const int xs[4] = {x4.x, x4.y, x4.z, x4.w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) to[(i + j) * 32] = from_float<T>(fmaf(fmaf(-e.zf, (float)xs[j], (float)(a[i + j] - e.zi * xs[j])), s[j] * scale, e.bias));
+      for (int j = 0; j < 4; ++j) f[j] = fmaf(fmaf(-e.zf, (float)xs[j], (float)(a[i + j] - e.zi * xs[j])), s[j] * scale, e.bias);
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) to[(i + j) * 32] = from_float<T>(fmaf((float)a[i + j], s[j] * scale, e.bias));
+      for (int j = 0; j < 4; ++j) f[j] = fmaf((float)a[i + j], s[j] * scale, e.bias);
     }
+    to[(i / 2) * 32] = Pair<T>::pack(f[0], f[1]);
+    to[(i / 2 + 1) * 32] = Pair<T>::pack(f[2], f[3]);
   }
   __syncwarp();
-#pragma unroll
-  for (int i = 0; i < 16; i += 8) {
-    const int m = m0 + i + lane / 4, n = e.n - lane + lane % 4 * 8;
-    const uint4 w = stage[(i + lane / 4) * 4 + lane % 4];
-    if (m < end && n < e.N) *reinterpret_cast<uint4*>(e.y + (int64_t)m * e.ldy + n) = w;
+  // rows 2 r, 2 r + 1 of eight columns, the halves in an order that spreads the lanes over the banks
+  const int r = lane / 4, first = r & 1, m = m0 + 2 * r, n = e.n - lane + lane % 4 * 8;
+  const uint4* from = stage + r * 8 + lane % 4 * 2;
+  const uint4 p = from[first], q = from[first ^ 1], lo = first ? q : p, hi = first ? p : q;
+  const uint4 even = make_uint4(__byte_perm(lo.x, lo.y, 0x5410), __byte_perm(lo.z, lo.w, 0x5410), __byte_perm(hi.x, hi.y, 0x5410), __byte_perm(hi.z, hi.w, 0x5410));
+  const uint4 odd = make_uint4(__byte_perm(lo.x, lo.y, 0x7632), __byte_perm(lo.z, lo.w, 0x7632), __byte_perm(hi.x, hi.y, 0x7632), __byte_perm(hi.z, hi.w, 0x7632));
+  if (n < e.N) {
+    T* at = e.y + (int64_t)m * e.ldy + n;
+    if (m < end) *reinterpret_cast<uint4*>(at) = even;
+    if (m + 1 < end) *reinterpret_cast<uint4*>(at + e.ldy) = odd;
   }
   __syncwarp();
 }
@@ -283,7 +292,7 @@ __device__ __forceinline__ void load16(uint32_t taddr, int (&a)[16]) {
 // ---- product, two SMs on a tile -------------------------------------------------------------------------------------------------------
 // cta_group::2: two SMs on a tile of 256 weight rows x mt activation rows.  Each loads its own 128 weight rows and half of the
 // activation rows, the MMA reads both halves: 32 KB per SM and unit at mt = 256, where one SM alone with a 128 x 256 tile needs 48 KB, and
-// that set its pace (half the MMAs took the same time: 87 GB/s and SM from L2; 28672 x 4096, 2048 rows 260 us against 164, 2940 Top/s).  The
+// that set its pace (half the MMAs took the same time: 87 GB/s and SM from L2; 28672 x 4096, 2048 rows 260 us against 158 - 164, 2930 - 3040 Top/s).  The
 // even thread block of a pair issues the MMAs; its `full` barrier counts the bytes of both; commits arrive in both.
 //
 // A cluster is one pair, walking over tiles, or (few tiles, long K) two or four pairs that split K of one tile: then each of them adds up
@@ -454,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, 1) w8a8_pair_kernel(const __grid_con
     const int q4 = warp & 3, c0 = (warp - 4) / 4 * 16, te = threadIdx.x - 4 * 32;
     const uint32_t empty_at = in_block(acc_empty, leader);
     Epilogue<T> epi(p);
-    // A tile's scales and steps are read while the tile before it is stored (2048 rows of 28672 x 256 @@).
+    // A tile's scales and steps are read while the tile before it is stored.
     static_assert(kEpiThreads >= 256, "a thread per activation row of a tile");
     float3 of, of_next;
     float mine = 0.f;
