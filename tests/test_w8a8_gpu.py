@@ -185,6 +185,19 @@ def test_layer_takes_the_integer_path_when_asked(cuda_lib):
                layer.bias, layer.input_scale)
 
 
+@pytest.mark.parametrize("m,n,k", [(1, 264, 2048), (16, 264, 6144), (20, 264, 2048), (40, 136, 8192), (300, 520, 256), (513, 1032, 512)])
+def test_outputs_stay_inside_their_rows(m, n, k, cuda_lib):
+    x, w, scale, _ = _data(m, n, k, m, torch.bfloat16)
+    want = w8a8_forward(x, w, scale)
+    _check(want, x, w, scale)
+    for pad, left in ((8, 0), (16, 8), (6, 2), (7, 1)):              # rows of 16-byte pieces, of 4-byte pieces, of neither
+        big = torch.full((m + 2, n + pad), 5.0, dtype=torch.bfloat16, device=DEV)
+        w8a8_forward(x, w, scale, out=big[1:-1, left:left + n])
+        assert torch.equal(big[1:-1, left:left + n], want)
+        big[1:-1, left:left + n] = 5.0
+        assert big.eq(5).all()
+
+
 @pytest.mark.parametrize("granularity", ["per_channel", "per_tensor"])
 def test_layer_follows_loaded_states_and_moves(granularity, cuda_lib):
     def layer(seed, sym):
