@@ -34,8 +34,7 @@ namespace {
 using namespace paged;
 
 constexpr int kHeads = 8;                  // query heads of a tile (MMA columns)
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
+constexpr int kWarpsPerSm = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kBias = 4.f, kSlack = 11.f;
 constexpr float kLowest = -3e38f;          // a reference below every score, and finite
@@ -47,7 +46,10 @@ struct Shape {
   static constexpr int kStages = D == 128 ? 3 : 6;
   static constexpr int kChunks = kUnit * D / 512;             // 16-byte chunks of a unit's keys (or values) per lane
   static constexpr int kRing = kStages * kStageBytes;         // per warp
-  static constexpr size_t kSmem = (size_t)kWarps * kRing;     // two thread blocks per SM
+  // An SM's warps in one thread block: of two, one runs ahead and leaves the other alone at the end (16 x 32768 tokens: 76 and 88 us, 86
+  // with one).  Not for short heads, whose calls are short.
+  static constexpr int kWarps = D == 128 ? kWarpsPerSm : kWarpsPerSm / 2, kThreads = kWarps * 32, kBlocksPerSm = kWarpsPerSm / kWarps;
+  static constexpr size_t kSmem = (size_t)kWarps * kRing;
   static constexpr int kPartFloats = kHeads * D + 2 * kHeads; // a part in the workspace: O as the lanes hold it, maxima, sums
 };
 
@@ -407,7 +409,7 @@ struct Tile {
 };
 
 template <typename T, int D, bool PACKED>
-__global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttnParams p) {
+__global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocksPerSm) paged_attn_kernel(const PagedAttnParams p) {
   using S = Shape<D>;
   extern __shared__ __align__(128) unsigned char smem[];
   pdl_launch_dependents();
@@ -418,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
   // The last token that begins at or before this run: 32 candidates a round, the first round together with the number of units
   const int all = p.unit_start[p.T], spread = (p.T + 31) / 32;
   const int mark = lane * spread < p.T ? p.unit_start[lane * spread] : 0x7fffffff;
-  const int64_t total = (int64_t)all * tiles, run = run_units(total, gridDim.x * kWarps);
+  const int64_t total = (int64_t)all * tiles, run = run_units(total, gridDim.x * S::kWarps);
   const int64_t u0 = me * run, u1 = min(u0 + run, total);
   if (u0 >= u1) return;
   const int x = (int)(u0 / tiles), k0 = 31 - __clz(__ballot_sync(0xffffffffu, mark <= x));
@@ -657,8 +659,7 @@ __global__ void __launch_bounds__(GROUPS > 1 ? GROUPS * 32 : D * 2) paged_merge_
   }
 }
 
-int attn_blocks() { return 2 * sm_count(); }
-size_t workspace_of(int D, int blocks) { return (size_t)blocks * kWarps * 2 * (kHeads * D + 2 * kHeads) * sizeof(float); }
+size_t workspace_of(int D) { return (size_t)sm_count() * kWarpsPerSm * 2 * (kHeads * D + 2 * kHeads) * sizeof(float); }
 
 }  // namespace
 }  // namespace pare
@@ -670,7 +671,7 @@ using namespace pare::paged;
 
 size_t pare_paged_attn_workspace_bytes(int D) {
   if (D != 64 && D != 128) return 0;
-  return workspace_of(D, attn_blocks());
+  return workspace_of(D);
 }
 
 int pare_paged_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h, const pare_paged_layer* l, const pare_paged_tables* tb, int Hq,
@@ -684,8 +685,7 @@ int pare_paged_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h, const
   if (T == 0) return PARE_OK;
   PARE_REQUIRE(q && out, PARE_ERR_SHAPE);
   PARE_REQUIRE(aligned16(q) && (q_stride_t | q_stride_h) % 8 == 0 && aligned16(workspace), PARE_ERR_ALIGN);
-  const int blocks = attn_blocks();
-  PARE_REQUIRE(workspace && workspace_bytes >= workspace_of(D, blocks), PARE_ERR_WORKSPACE);
+  PARE_REQUIRE(workspace && workspace_bytes >= workspace_of(D), PARE_ERR_WORKSPACE);
   const int group = Hq / H, sub = (group + kHeads - 1) / kHeads, packs = !packs_tokens(tb->R, T) || group > 4 ? 0 : group == 1 ? 3 : group == 2 ? 2 : 1;
   PARE_REQUIRE((int64_t)T * H * sub < (int64_t)1 << 31, PARE_ERR_UNSUPPORTED);
   // the step counts its units in 32 bits
@@ -703,10 +703,11 @@ int pare_paged_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h, const
     constexpr int kD = decltype(dim)::value;
     constexpr bool kPacked = decltype(packed)::value;
     const auto kern = paged_attn_kernel<E, kD, kPacked>;
+    const int sms = sm_count();
     if (!ensure_smem_attr(reinterpret_cast<const void*>(kern), (int)Shape<kD>::kSmem)) return (int)PARE_ERR_CUDA;
-    int status = launch_pdl(kern, dim3(blocks), dim3(kThreads), Shape<kD>::kSmem, st, p);
+    int status = launch_pdl(kern, dim3(sms * Shape<kD>::kBlocksPerSm), dim3(Shape<kD>::kThreads), Shape<kD>::kSmem, st, p);
     if (status != PARE_OK) return status;
-    const int jobs = T * H * sub, sms = blocks / 2, warps = blocks * kWarps;
+    const int jobs = T * H * sub, warps = sms * kWarpsPerSm;
     auto merge = [&](auto kernel, int groups) {
       return groups > 1 ? launch_pdl(kernel, dim3(jobs, kD / 16), dim3(groups * 32), 0, st, p, warps)
                         : launch_pdl(kernel, dim3(std::min(jobs, 32 * sms)), dim3(2 * kD), 0, st, p, warps);
