@@ -20,9 +20,10 @@
 //
 // A tile's eight columns are heads of one token, or, where a step has more rows than requests, heads of up to eight tokens of a request.
 //
-// Bound: the cache's bytes for long contexts, instructions (conversion of codes, 0.6 - 0.7 of the issue slots) close behind; one sequence
-// is a chain of dependent reads.  Both launches: 16 x 32768 tokens, 28 / 4 heads, fp16 103 us (540 MB: 0.80 of the copy rate); 64 requests of
-// up to 2000 tokens, 32 / 8 heads, bf16 60 us (0.66); one of 4096 tokens 12.7 us; three tokens of 12 requests over 1500, D = 64 20 us.
+// Bound: the cache's bytes for long contexts, instructions (conversion of codes, 0.6 - 0.7 of the issue slots) close behind, and 8 us that
+// the second launch takes after the last warp; one sequence is a chain of dependent reads.  Both launches: 16 x 32768 tokens, 28 / 4 heads, fp16
+// 102 us (540 MB: 0.81 of the copy rate; the first launch alone 96); 64 requests of up to 3600 tokens, 32 / 8 heads, bf16 59 us (0.68); one of
+// 4096 tokens 12.6 us; three tokens of 12 requests over 1500 on average, D = 64 20 us.
 #include <algorithm>
 #include <type_traits>
 
