@@ -20,10 +20,10 @@
 //
 // A tile's eight columns are heads of one token, or, where a step has more rows than requests, heads of up to eight tokens of a request.
 //
-// Bound: the cache's bytes for long contexts, instructions (conversion of codes, 0.6 - 0.7 of the issue slots) close behind, and 8 us that
+// Bound: the cache's bytes for long contexts, instructions (conversion of codes, 0.6 - 0.7 of the issue slots) close behind, and 7 us that
 // the second launch takes after the last warp; one sequence is a chain of dependent reads.  Both launches: 16 x 32768 tokens, 28 / 4 heads, fp16
-// 102 us (540 MB: 0.81 of the copy rate; the first launch alone 96); 64 requests of up to 3600 tokens, 32 / 8 heads, bf16 59 us (0.68); one of
-// 4096 tokens 12.6 us; three tokens of 12 requests over 1500 on average, D = 64 20 us.
+// 100 us (540 MB: 0.82 of the copy rate; the first launch alone 96); 64 requests of up to 3600 tokens, 32 / 8 heads, bf16 59 us (0.68); one of
+// 4096 tokens 11.8 us; three tokens of 12 requests over 1500 on average, D = 64 19.3 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -413,11 +413,11 @@ template <typename T, int D, bool PACKED>
 __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocksPerSm) paged_attn_kernel(const PagedAttnParams p) {
   using S = Shape<D>;
   extern __shared__ __align__(128) unsigned char smem[];
-  pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   const int tiles = p.H * p.sub;       // tiles of eight heads per token
   const int me = warp * gridDim.x + blockIdx.x;      // a few runs spread over all SMs
   pdl_wait();
+  pdl_launch_dependents();      // not before: the second launch reads the step before it waits for this one
   // The last token that begins at or before this run: 32 candidates a round, the first round together with the number of units
   const int all = p.unit_start[p.T], spread = (p.T + 31) / 32;
   const int mark = lane * spread < p.T ? p.unit_start[lane * spread] : 0x7fffffff;
@@ -588,15 +588,17 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocksPerSm) pa
 // (D / 8) g + 2 i, + 1 x heads 2 t, 2 t + 1).  Many tiles have few parts each: a thread block per tile, a warp per piece.  Few tiles have
 // many (one sequence: 86): GROUPS warps share a piece, each every GROUPS-th part, and are added up in order.  A warp alone gets
 // through one instruction in about eight cycles, so what is serial counts: 8 tiles of 4096 tokens, both kernels, 22.7 / 15.8 / 13.1 / 12.7 us
-// with 2 / 4 / 8 / 16 groups; 64 tiles of 32768 tokens 101 / 99 / 99 / 106 us, 108 with one.
+// with 2 / 4 / 8 / 16 groups (11.8 now: six parts in flight, the step read before the wait, which saves 0.8 us everywhere); 64 tiles of 32768
+// tokens 101 / 99 / 99 / 106 us, 108 with one.
 template <typename T, int D, int GROUPS, bool PACKED>
 __global__ void __launch_bounds__(GROUPS > 1 ? GROUPS * 32 : D * 2) paged_merge_kernel(const PagedAttnParams p, int warps) {
   using S = Shape<D>;
-  constexpr int kFlight = 4;     // parts in flight per warp
+  constexpr int kFlight = GROUPS == 16 ? 6 : 4;     // parts in flight per warp
   __shared__ float4 s_o[GROUPS][32], s_ml[GROUPS][32];
   const int tiles = p.H * p.sub, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   const int group = GROUPS > 1 ? warp : 0, piece = GROUPS > 1 ? blockIdx.y : warp;
-  pdl_wait();
+  // The step was complete before the first launch let this one begin; its parts are there, and its readers of `out` gone, after the wait.
+  bool waited = false;
   const int64_t total = (int64_t)p.unit_start[p.T] * tiles, run = run_units(total, warps);
   auto run_of = [&](int64_t u) { return total >> 32 ? (int)(u / run) : (int)((uint32_t)u / (uint32_t)run); };
   for (int job = blockIdx.x; job < p.T * tiles; job += gridDim.x) {
@@ -605,6 +607,10 @@ __global__ void __launch_bounds__(GROUPS > 1 ? GROUPS * 32 : D * 2) paged_merge_
     const int64_t a = (int64_t)first_unit * tiles + (int64_t)h * units;
     const int first = run_of(a), last = units ? run_of(a + units - 1) : first;
     if (first == last) continue;
+    if (!waited) {
+      waited = true;
+      pdl_wait();
+    }
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     float2 top = make_float2(-INFINITY, -INFINITY), l = make_float2(0.f, 0.f);
     auto add = [&](const float2& m, const float2& s, const float4& x) {
@@ -658,6 +664,7 @@ __global__ void __launch_bounds__(GROUPS > 1 ? GROUPS * 32 : D * 2) paged_merge_
     if (out0) out0[c] = from_float<T>(o.x / l.x), out0[c + 1] = from_float<T>(o.z / l.x);
     if (out1) out1[c] = from_float<T>(o.y / l.y), out1[c + 1] = from_float<T>(o.w / l.y);
   }
+  if (!waited) pdl_wait();      // what comes after this launch comes after the first one too
 }
 
 size_t workspace_of(int D) { return (size_t)sm_count() * kWarpsPerSm * 2 * (kHeads * D + 2 * kHeads) * sizeof(float); }
