@@ -383,7 +383,7 @@ int pare_paged_dense(const pare_paged_layer* layer, const pare_paged_tables* tab
 
 /* Attention of the step's tokens over the layer, after the step's append: token t of request r attends to the positions up to its
  * own.  q, out [T][Hq][D] (element strides; q's multiples of 8, 16-byte aligned), query head hq reads KV head hq / (Hq / H), any
- * ratio; T <= 4096.  Rows that belong to nobody are left as they were.  Ids not in the pool read as NaN.  The workspace
+ * ratio; T <= 4096 and T * (max_blocks * block_size / 16 + 2) < 2^31 (a 32-bit count of work).  Rows that belong to nobody are left as they were.  Ids not in the pool read as NaN.  The workspace
  * (16-byte aligned, pare_paged_attn_workspace_bytes()) need not be initialised and holds nothing between calls. */
 size_t pare_paged_attn_workspace_bytes(int D);
 int pare_paged_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h, const pare_paged_layer* layer, const pare_paged_tables* tables,

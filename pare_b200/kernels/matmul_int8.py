@@ -39,7 +39,7 @@ def w8a8_forward(x: Tensor, q_weight: Tensor, scale: Tensor, zero: Tensor | None
     ``q_weight`` is int8 ``[N, K]`` (rows a multiple of 16 bytes apart and 16-byte aligned; others are copied), ``scale`` and the
     optional ``zero`` float32 ``[N]``, ``input_scale`` float32 ``[K]`` divides the activations first (the quotient rounded to
     their dtype), ``bias`` ``[N]``.  ``K`` is at most 65536.  The result has the dtype of ``x``; a row of ``x`` with an infinity or
-    NaN gives NaN.  ``out``: where to put it (``[M, N]``, adjacent columns, not overlapping ``x``).
+    NaN gives NaN.  ``out``: where to put it (``[M, N]``, adjacent columns, not overlapping ``x``).  No gradients.
     """
     if not x.is_cuda:
         raise RuntimeError("w8a8_forward requires CUDA tensors.")
