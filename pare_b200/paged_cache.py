@@ -189,25 +189,29 @@ def plan_blocks(seq_lens: Tensor, new_lens: Tensor, block_table: Tensor, free_bl
     lengths and free blocks stay): :meth:`PagedStep.check`.  Other inputs than the table are not written; to go on from the step,
     use its ``seq_lens`` and ``free_count``.
     """
-    dev = seq_lens.device
+    dev, index, i32 = seq_lens.device, seq_lens.get_device(), torch.int32
     if dev.type != "cuda":
         raise RuntimeError("plan_blocks runs on CUDA tensors only")
-    shape, rows, capacity, i32 = seq_lens.shape, block_table.shape, free_blocks.numel(), torch.int32
-    n = shape[0] if len(shape) == 1 else 0
-    for t, want, what in ((seq_lens, (n,), "seq_lens"), (new_lens, (n,), "new_lens"), (free_count, (1,), "free_count"),
-                          (free_blocks, (capacity,), "free_blocks")):
-        if t.dtype is not i32 or t.shape != want or t.device != dev or not t.is_contiguous():
+    n, capacity = seq_lens.numel(), free_blocks.numel()
+    width = ld = block_table.shape[1] if block_table.dim() == 2 else 0
+    if not (seq_lens.dtype is new_lens.dtype is free_blocks.dtype is free_count.dtype is block_table.dtype is i32
+            and seq_lens.dim() == new_lens.dim() == free_blocks.dim() == free_count.dim() == 1 and new_lens.numel() == n and free_count.numel() == 1
+            and width and block_table.shape[0] == n
+            and index == new_lens.get_device() == free_blocks.get_device() == free_count.get_device() == block_table.get_device()
+            and seq_lens.is_contiguous() and new_lens.is_contiguous() and free_blocks.is_contiguous() and free_count.is_contiguous()
+            and block_table.is_contiguous()):
+        for t, want, what in ((seq_lens, (n,), "seq_lens"), (new_lens, (n,), "new_lens"), (free_count, (1,), "free_count"),
+                              (free_blocks, (capacity,), "free_blocks")):
             _ints(t, want, dev, what)
-    ld = rows[1] if len(rows) == 2 else 0
-    if block_table.dtype is not i32 or ld == 0 or rows[0] != n or block_table.device != dev or not block_table.is_contiguous():
-        if block_table.dtype is not i32 or ld == 0 or rows[0] != n or block_table.device != dev or block_table.stride(1) != 1 or block_table.stride(0) < ld:
+        if (block_table.dtype is not i32 or not width or block_table.shape[0] != n or block_table.device != dev or block_table.stride(1) != 1
+                or (n > 1 and block_table.stride(0) < width)):
             raise ValueError(f"block_table must be int32 [{n}, blocks per request] with adjacent columns on {dev}")
-        ld = block_table.stride(0)
+        ld = block_table.stride(0) if n > 1 else width
     nbytes, at = _step_layout(n, tokens, block_size)
     words = seq_lens.new_empty(nbytes // 4)
     step = PagedStep(words, at, n, tokens, block_size, block_table, ld)
     _call(dev, _lib.lib().pare_paged_plan, "pare_paged_plan", seq_lens.data_ptr(), new_lens.data_ptr(), n, block_table.data_ptr(),
-          ld, rows[1], free_blocks.data_ptr(), capacity, free_count.data_ptr(), block_size, tokens, words.data_ptr(), nbytes)
+          ld, width, free_blocks.data_ptr(), capacity, free_count.data_ptr(), block_size, tokens, words.data_ptr(), nbytes)
     return step
 
 
