@@ -10,7 +10,8 @@
 // two per head that puts its largest magnitude into [256, 512): every bf16 value within 2^-22 of that is exact, smaller ones are
 // within 2^-34 of the largest.  Softmax runs online: a reference value per head which only moves when a score passes it by more than
 // 2^kSlack (one vote per 16 tokens instead of a reduction); probabilities are kept times 2^kBias of that, so those down to 2^-18 of
-// the reference are normal fp16 numbers and none passes 2^15.  Their sum is taken before their rounding to fp16.
+// the reference are normal fp16 numbers and none passes 2^15.  Their sum is taken before they become two fp16 numbers each (those of
+// open rows two of the rows' type).
 //
 // Work.  Units of 16 tokens of one (token, group of heads), counted by the step's tables; each WARP takes one contiguous run of
 // units, all runs equally long, so ragged lengths balance by themselves and the host needs to know none of them.  A warp feeds
@@ -158,9 +159,6 @@ __device__ __forceinline__ int64_t run_units(int64_t total, int warps) {
 template <typename T, int D, bool PACKED>
 struct Tile {
   using S = Shape<D>;
-  // Rounding a probability to fp16 is off by 2^-11 of it: nothing beside a bf16 result, as much as the rounding of an fp16 result.
-  // There it is two numbers, the second what the first left (16 x 32768 tokens: 105 us instead of 98).
-  static constexpr bool kTwoTerms = std::is_same<T, __half>::value;
   static constexpr int kJ = D / 64;              // 16-byte chunks of a key row per lane
   static constexpr int kW = D / 32;              // words of four value channels per lane and token: channels (D / 8) g ..
   uint32_t qh[kJ][4][2];                         // query operand, fp16: channels 16 (t + 4 j) + 4 w + {0, 1}, {2, 3} of head g
@@ -287,13 +285,11 @@ struct Tile {
     softmax(s, ks * f0, ks * f1, least, seen0, seen1, g);
     // a block that a head does not see at all may have a scale that is not finite
     const float vs0 = PACKED && seen0 <= 0 ? 0.f : vs, vs1 = PACKED && seen1 <= 0 ? 0.f : vs;
+    // Rounding a probability to fp16 is off by up to 2^-11 of it, which changes a tenth of bf16 results by a step and is as much as the
+    // rounding of an fp16 result.  So it is two numbers, the second what the first left: off by 2^-22.
     const uint32_t h0 = pack_half2(s[0], s[1]), h1 = pack_half2(s[2], s[3]), p0 = transpose8x8(h0), p1 = transpose8x8(h1);
-    uint32_t r0 = 0, r1 = 0;       // what the rounding left
-    if constexpr (kTwoTerms) {
-      const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h0)), b = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-      r0 = transpose8x8(pack_half2(s[0] - a.x, s[1] - a.y));
-      r1 = transpose8x8(pack_half2(s[2] - b.x, s[3] - b.y));
-    }
+    const float2 e0 = __half22float2(*reinterpret_cast<const __half2*>(&h0)), e1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+    const uint32_t r0 = transpose8x8(pack_half2(s[0] - e0.x, s[1] - e0.y)), r1 = transpose8x8(pack_half2(s[2] - e1.x, s[3] - e1.y));
     const uint32_t vbase = stage + kUnit * D;
     uint32_t v[4][kW];   // tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 x channels (D / 8) g ..
 #pragma unroll
@@ -317,10 +313,8 @@ struct Tile {
       float x[4], y[4];
       mma16816_first(x, a[0], a[1], a[2], a[3], p0, p1);
       mma16816_first(y, b[0], b[1], b[2], b[3], p0, p1);
-      if constexpr (kTwoTerms) {
-        mma16816<__half>(x, a[0], a[1], a[2], a[3], r0, r1);
-        mma16816<__half>(y, b[0], b[1], b[2], b[3], r0, r1);
-      }
+      mma16816<__half>(x, a[0], a[1], a[2], a[3], r0, r1);
+      mma16816<__half>(y, b[0], b[1], b[2], b[3], r0, r1);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         o[2 * w][i] = fmaf((i & 1) ? vs1 : vs0, x[i], o[2 * w][i]);

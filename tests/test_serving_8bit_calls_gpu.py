@@ -1,0 +1,49 @@
+"""Calls of the 8-bit operators that the tests of each operator do not make: precision between roundings, steps and layers that change
+under a program, calls that are refused half way, other streams."""
+
+import math
+
+import pytest
+import torch
+
+from pare_b200 import paged_cache as pc
+from test_paged_gpu import _cache, _feed, _Model, _rand
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+
+
+# ---- attention: nothing but the result is rounded to 16 bits ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("h,group,d,new", [(2, 4, 128, 1), (8, 4, 128, 1), (4, 7, 128, 1), (2, 8, 64, 1), (2, 1, 128, 4), (2, 2, 64, 3)])
+def test_probabilities_keep_more_than_the_result(h, group, d, new, dtype, cuda_lib):
+    """A probability rounded to one 16-bit number would change a tenth of the bf16 results."""
+    cache, model = _cache(2, h, d, 16, dtype, blocks=400), _Model(2, h, d, 16, dtype)
+    _feed(cache, model, [1500, 333], 1)
+    step, _, _ = _feed(cache, model, [new, new], 2)
+    q = _rand((2 * new, h * group, d), 3, dtype)
+    out = pc.attend_blocks(cache.layers[0], step, q)
+    wrong = total = 0
+    for row in range(2 * new):
+        r = row // new
+        seen = model.k[r].shape[1] - new + row % new + 1
+        k, v = model.dense(model.k[r])[:, :seen], model.dense(model.v[r])[:, :seen]
+        qq = q[row].double().view(h, group, d)
+        s = qq @ k.transpose(1, 2) / math.sqrt(d)
+        p = torch.softmax(s, -1)
+        want = (p @ v).reshape(-1, d)
+        # Before the result's own rounding.  Scores: sums of d products in fp32, 2 d + 8 roundings of the magnitudes at most, twice (numerator and
+        # denominator).  Probabilities in two terms: 2^-16 of them; ex2 and the rescales 2^-18; what is subnormal in fp16 loses at most
+        # 2^-25 where the largest is 2^4 or more.
+        mag = (qq.abs() @ k.abs().transpose(1, 2)).amax(-1, keepdim=True) / math.sqrt(d)
+        rel = 2.0 ** -16 + 2 * ((2 * d + 8) * 2.0 ** -24 * mag) + 2.0 ** -18
+        bound = (rel * (p @ v.abs()) + seen * 2.0 ** -29 * v.abs().amax(1, keepdim=True)).reshape(-1, d)
+        half = torch.finfo(dtype).eps / 2 * want.abs() * (1 + torch.finfo(dtype).eps) + (2.0 ** -25 if dtype is torch.float16 else 0)
+        assert bool(((out[row].double() - want).abs() <= half + bound).all())
+        wrong += int((out[row] != want.to(dtype)).sum())
+        total += want.numel()
+    # An error of `bound` crosses a border between two results with a probability of 2 bound / step; the errors are far smaller than
+    # their bounds, so one result in fifty is more than what two terms can change and less than what one term does.
+    assert wrong <= total / 50 if dtype is torch.bfloat16 else wrong <= total / 10
