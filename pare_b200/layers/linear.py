@@ -50,8 +50,13 @@ from pare_b200.kernels.matmul_int8 import aligned_rows, w8a8_forward as _w8a8
 _FP8 = (QuantDtype.FP8_E4M3, QuantDtype.FP8_E5M2)
 
 
+def _version(t: Tensor) -> int:
+    return -1 if t.is_inference() else t._version
+
+
 class QuantizedLinear(nn.Module):
     int8_kernel = False
+    _int8_made: tuple | None = None      # q_weight, scale and zero that the derived tensors were made from, and their versions
 
     def __init__(
         self,
@@ -193,9 +198,7 @@ class QuantizedLinear(nn.Module):
         return y if flat else y.reshape(*shape[:-1], self.out_features)
 
     def _forward_int8(self, x: Tensor) -> Tensor:
-        bufs, k, shape, dtype = self._buffers, self.in_features, x.shape, x.dtype
-        if "_q_weight_int8" not in bufs:
-            self._prepare_int8_buffers()
+        bufs, shape, dtype = self._int8_buffers(), x.shape, x.dtype
         x2d = x if len(shape) == 2 else x.reshape(-1, shape[-1])
         if dtype is not torch.float16 and dtype is not torch.bfloat16:
             x2d = x2d.to(torch.float16)
@@ -204,30 +207,52 @@ class QuantizedLinear(nn.Module):
             y = y.to(dtype)
         return y if len(shape) == 2 else y.reshape(*shape[:-1], self.out_features)
 
+    # The integer product's derived, non-persistent tensors follow what they were made from: each call looks whether that has been
+    # replaced or (by its version counter, which `.data` and tensors made under inference_mode bypass) written to.
+    def _int8_buffers(self) -> dict:
+        bufs, made = self._buffers, self._int8_made
+        q, s, z = bufs["q_weight"], bufs["scale"], bufs["zero"]
+        if made is None or made[0] is not q or made[1] is not s or made[2] is not z or made[3] != (_version(q), _version(s), _version(z)):
+            self._prepare_int8_buffers()
+        return bufs
+
     def _prepare_int8_buffers(self) -> None:
-        """The derived, non-persistent tensors of the integer product (first call only)."""
-        n, scale, zero = self.out_features, self.scale, self.zero
+        bufs, n, made = self._buffers, self.out_features, self._int8_made or (None, None, None)
+        q_weight, scale, zero = sources = self.q_weight, self.scale, self.zero
         if self.config.effective_dtype is not QuantDtype.INT8 or not self.quantize_inputs or self.g_idx is not None:
             raise ValueError("int8_kernel needs an INT8 layer with quantize_inputs and without g_idx")
         if scale.numel() not in (1, n) or zero.numel() not in (1, n):
             raise ValueError("int8_kernel needs one scale per output channel or per tensor (granularity per_channel or per_tensor)")
-        zero = zero.float().reshape(-1).expand(n).contiguous()
-        self.register_buffer("_scale_int8", scale.float().reshape(-1).expand(n).contiguous(), persistent=False)
-        self.register_buffer("_zero_int8", zero if bool(zero.any()) else None, persistent=False)
-        self.register_buffer("_q_weight_int8", aligned_rows(self.q_weight), persistent=False)
+        versions = _version(q_weight), _version(scale), _version(zero)
 
-    def _drop_int8_buffers(self) -> None:
+        def keep(name: str, now: Tensor, source: int) -> None:
+            # a tensor that was only written to: its derived one as well, where a captured graph reads it
+            if made[source] is sources[source] and bufs.get(name) is not None:
+                if bufs[name].data_ptr() != now.data_ptr():
+                    bufs[name].copy_(now)
+            else:
+                self.register_buffer(name, now, persistent=False)
+
+        zero = zero.float().reshape(-1).expand(n).contiguous()
+        keep("_scale_int8", scale.float().reshape(-1).expand(n).contiguous(), 1)
+        if bool(zero.any()) or (made[2] is self.zero and bufs.get("_zero_int8") is not None):
+            keep("_zero_int8", zero, 2)
+        else:
+            self.register_buffer("_zero_int8", None, persistent=False)
+        keep("_q_weight_int8", aligned_rows(q_weight), 0)
+        self._int8_made = (*sources, versions)
+
+    def _load_from_state_dict(self, *args, **kwargs) -> None:
+        super()._load_from_state_dict(*args, **kwargs)
+        if self._int8_made is not None:
+            self._int8_made = (*self._int8_made[:3], None)
+
+    # The tensors move or change their type, and moving the derived ones would lose their rows' alignment.
+    def _apply(self, *args, **kwargs):
+        self._int8_made = None
         for name in ("_q_weight_int8", "_scale_int8", "_zero_int8"):
             if name in self._buffers:
                 delattr(self, name)
-
-    # Both may change what the derived tensors were made from (moving them would also lose their rows' alignment).
-    def _load_from_state_dict(self, *args, **kwargs) -> None:
-        self._drop_int8_buffers()
-        super()._load_from_state_dict(*args, **kwargs)
-
-    def _apply(self, *args, **kwargs):
-        self._drop_int8_buffers()
         return super()._apply(*args, **kwargs)
 
     def supports_prepared(self, rows: int) -> bool:

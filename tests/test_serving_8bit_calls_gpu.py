@@ -5,9 +5,12 @@ import math
 
 import pytest
 import torch
+import torch.nn as nn
 
+from pare_b200 import QuantConfig, QuantizedLinear
 from pare_b200 import paged_cache as pc
 from test_paged_gpu import _cache, _feed, _Model, _rand
+from test_w8a8_gpu import _check as _check_linear
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +50,65 @@ def test_probabilities_keep_more_than_the_result(h, group, d, new, dtype, cuda_l
     # An error of `bound` crosses a border between two results with a probability of 2 bound / step; the errors are far smaller than
     # their bounds, so one result in fifty is more than what two terms can change and less than what one term does.
     assert wrong <= total / 50 if dtype is torch.bfloat16 else wrong <= total / 10
+
+
+# ---- integer layers -----------------------------------------------------------------------------------------------------------------
+
+def _layer(k=500, n=300, seed=0, sym=False, granularity="per_channel", input_scale=False):
+    torch.manual_seed(seed)
+    layer = QuantizedLinear.from_linear(nn.Linear(k, n), QuantConfig(bits=8, scheme="smoothquant", granularity=granularity, sym=sym))
+    if input_scale:
+        layer.input_scale = 0.5 + torch.rand(k)
+    layer.quantize_inputs, layer.use_kernel, layer.int8_kernel = True, True, True
+    return layer.cuda()
+
+
+def _as_defined(layer, x):
+    n = layer.out_features
+    ins = None if layer.input_scale is None else layer.input_scale.float()
+    y = layer(x)
+    _check_linear(y, x, layer.q_weight, layer.scale.float().reshape(-1).expand(n), layer.zero.float().reshape(-1).expand(n), layer.bias, ins)
+    return y
+
+
+@pytest.mark.parametrize("k", [500, 512])
+@pytest.mark.parametrize("granularity", ["per_channel", "per_tensor"])
+def test_layer_follows_its_tensors(granularity, k, cuda_lib):
+    """Weights, scales and zero-points that are replaced or written to between calls."""
+    x = torch.randn(5, k, device=DEV, dtype=torch.float16)
+    layer = _layer(k, granularity=granularity, sym=True)
+    _as_defined(layer, x)
+    layer.zero.copy_(torch.tensor(7.0))                     # a zero-point where there was none
+    _as_defined(layer, x)
+    layer.scale.mul_(3.0)
+    _as_defined(layer, x)
+    layer.q_weight.copy_(layer.q_weight.flip(0))
+    _as_defined(layer, x)
+    layer.zero.zero_()
+    _as_defined(layer, x)
+    made = layer._int8_made
+    _as_defined(layer, x)
+    assert layer._int8_made is made                         # nothing is made again while nothing changes
+    old = layer.scale.clone(), layer.q_weight.clone()
+    gone = layer.scale, layer.q_weight
+    layer.scale, layer.zero = layer.scale * 2, layer.zero - 3.0
+    _as_defined(layer, x)
+    layer.q_weight = -layer.q_weight.clamp(-127, 127)
+    _as_defined(layer, x)
+    assert torch.equal(gone[0], old[0]) and torch.equal(gone[1], old[1])      # what was replaced is left alone
+
+
+def test_a_captured_layer_follows_a_loaded_state(cuda_lib):
+    """Loading writes into the layer's tensors; after the next call a graph that was captured before reads them too."""
+    first, other = _layer(seed=1), _layer(seed=2)
+    x = torch.randn(5, 500, device=DEV, dtype=torch.float16)
+    first(x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = first(x)
+    first.load_state_dict(other.state_dict())
+    want = _as_defined(first, x)
+    torch.empty(1 << 20, dtype=torch.uint8, device=DEV).fill_(77)             # freed memory would be in use again
+    graph.replay()
+    assert torch.equal(y, want) and torch.equal(want, other(x))
