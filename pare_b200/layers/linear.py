@@ -225,21 +225,23 @@ class QuantizedLinear(nn.Module):
             raise ValueError("int8_kernel needs one scale per output channel or per tensor (granularity per_channel or per_tensor)")
         versions = _version(q_weight), _version(scale), _version(zero)
 
-        def keep(name: str, now: Tensor, source: int) -> None:
+        def derived(name: str, now: Tensor, source: int) -> Tensor:
             # a tensor that was only written to: its derived one as well, where a captured graph reads it
-            if made[source] is sources[source] and bufs.get(name) is not None:
-                if bufs[name].data_ptr() != now.data_ptr():
-                    bufs[name].copy_(now)
-            else:
-                self.register_buffer(name, now, persistent=False)
+            old = bufs.get(name) if made[source] is sources[source] else None
+            if old is None or old.data_ptr() == now.data_ptr():
+                return now if old is None else old
+            return old.copy_(now)
 
-        zero = zero.float().reshape(-1).expand(n).contiguous()
-        keep("_scale_int8", scale.float().reshape(-1).expand(n).contiguous(), 1)
-        if bool(zero.any()) or (made[2] is self.zero and bufs.get("_zero_int8") is not None):
-            keep("_zero_int8", zero, 2)
-        else:
-            self.register_buffer("_zero_int8", None, persistent=False)
-        keep("_q_weight_int8", aligned_rows(q_weight), 0)
+        zeros = zero.float().reshape(-1).expand(n).contiguous()
+        new = {"_q_weight_int8": derived("_q_weight_int8", aligned_rows(q_weight), 0),
+               "_scale_int8": derived("_scale_int8", scale.float().reshape(-1).expand(n).contiguous(), 1),
+               "_zero_int8": derived("_zero_int8", zeros, 2)}
+        # Reading whether there is a zero-point waits for this stream: the next call may come on another one, which knows nothing of the
+        # copies.  They are in the layer's hands only then, another thread may be in a call.
+        if not bool(zeros.any()) and (made[2] is not zero or bufs.get("_zero_int8") is None):
+            new["_zero_int8"] = None
+        for name, t in new.items():
+            self.register_buffer(name, t, persistent=False)
         self._int8_made = (*sources, versions)
 
     def _load_from_state_dict(self, *args, **kwargs) -> None:

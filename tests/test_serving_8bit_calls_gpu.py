@@ -112,3 +112,26 @@ def test_a_captured_layer_follows_a_loaded_state(cuda_lib):
     torch.empty(1 << 20, dtype=torch.uint8, device=DEV).fill_(77)             # freed memory would be in use again
     graph.replay()
     assert torch.equal(y, want) and torch.equal(want, other(x))
+
+
+def test_a_layer_that_two_streams_call_first(cuda_lib, monkeypatch):
+    """The first call makes the derived tensors on its stream; the next one, on another stream, finds them made."""
+    from pare_b200.layers import linear
+
+    copy = linear.aligned_rows
+
+    def late(q_weight):
+        torch.cuda._sleep(200_000_000)                      # a tenth of a second: the copy ends long after the call has returned
+        return copy(q_weight)
+
+    layer, same = _layer(seed=3), _layer(seed=3)
+    x = torch.randn(20, 500, device=DEV, dtype=torch.float16)
+    want = same(x)
+    torch.cuda.synchronize()
+    monkeypatch.setattr(linear, "aligned_rows", late)
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for s in streams:
+        with torch.cuda.stream(s):
+            got.append(layer(x))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want) for y in got)
