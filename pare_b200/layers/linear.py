@@ -50,13 +50,13 @@ from pare_b200.kernels.matmul_int8 import aligned_rows, w8a8_forward as _w8a8
 _FP8 = (QuantDtype.FP8_E4M3, QuantDtype.FP8_E5M2)
 
 
-def _version(t: Tensor) -> int:
-    return -1 if t.is_inference() else t._version
+def _versions(*tensors: Tensor | None) -> tuple:
+    return tuple([-1 if t is None or t.is_inference() else t._version for t in tensors])
 
 
 class QuantizedLinear(nn.Module):
     int8_kernel = False
-    _int8_made: tuple | None = None      # q_weight, scale and zero that the derived tensors were made from, and their versions
+    _int8_made: tuple | None = None      # q_weight, scale, zero and input_scale that the derived tensors were made from, and their versions
 
     def __init__(
         self,
@@ -202,7 +202,8 @@ class QuantizedLinear(nn.Module):
         x2d = x if len(shape) == 2 else x.reshape(-1, shape[-1])
         if dtype is not torch.float16 and dtype is not torch.bfloat16:
             x2d = x2d.to(torch.float16)
-        y = _w8a8(x2d, bufs["_q_weight_int8"], bufs["_scale_int8"], bufs["_zero_int8"], bias=self.bias, input_scale=bufs["input_scale"])
+        y = _w8a8(x2d, bufs["_q_weight_int8"], bufs["_scale_int8"], bufs["_zero_int8"], bias=self.bias,
+                  input_scale=bufs["_input_scale_int8"])
         if y.dtype is not dtype:
             y = y.to(dtype)
         return y if len(shape) == 2 else y.reshape(*shape[:-1], self.out_features)
@@ -211,19 +212,19 @@ class QuantizedLinear(nn.Module):
     # replaced or (by its version counter, which `.data` and tensors made under inference_mode bypass) written to.
     def _int8_buffers(self) -> dict:
         bufs, made = self._buffers, self._int8_made
-        q, s, z = bufs["q_weight"], bufs["scale"], bufs["zero"]
-        if made is None or made[0] is not q or made[1] is not s or made[2] is not z or made[3] != (_version(q), _version(s), _version(z)):
+        q, s, z, i = bufs["q_weight"], bufs["scale"], bufs["zero"], bufs["input_scale"]
+        if made is None or made[0] is not q or made[1] is not s or made[2] is not z or made[3] is not i or made[4] != _versions(q, s, z, i):
             self._prepare_int8_buffers()
         return bufs
 
     def _prepare_int8_buffers(self) -> None:
-        bufs, n, made = self._buffers, self.out_features, self._int8_made or (None, None, None)
-        q_weight, scale, zero = sources = self.q_weight, self.scale, self.zero
+        bufs, n, made = self._buffers, self.out_features, self._int8_made or (None, None, None, None)
+        q_weight, scale, zero, input_scale = sources = self.q_weight, self.scale, self.zero, self.input_scale
         if self.config.effective_dtype is not QuantDtype.INT8 or not self.quantize_inputs or self.g_idx is not None:
             raise ValueError("int8_kernel needs an INT8 layer with quantize_inputs and without g_idx")
         if scale.numel() not in (1, n) or zero.numel() not in (1, n):
             raise ValueError("int8_kernel needs one scale per output channel or per tensor (granularity per_channel or per_tensor)")
-        versions = _version(q_weight), _version(scale), _version(zero)
+        versions = _versions(*sources)
 
         def derived(name: str, now: Tensor, source: int) -> Tensor:
             # a tensor that was only written to: its derived one as well, where a captured graph reads it
@@ -235,7 +236,8 @@ class QuantizedLinear(nn.Module):
         zeros = zero.float().reshape(-1).expand(n).contiguous()
         new = {"_q_weight_int8": derived("_q_weight_int8", aligned_rows(q_weight), 0),
                "_scale_int8": derived("_scale_int8", scale.float().reshape(-1).expand(n).contiguous(), 1),
-               "_zero_int8": derived("_zero_int8", zeros, 2)}
+               "_zero_int8": derived("_zero_int8", zeros, 2),
+               "_input_scale_int8": None if input_scale is None else derived("_input_scale_int8", input_scale.float().contiguous(), 3)}
         # Reading whether there is a zero-point waits for this stream: the next call may come on another one, which knows nothing of the
         # copies.  They are in the layer's hands only then, another thread may be in a call.
         if not bool(zeros.any()) and (made[2] is not zero or bufs.get("_zero_int8") is None):
@@ -247,12 +249,12 @@ class QuantizedLinear(nn.Module):
     def _load_from_state_dict(self, *args, **kwargs) -> None:
         super()._load_from_state_dict(*args, **kwargs)
         if self._int8_made is not None:
-            self._int8_made = (*self._int8_made[:3], None)
+            self._int8_made = (*self._int8_made[:4], None)
 
     # The tensors move or change their type, and moving the derived ones would lose their rows' alignment.
     def _apply(self, *args, **kwargs):
         self._int8_made = None
-        for name in ("_q_weight_int8", "_scale_int8", "_zero_int8"):
+        for name in ("_q_weight_int8", "_scale_int8", "_zero_int8", "_input_scale_int8"):
             if name in self._buffers:
                 delattr(self, name)
         return super()._apply(*args, **kwargs)

@@ -135,3 +135,21 @@ def test_a_layer_that_two_streams_call_first(cuda_lib, monkeypatch):
             got.append(layer(x))
     torch.cuda.synchronize()
     assert all(torch.equal(y, want) for y in got)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 20])
+def test_a_smoothed_layer_in_a_16_bit_model(rows, dtype, cuda_lib):
+    """A cast of the module rounds input_scale too; the product then divides by the rounded one in float32, as the eager branch does."""
+    layer = _layer(512, input_scale=True)
+    x = torch.randn(rows, 512, device=DEV).to(dtype)
+    _as_defined(layer, x)
+    layer.to(dtype)
+    assert layer.input_scale.dtype is dtype
+    _as_defined(layer, x)
+    layer.input_scale.mul_(2.0)
+    _as_defined(layer, x)
+    layer.input_scale = (0.5 + torch.rand(1024, device=DEV))[::2]
+    _as_defined(layer, x)
+    layer.input_scale = None
+    _as_defined(layer, x)
