@@ -333,7 +333,7 @@ class PagedKVCache:
                               (c.max_requests, num_kv_heads, c.block_size, head_dim))
         self.layers = [PagedLayer(*(torch.empty(codes, dtype=torch.int8, device=device) for _ in range(2)),
                                   *(torch.zeros(scale, dtype=torch.float32, device=device) for _ in range(2)),
-                                  *(torch.empty(tail, dtype=dtype, device=device) for _ in range(2))) for _ in range(num_layers)]
+                                  *(torch.zeros(tail, dtype=dtype, device=device) for _ in range(2))) for _ in range(num_layers)]
         self.block_table = torch.zeros(c.max_requests, -(-c.max_seq_len // c.block_size), dtype=torch.int32, device=device)
         self._state = torch.zeros(c.max_requests + 1, dtype=torch.int32, device=device)    # lengths, then the number of free blocks
         self.seq_lens, self.free_count = self._state[:-1], self._state[-1:]

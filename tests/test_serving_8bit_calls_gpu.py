@@ -52,6 +52,17 @@ def test_probabilities_keep_more_than_the_result(h, group, d, new, dtype, cuda_l
     assert wrong <= total / 50 if dtype is torch.bfloat16 else wrong <= total / 10
 
 
+# ---- a cache's tensors --------------------------------------------------------------------------------------------------------------
+
+def test_a_new_cache_holds_numbers(cuda_lib):
+    """Copies and comparisons of a cache's tensors do not meet what other tensors left in their memory."""
+    shape = (4, 2, 16, 128)
+    left = [torch.full(shape, float("nan"), dtype=torch.float16, device=DEV) for _ in range(400)]
+    del left                                                # their memory is what the next small tensors get
+    layer = _cache(4, 2, 128, 16, torch.float16).layers[0]
+    assert layer.tail_k.shape == shape and all(t.eq(0).all() for t in layer[2:])
+
+
 # ---- integer layers -----------------------------------------------------------------------------------------------------------------
 
 def _layer(k=500, n=300, seed=0, sym=False, granularity="per_channel", input_scale=False):
