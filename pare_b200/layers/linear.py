@@ -29,8 +29,9 @@ Differences, all additive:
   (half the metadata traffic, scale rounded to 11 bits).
 * ``int8_kernel = True`` (with ``use_kernel``, on an INT8 layer with ``quantize_inputs``) multiplies the int8 activations and
   weights as integers on the tensor cores instead of fake-quantizing and multiplying in floats; per_channel and per_tensor
-  scales.  Off by default: the eager branch rounds the activations' step and the weights to the input dtype, the integer
-  product rounds neither, so the two differ by those roundings.
+  scales; float16 / bfloat16 activations (others take the eager branch).  Off by default: the eager branch rounds the
+  activations' step and the weights to the input dtype, the integer product rounds neither, so the two differ by those
+  roundings; and like the other kernels it computes no gradients.
 """
 
 from __future__ import annotations
@@ -125,7 +126,8 @@ class QuantizedLinear(nn.Module):
             and x.is_cuda
         ):
             return self._forward_kernel(x)
-        if self.int8_kernel and self.use_kernel and x.is_cuda:
+        # other types would lose range and bits on their way to 16
+        if self.int8_kernel and self.use_kernel and x.is_cuda and (x.dtype is torch.float16 or x.dtype is torch.bfloat16):
             return self._forward_int8(x)
 
         weight = self.dequantize().to(x.dtype)
@@ -198,14 +200,10 @@ class QuantizedLinear(nn.Module):
         return y if flat else y.reshape(*shape[:-1], self.out_features)
 
     def _forward_int8(self, x: Tensor) -> Tensor:
-        bufs, shape, dtype = self._int8_buffers(), x.shape, x.dtype
+        bufs, shape = self._int8_buffers(), x.shape
         x2d = x if len(shape) == 2 else x.reshape(-1, shape[-1])
-        if dtype is not torch.float16 and dtype is not torch.bfloat16:
-            x2d = x2d.to(torch.float16)
         y = _w8a8(x2d, bufs["_q_weight_int8"], bufs["_scale_int8"], bufs["_zero_int8"], bias=self.bias,
                   input_scale=bufs["_input_scale_int8"])
-        if y.dtype is not dtype:
-            y = y.to(dtype)
         return y if len(shape) == 2 else y.reshape(*shape[:-1], self.out_features)
 
     # The integer product's derived, non-persistent tensors follow what they were made from: each call looks whether that has been

@@ -164,3 +164,17 @@ def test_a_smoothed_layer_in_a_16_bit_model(rows, dtype, cuda_lib):
     _as_defined(layer, x)
     layer.input_scale = None
     _as_defined(layer, x)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+def test_activations_of_more_than_16_bits_stay_what_they_are(dtype, cuda_lib):
+    layer = _layer(512, input_scale=True)
+    x = torch.randn(4, 512, device=DEV, dtype=dtype)
+    x[1, 7], x[2] = 3e5, x[2] * 1e-9                        # beyond float16, on either side
+    layer.int8_kernel = False
+    if dtype is torch.float64:
+        layer.double()
+    want = layer(x)
+    layer.int8_kernel = True
+    y = layer(x)
+    assert y.dtype is dtype and bool(y.isfinite().all()) and torch.equal(y, want)
