@@ -102,12 +102,13 @@ def _step_layout(requests: int, tokens: int, block_size: int) -> tuple[int, tupl
 class PagedStep:
     """Tables of one step (made by :func:`plan_blocks`); the properties are views of one buffer on the GPU."""
 
-    __slots__ = ("words", "requests", "tokens", "block_size", "block_table", "device", "lengths", "_at", "_ld", "_struct", "_c")
+    __slots__ = ("words", "requests", "tokens", "block_size", "block_table", "device", "lengths", "written_once", "_at", "_ld", "_struct", "_c")
 
     def __init__(self, words: Tensor, at: tuple[int, ...], requests: int, tokens: int, block_size: int, block_table: Tensor, ld: int) -> None:
         self.words, self._at, self.device = words, at, words.device
         self.requests, self.tokens, self.block_size, self.block_table, self._ld = requests, tokens, block_size, block_table, ld
         self.lengths: list[tuple[int, int]] | None = None    # (old, new) per request where the host knows them
+        self.written_once = False      # True: no graph writes the step again, so lengths that were read from it stay true
         self._c = 0
 
     def _tables(self) -> int:
@@ -369,8 +370,10 @@ class PagedKVCache:
         if isinstance(new_lens, Tensor):
             if tokens is None:
                 raise ValueError("plan: the number of rows is needed when lengths are on the GPU")
-            self._captured |= torch.cuda.is_current_stream_capturing()
+            captured = torch.cuda.is_current_stream_capturing()
+            self._captured |= captured
         else:
+            captured = False      # a copy from the host cannot be captured
             if isinstance(new_lens, dict):
                 if any(not 0 <= r < c.max_requests for r in new_lens):
                     raise ValueError(f"plan: requests are numbered 0 to {c.max_requests - 1}")
@@ -395,7 +398,7 @@ class PagedKVCache:
             new_lens = torch.tensor(new, dtype=torch.int32).to(self.device)
         step = plan_blocks(self.seq_lens, new_lens, self.block_table, self.free_blocks, self.free_count, c.block_size, tokens)
         self._state.copy_(step.words.narrow(0, step._at[2], c.max_requests + 1))
-        step.lengths = lengths
+        step.lengths, step.written_once = lengths, not captured
         self._lens = None if lengths is None else [a + n for a, n in lengths]
         return step
 
@@ -436,23 +439,26 @@ class PagedKVCache:
         """Causal attention of prompts' queries ``[tokens, Hq, D]`` with the step's own keys and values at full precision, older
         tokens as the cache holds them, and the append (``head_dim`` 128; what ``QuantizedKVCache.prefill`` does, request by
         request on the prompt attention kernel).  The host needs the lengths: where they were given as tensors it waits for
-        them."""
+        them, once for a step, but in every call where the step was planned in a graph that may have been replayed since."""
         layer = self.layers[layer_idx]
         if layer.head_dim != 128:
             raise ValueError("prefill needs head_dim 128: use attend")
         q = _rows(q, step.tokens, q.shape[1] if q.dim() == 3 else 0, layer, "q")[0]
-        if step.lengths is None:
+        lengths = step.lengths
+        if lengths is None:
             step.check()
             start, end = step.query_start.tolist(), step.seq_lens.tolist()
-            step.lengths = [(e - (b - a), b - a) for e, a, b in zip(end, start, start[1:])]
+            lengths = [(e - (b - a), b - a) for e, a, b in zip(end, start, start[1:])]
+            if step.written_once:
+                step.lengths = lengths
         append_blocks(layer, step, new_k, new_v)
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         full_k = full_v = None
-        if any(old and new for old, new in step.lengths):
-            full_k, full_v = dense_blocks(layer, step, sum(old + new for old, new in step.lengths if new))
+        if any(old and new for old, new in lengths):
+            full_k, full_v = dense_blocks(layer, step, sum(old + new for old, new in lengths if new))
         row = ctx = 0
         with torch.cuda.device(self.device):
-            for old, new in step.lengths:
+            for old, new in lengths:
                 if not new:
                     continue
                 k, v = new_k[row:row + new], new_v[row:row + new]

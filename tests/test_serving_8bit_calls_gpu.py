@@ -63,6 +63,66 @@ def test_a_new_cache_holds_numbers(cuda_lib):
     assert layer.tail_k.shape == shape and all(t.eq(0).all() for t in layer[2:])
 
 
+# ---- steps that a graph writes again ------------------------------------------------------------------------------------------------
+
+def _prompt(q, k, v):
+    """Causal attention of a prompt's rows ``[n, heads, d]`` among themselves in 64 bits, and the bound of a 16-bit result's error."""
+    qq, kk, vv = (x.double().transpose(0, 1) for x in (q, k, v))
+    n, group = q.shape[0], q.shape[1] // k.shape[1]
+    s = qq @ kk.repeat_interleave(group, 0).transpose(1, 2) / math.sqrt(q.shape[2])
+    s = s.masked_fill(torch.ones(n, n, device=DEV, dtype=torch.bool).triu(1), float("-inf"))
+    want = (torch.softmax(s, -1) @ vv.repeat_interleave(group, 0)).transpose(0, 1)
+    # half a step of the result, and as much again of the largest value for the probabilities' rounding
+    return want, torch.finfo(q.dtype).eps / 2 * (want.abs() + vv.abs().max())
+
+
+@pytest.mark.parametrize("planned_by", ["class", "function"])
+def test_prefill_after_replays_of_a_captured_plan(planned_by, cuda_lib):
+    """Every replay gives the step other lengths; prefill has to go by those of the last one."""
+    cache = _cache(3, 2, 128, 16, torch.float16, blocks=100, layers=2)
+    new = torch.tensor([20, 0, 3], dtype=torch.int32, device=DEV)
+    rows = 40
+
+    def plan():
+        if planned_by == "class":
+            return cache.plan(new, tokens=rows)
+        return pc.plan_blocks(cache.seq_lens, new, cache.block_table, cache.free_blocks, cache.free_count, 16, rows)
+
+    plan()
+    cache.reset()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step = plan()
+    for i, lens in enumerate(([20, 0, 3], [5, 30, 2], [0, 0, 40], [40, 0, 0], [1, 1, 1])):
+        cache.reset()
+        new.copy_(torch.tensor(lens, dtype=torch.int32))
+        graph.replay()
+        for layer in range(2):
+            q, k, v = (_rand((rows, n, 128), 100 * i + 10 * layer + n, torch.float16) for n in (8, 2, 1))
+            v = v.expand(rows, 2, 128)
+            out = cache.prefill(layer, step, q, k, v)
+            at = 0
+            for n in lens:
+                if n:
+                    want, bound = _prompt(q[at:at + n], k[at:at + n], v[at:at + n])
+                    assert bool(((out[at:at + n].double() - want).abs() <= bound).all()), (i, layer, n)
+                at += n
+    new.copy_(torch.tensor([41, 0, 0], dtype=torch.int32))
+    graph.replay()
+    with pytest.raises(RuntimeError, match="refused"):
+        cache.prefill(0, step, q, k, v)
+
+
+def test_prefill_reads_an_eager_step_once(cuda_lib):
+    cache = _cache(2, 2, 128, 16, torch.float16, blocks=20, layers=2)
+    step = cache.plan(torch.tensor([5, 0], dtype=torch.int32, device=DEV), tokens=5)
+    q = _rand((5, 2, 128), 1, torch.float16)
+    assert step.lengths is None
+    cache.prefill(0, step, q, q, q)
+    assert step.lengths == [(0, 5), (0, 0)]
+
+
 # ---- integer layers -----------------------------------------------------------------------------------------------------------------
 
 def _layer(k=500, n=300, seed=0, sym=False, granularity="per_channel", input_scale=False):
