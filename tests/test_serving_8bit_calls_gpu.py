@@ -9,7 +9,7 @@ import torch.nn as nn
 
 from pare_b200 import QuantConfig, QuantizedLinear
 from pare_b200 import paged_cache as pc
-from test_paged_gpu import _cache, _feed, _Model, _rand
+from test_paged_gpu import _cache, _check_attend, _feed, _Model, _rand
 from test_w8a8_gpu import _check as _check_linear
 
 pytestmark = pytest.mark.gpu
@@ -121,6 +121,48 @@ def test_prefill_reads_an_eager_step_once(cuda_lib):
     assert step.lengths is None
     cache.prefill(0, step, q, q, q)
     assert step.lengths == [(0, 5), (0, 0)]
+
+
+# ---- refusals half way --------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("call", ["attend", "prefill"])
+def test_a_refused_call_has_stored_nothing(call, cuda_lib):
+    """A block fills up and the rows behind it are written again: what a refused call had stored could not be stored a second time."""
+    cache, model = _cache(2, 2, 128, 16, torch.float16, blocks=100), _Model(2, 2, 128, 16, torch.float16)
+    _feed(cache, model, [10, 3], 1)
+    new = [30, 1]
+    step = cache.plan(new)
+    q, k, v = (_rand((31, n, 128), 5 + n, torch.float16) for n in (8, 2, 1))
+    v = v.expand(31, 2, 128).contiguous()
+    before = [t.clone() for t in cache.layers[0]]
+    go = getattr(cache, call)
+    bad_out = [] if call == "prefill" else [lambda: go(0, step, q, k, v, out=q.transpose(1, 2).contiguous().transpose(1, 2)),
+                                            lambda: go(0, step, q, k, v, out=q.float())]
+    for refused in (lambda: go(0, step, q[:, :7], k, v), lambda: go(0, step, q[:, :0], k, v), lambda: go(0, step, q[:30], k, v),
+                    lambda: go(0, step, q.float(), k, v), lambda: go(0, step, q, k[:30], v), lambda: go(0, step, q, k, v[:, :1]),
+                    lambda: go(0, step, q, k, v, scale="?"), *bad_out):
+        with pytest.raises((ValueError, IndexError)):
+            refused()
+        assert all(torch.equal(a, b) for a, b in zip(before, cache.layers[0]))
+    out = go(0, step, q, k, v)
+    model.add(0, k[:30], v[:30])
+    model.add(1, k[30:], v[30:])
+    if call == "attend":
+        _check_attend(model, step, new, q, out)
+    for r in range(2):
+        n = model.k[r].shape[1] // 16
+        ids = cache.block_table[r, :n].long()
+        assert torch.equal(cache.layers[0].k_codes[ids].transpose(0, 1).float(), model.blocks(model.k[r])[0])
+
+
+def test_too_many_rows_for_attention_are_not_stored(cuda_lib):
+    cache = _cache(1, 1, 64, 16, torch.float16, blocks=300, max_len=4800)
+    step = cache.plan([4097])
+    q, k = torch.ones(4097, 1, 64, dtype=torch.float16, device=DEV), torch.ones(4097, 1, 64, dtype=torch.float16, device=DEV)
+    before = [t.clone() for t in cache.layers[0]]
+    with pytest.raises(ValueError, match="at most 4096"):
+        cache.attend(0, step, q, k, k)
+    assert all(torch.equal(a, b) for a, b in zip(before, cache.layers[0]))
 
 
 # ---- integer layers -----------------------------------------------------------------------------------------------------------------
