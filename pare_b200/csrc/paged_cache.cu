@@ -384,6 +384,14 @@ struct DenseParams {
   int R, H, bs_log2, num_blocks, max_blocks;
 };
 
+// Sixteen codes.  Not the read-only path (.nc): that asks for data which nobody writes while the kernel lives, and this one is launched
+// while the append before it still writes codes.
+__device__ __forceinline__ uint4 ld_codes16(const int8_t* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
+
 // sixteen codes times their scale, rounded
 template <typename T>
 __device__ __forceinline__ void scaled16(const uint4& c, float s, uint4 (&out)[2]) {
@@ -438,8 +446,8 @@ __global__ void __launch_bounds__(kDenseThreads) paged_dense_kernel(const DenseP
       const long long w = __shfl_sync(0xffffffffu, where, i);
       const int block = __shfl_sync(0xffffffffu, id, i);
       if (inside && i < tokens && w >= 0 && w < kNothing) {
-        ck[i] = ld_stream_v4(p.k_codes + w * D + skip);
-        cv[i] = ld_stream_v4(p.v_codes + w * D + skip);
+        ck[i] = ld_codes16(p.k_codes + w * D + skip);
+        cv[i] = ld_codes16(p.v_codes + w * D + skip);
         sk[i] = p.k_scale[(int64_t)block * p.H + h];
         sv[i] = p.v_scale[(int64_t)block * p.H + h];
       }
