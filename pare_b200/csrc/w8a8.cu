@@ -1056,7 +1056,8 @@ int pare_w8a8_forward(const void* x, int x_dtype, int64_t ldx, const int8_t* wei
     constexpr bool kS = decltype(scaled)::value;
     auto go = [&](auto kern, int threads) -> int {
       const size_t row = vec ? (size_t)K * 2 : 0;
-      if (row > 48 * 1024 && !ensure_smem_attr(reinterpret_cast<const void*>(kern), kMaxK * 2)) return PARE_ERR_CUDA;
+      // 48 KB without asking, static shared memory (256 bytes at most) among them
+      if (row > 47 * 1024 && !ensure_smem_attr(reinterpret_cast<const void*>(kern), kMaxK * 2)) return PARE_ERR_CUDA;
       return launch_pdl(kern, dim3(M), dim3(threads), row, st, q);
     };
     if (!vec) return go(w8a8_quantize_kernel<E, 512, false, kS>, 512);

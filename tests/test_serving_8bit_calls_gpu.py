@@ -9,6 +9,7 @@ import torch.nn as nn
 
 from pare_b200 import QuantConfig, QuantizedLinear
 from pare_b200 import paged_cache as pc
+from pare_b200.kernels import w8a8_forward
 from test_paged_gpu import _cache, _check_attend, _feed, _Model, _rand
 from test_w8a8_gpu import _check as _check_linear
 
@@ -280,3 +281,18 @@ def test_activations_of_more_than_16_bits_stay_what_they_are(dtype, cuda_lib):
     layer.int8_kernel = True
     y = layer(x)
     assert y.dtype is dtype and bool(y.isfinite().all()) and torch.equal(y, want)
+
+
+# ---- linear -------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("k", [24064, 24072, 24448, 24456, 24560, 24568, 24576, 24584])
+@pytest.mark.parametrize("m", [12, 300, 600, 1300])
+def test_rows_of_about_48_kilobytes(m, k, dtype, cuda_lib):
+    """A row waits in shared memory between maximum and codes: beside it there is the kernel's static shared memory."""
+    g = torch.Generator(device=DEV).manual_seed(m + k)
+    x = torch.randn(m, k, device=DEV, generator=g).to(dtype)
+    w = torch.randint(-128, 128, (130, k), device=DEV, generator=g, dtype=torch.int8)
+    scale, ins = torch.rand(130, device=DEV, generator=g) * 1e-3, 0.5 + torch.rand(k, device=DEV, generator=g)
+    _check_linear(w8a8_forward(x, w, scale), x, w, scale)
+    _check_linear(w8a8_forward(x, w, scale, input_scale=ins), x, w, scale, None, None, ins)
