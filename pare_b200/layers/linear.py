@@ -211,7 +211,8 @@ class QuantizedLinear(nn.Module):
     def _int8_buffers(self) -> dict:
         bufs, made = self._buffers, self._int8_made
         q, s, z, i = bufs["q_weight"], bufs["scale"], bufs["zero"], bufs["input_scale"]
-        if made is None or made[0] is not q or made[1] is not s or made[2] is not z or made[3] is not i or made[4] != _versions(q, s, z, i):
+        if (made is None or made[0] is not q or made[1] is not s or made[2] is not z or made[3] is not i or made[4] != _versions(q, s, z, i)
+                or not self.quantize_inputs or bufs["g_idx"] is not None):
             self._prepare_int8_buffers()
         return bufs
 

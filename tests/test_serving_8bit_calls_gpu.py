@@ -283,6 +283,20 @@ def test_activations_of_more_than_16_bits_stay_what_they_are(dtype, cuda_lib):
     assert y.dtype is dtype and bool(y.isfinite().all()) and torch.equal(y, want)
 
 
+def test_layer_refuses_what_it_was_changed_to(cuda_lib):
+    """A layer that has run and then stops quantizing its inputs, or gets an order of columns, is not the integer product's any more."""
+    layer, x = _layer(), torch.randn(3, 500, device=DEV, dtype=torch.float16)
+    _as_defined(layer, x)
+    layer.quantize_inputs = False
+    with pytest.raises(ValueError, match="int8_kernel needs"):
+        layer(x)
+    layer.quantize_inputs = True
+    _as_defined(layer, x)
+    layer.g_idx = torch.arange(500, dtype=torch.int32, device=DEV)
+    with pytest.raises(ValueError, match="int8_kernel needs"):
+        layer(x)
+
+
 # ---- linear -------------------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
