@@ -250,13 +250,17 @@ class QuantizedLinear(nn.Module):
         if self._int8_made is not None:
             self._int8_made = (*self._int8_made[:4], None)
 
-    # The tensors move or change their type, and moving the derived ones would lose their rows' alignment.
+    # Where the tensors move or change their type the derived ones are made again (moving them would lose their rows' alignment); where
+    # nothing does they stay, for graphs that read them.
     def _apply(self, *args, **kwargs):
+        made, bufs = self._int8_made, self._buffers
+        derived = {name: bufs.pop(name) for name in ("_q_weight_int8", "_scale_int8", "_zero_int8", "_input_scale_int8") if name in bufs}
         self._int8_made = None
-        for name in ("_q_weight_int8", "_scale_int8", "_zero_int8", "_input_scale_int8"):
-            if name in self._buffers:
-                delattr(self, name)
-        return super()._apply(*args, **kwargs)
+        super()._apply(*args, **kwargs)
+        if made is not None and all(bufs[name] is t for name, t in zip(("q_weight", "scale", "zero", "input_scale"), made)):
+            bufs.update(derived)
+            self._int8_made = made
+        return self
 
     def supports_prepared(self, rows: int) -> bool:
         """True if :meth:`forward_prepared` can serve ``rows`` activation rows of this layer."""

@@ -228,6 +228,29 @@ def test_a_captured_layer_follows_a_loaded_state(cuda_lib):
     assert torch.equal(y, want) and torch.equal(want, other(x))
 
 
+def test_a_captured_layer_stays_where_a_move_moves_nothing(cuda_lib):
+    layer = _layer(input_scale=True)
+    x = torch.randn(20, 500, device=DEV, dtype=torch.float16)
+    want = _as_defined(layer, x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = layer(x)
+    names = ("_q_weight_int8", "_scale_int8", "_zero_int8", "_input_scale_int8")
+    read = [layer._buffers[name] for name in names]
+    for move in (lambda: layer.cuda(), lambda: layer.to(DEV), lambda: layer.to(torch.float32)):
+        assert move() is layer
+        assert all(layer._buffers[name] is t for name, t in zip(names, read))
+    y.zero_()
+    graph.replay()
+    assert torch.equal(y, want) and torch.equal(layer(x), want)
+    keys = set(layer.state_dict())
+    layer.half()
+    assert not any(name in layer._buffers for name in names) and set(layer.state_dict()) == keys
+    _as_defined(layer, x)
+    assert set(layer.state_dict()) == keys
+
+
 def test_a_layer_that_two_streams_call_first(cuda_lib, monkeypatch):
     """The first call makes the derived tensors on its stream; the next one, on another stream, finds them made."""
     from pare_b200.layers import linear
