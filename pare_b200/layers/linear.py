@@ -230,7 +230,8 @@ class QuantizedLinear(nn.Module):
             old = bufs.get(name) if made[source] is sources[source] else None
             if old is None or old.data_ptr() == now.data_ptr():
                 return now if old is None else old
-            return old.copy_(now)
+            with torch.inference_mode():      # it may have been made in that mode
+                return old.copy_(now)
 
         zeros = zero.float().reshape(-1).expand(n).contiguous()
         new = {"_q_weight_int8": derived("_q_weight_int8", aligned_rows(q_weight), 0),

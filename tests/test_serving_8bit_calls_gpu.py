@@ -228,6 +228,18 @@ def test_a_captured_layer_follows_a_loaded_state(cuda_lib):
     assert torch.equal(y, want) and torch.equal(want, other(x))
 
 
+@pytest.mark.parametrize("first", [torch.inference_mode, torch.no_grad])
+@pytest.mark.parametrize("then", [torch.inference_mode, torch.no_grad, torch.enable_grad])
+def test_layer_follows_a_loaded_state_across_modes(first, then, cuda_lib):
+    layer, other = _layer(granularity="per_tensor", seed=1, input_scale=True), _layer(granularity="per_tensor", seed=2, input_scale=True)
+    x = torch.randn(5, 500, device=DEV, dtype=torch.float16)
+    with first():
+        _as_defined(layer, x)
+    layer.load_state_dict(other.state_dict())
+    with then():
+        assert torch.equal(_as_defined(layer, x), other(x))
+
+
 def test_a_captured_layer_stays_where_a_move_moves_nothing(cuda_lib):
     layer = _layer(input_scale=True)
     x = torch.randn(20, 500, device=DEV, dtype=torch.float16)
