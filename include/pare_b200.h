@@ -373,7 +373,8 @@ int pare_paged_release(const int32_t* release, int32_t* seq_lens, int R, const i
                        int32_t* free_blocks, int free_capacity, int32_t* free_count, int block_size, void* stream);
 
 /* The step's new keys and values [T][H][D] (element strides, multiples of 8; channels contiguous; 16-byte aligned) into one layer.
- * Ids that are not in the pool are not written to. */
+ * Ids that are not in the pool are not written to.  Once per step and layer: where a block fills up, its open rows are written over by
+ * the tokens behind it. */
 int pare_paged_append(const void* k, const void* v, int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h,
                       const pare_paged_layer* layer, const pare_paged_tables* tables, void* stream);
 
@@ -382,7 +383,7 @@ int pare_paged_append(const void* k, const void* v, int64_t k_stride_t, int64_t 
 int pare_paged_dense(const pare_paged_layer* layer, const pare_paged_tables* tables, void* out_k, void* out_v, int64_t total, void* stream);
 
 /* Attention of the step's tokens over the layer, after the step's append: token t of request r attends to the positions up to its
- * own.  q, out [T][Hq][D] (element strides; q's multiples of 8, 16-byte aligned), query head hq reads KV head hq / (Hq / H), any
+ * own, as they are stored now: a block that the step filled up in 8 bits, for its earlier tokens too.  q, out [T][Hq][D] (element strides; q's multiples of 8, 16-byte aligned), query head hq reads KV head hq / (Hq / H), any
  * ratio; T <= 4096 and T * (max_blocks * block_size / 16 + 2) < 2^31 (a 32-bit count of work).  Rows that belong to nobody are left as they were.  Ids not in the pool read as NaN.  The workspace
  * (16-byte aligned, pare_paged_attn_workspace_bytes()) need not be initialised and holds nothing between calls. */
 size_t pare_paged_attn_workspace_bytes(int D);

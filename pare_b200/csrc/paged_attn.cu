@@ -7,11 +7,11 @@
 //
 // Mathematics.  Codes are integers of at most 127: exact in fp16, so S = code . q and O' = code^T . P run on fp16 operands with fp32
 // sums, and the block's scales multiply S and O' outside (one number per 16 tokens).  q is fp16 as it is, or bf16 times a power of
-// two per head that puts its largest magnitude into [256, 512): every bf16 value within 2^-22 of that is exact, smaller ones are
-// within 2^-34 of the largest.  Softmax runs online: a reference value per head which only moves when a score passes it by more than
-// 2^kSlack (one vote per 16 tokens instead of a reduction); probabilities are kept times 2^kBias of that, so those down to 2^-18 of
-// the reference are normal fp16 numbers and none passes 2^15.  Their sum is taken before they become two fp16 numbers each (those of
-// open rows two of the rows' type).
+// two per head that puts its largest magnitude into [256, 512), where that is 2^-112 or more: every bf16 value within 2^-22 of that is
+// exact, smaller ones are within 2^-33 of the largest.  Softmax runs online: a reference value per head which only moves when a score
+// passes it by more than 2^kSlack (one vote per 16 tokens instead of a reduction); probabilities are kept times 2^kBias of that, so those
+// down to 2^-18 of the reference are normal fp16 numbers and none passes 2^15.  Their sum is taken before they become two fp16 numbers
+// each (those of open rows two of the rows' type).  Values above 2^112 / tokens may overflow the sums.
 //
 // Work.  Units of 16 tokens of one (token, group of heads), counted by the step's tables; each WARP takes one contiguous run of
 // units, all runs equally long, so ragged lengths balance by themselves and the host needs to know none of them.  A warp feeds
@@ -21,10 +21,10 @@
 //
 // A tile's eight columns are heads of one token, or, where a step has more rows than requests, heads of up to eight tokens of a request.
 //
-// Bound: the cache's bytes for long contexts, instructions (conversion of codes, 0.6 - 0.7 of the issue slots) close behind, and 7 us that
-// the second launch takes after the last warp; one sequence is a chain of dependent reads.  Both launches: 16 x 32768 tokens, 28 / 4 heads, fp16
-// 100 us (540 MB: 0.82 of the copy rate; the first launch alone 96); 64 requests of up to 3600 tokens, 32 / 8 heads, bf16 59 us (0.68); one of
-// 4096 tokens 11.8 us; three tokens of 12 requests over 1500 on average, D = 64 19.3 us.
+// Bound: the cache's bytes for long contexts, instructions (conversion of codes: 0.61 of the issue slots there, 0.50 for ragged requests) close
+// behind; one sequence is a chain of dependent reads.  Both launches, of many in a graph, and how much of that the second one adds:
+// 16 x 32768 tokens, 28 / 4 heads 100 us (540 MB: 0.82 of the copy rate), 8; 64 requests of up to 3600 tokens, 32 / 8 heads, bf16 62 us (0.65), 7;
+// one of 4096 tokens 13.3 us, 4.7; three tokens of 12 requests over 1500 on average, D = 64 20.4 us, 6.4.
 #include <algorithm>
 #include <type_traits>
 
@@ -579,10 +579,11 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocksPerSm) pa
 }
 
 // Tiles that span warps.  A warp takes one piece of a tile's O (float4 per lane as the attention's lanes held it: channels
-// (D / 8) g + 2 i, + 1 x heads 2 t, 2 t + 1).  Many tiles have few parts each: a thread block per tile, a warp per piece.  Few tiles have
+// (D / 8) g + 2 i, + 1 x heads 2 t, 2 t + 1).  Many tiles have few parts each, or most of them (one
+// far longer than the others is added up by one warp a piece): a thread block per tile, a warp per piece.  Few tiles have
 // many (one sequence: 86): GROUPS warps share a piece, each every GROUPS-th part, and are added up in order.  A warp alone gets
 // through one instruction in about eight cycles, so what is serial counts: 8 tiles of 4096 tokens, both kernels, 22.7 / 15.8 / 13.1 / 12.7 us
-// with 2 / 4 / 8 / 16 groups (11.8 now: six parts in flight, the step read before the wait, which saves 0.8 us everywhere); 64 tiles of 32768
+// with 2 / 4 / 8 / 16 groups (six parts in flight and the step read before the wait have saved another 0.8 us since); 64 tiles of 32768
 // tokens 101 / 99 / 99 / 106 us, 108 with one.
 template <typename T, int D, int GROUPS, bool PACKED>
 __global__ void __launch_bounds__(GROUPS > 1 ? GROUPS * 32 : D * 2) paged_merge_kernel(const PagedAttnParams p, int warps) {

@@ -284,8 +284,9 @@ __global__ void __launch_bounds__(kPlanThreads) paged_release_kernel(const int* 
 // A team of threads takes one (touched block of tokens, head) of the keys or of the values.  A block that fills up is held in registers
 // between the maximum and the codes, so its tokens are read once.  Four threads per token (32 values each, all loads in flight at
 // once) where eight per token would take several rounds of the SMs, else eight: 32768 tokens of 4 heads 25.6 us against 34, but 2056 tokens of 8
-// heads 8.7 against 6.2 (two threads per token: 26.7; with cheaper codes since then 22.0 and 5.1).  Bound: bytes, 15.4 us for the
-// first; a decode step of one request 1.2 us.
+// heads 8.7 against 6.2 (two threads per token: 26.7; with cheaper codes since then 23.0 and 5.1).  Bytes would take 15.4 us for the
+// first; it fills 55 % of the issue slots and 32 % of DRAM's rate with 44 % of the warps an SM holds (62 registers hold the block).  A decode step
+// of one request 1.3 us.
 __host__ __device__ constexpr int append_threads(int team) { return team > 256 ? team : 256; }
 
 struct AppendParams {

@@ -60,8 +60,9 @@ __device__ __forceinline__ uint32_t magnitude(T v) {   // orders like |v|, infin
 
 // A row per thread block; where rows allow 16-byte pieces (VEC) it waits in shared memory between the maximum and the codes (and is divided
 // by input_scale once: SCALED), all of it on its way at the same time and no registers held, so that as many rows as possible are
-// resident.  Others are read twice.  Bound: the codes' arithmetic.  2048 rows of 4096 6.8 us (bytes: 3.8), 1024 of 14336 9.1 (6.7), 333 of 18944
-// 5.9 and with input_scale 10.4 (2.9; rows held in registers, fewer of them at once: 12 and 18).
+// resident (32 registers, without smoothing 16 bytes of them in local memory).  Others are read twice.  Neither DRAM (20 %) nor the issue
+// slots (40 %) are full; the codes' arithmetic counts most (cheaper codes halved the time).  2048 rows of 4096 6.8 us (bytes: 3.8), 1024 of
+// 14336 9.1 (6.7), 333 of 18944 5.9 and with input_scale 10.4 (2.9; rows held in registers, fewer of them at once: 12 and 18).
 template <typename T, int THREADS, bool VEC, bool SCALED>
 __global__ void __launch_bounds__(THREADS, (SCALED ? 1536 : 2048) / THREADS) w8a8_quantize_kernel(const QuantParams p) {
   pdl_wait();
@@ -914,7 +915,7 @@ struct W8Plan {
 // Height of the activation tiles (equal, a multiple of 32) and whether two or four pairs of SMs split K, by an estimate in microseconds: rounds of
 // all pairs x units x what a unit of that height takes (0.21 at 32 rows, 0.36 at 256), the weights' way from memory as a lower
 // bound, and what a split adds.  Within a few per cent of the best of 8 heights x 2 splits for 23 shapes of 17 - 3000 rows; four pairs, where
-// all their clusters fit the device at once (not 16 of them): 17 rows of 512 x 18944 16.3 us against 22.7, of 3584 x 18944 19.1 against 24.1.
+// all their clusters fit the device at once (not 16 of them): 17 rows of 512 x 18944 15.5 us against 22.7, of 3584 x 18944 18.9 against 24.1.
 W8Plan w8_plan(int M, int N, int K) {
   W8Plan best{};
   double least = 1e30;

@@ -31,7 +31,8 @@ Differences, all additive:
   weights as integers on the tensor cores instead of fake-quantizing and multiplying in floats; per_channel and per_tensor
   scales; float16 / bfloat16 activations (others take the eager branch).  Off by default: the eager branch rounds the
   activations' step and the weights to the input dtype, the integer product rounds neither, so the two differ by those
-  roundings; and like the other kernels it computes no gradients.
+  roundings; and like the other kernels it computes no gradients.  ``load_quantized(use_kernel=True)`` leaves it off: set it on
+  the loaded layers.
 """
 
 from __future__ import annotations

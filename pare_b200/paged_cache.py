@@ -5,7 +5,8 @@ sequences all have the same length.  A server's requests start and end at their 
 tokens is shared by up to ``max_requests`` of them through a block table.  A block holds int8 codes with one scale per head for its
 keys and one for its values; it is quantized once, when its last token arrives.  Until then the tokens stay in the input type
 (``tail_k`` / ``tail_v``), so what is stored does not depend on how the tokens were cut into calls, as with the reference's
-residual window.  An infinity or NaN in a block makes that head's whole block NaN once it is quantized.
+residual window.  An infinity or NaN in a block makes that head's whole block NaN once it is quantized; a query that sees one in
+an open row gets no finite result.
 
 Three functions work on plain tensors, and :class:`PagedKVCache` keeps those tensors for all layers of a model:
 
@@ -13,7 +14,12 @@ Three functions work on plain tensors, and :class:`PagedKVCache` keeps those ten
   token goes, which blocks are taken.  One step serves every layer.
 * :func:`append_blocks` stores a step's new keys and values in one layer, :func:`dense_blocks` gives whole sequences back.
 * :func:`attend_blocks` is the attention of the step's queries over the layer: one new token per request (decode) or several
-  (drafted tokens, short prompts), causal.
+  (short prompts, continuations), causal by position.
+
+A step's tokens stay: there is no way to take some of them back (drafted tokens that a check rejects, say), for a block that they
+filled up has been quantized with them, and its open rows hold the tokens behind it.  And attention reads what is stored: where a block
+fills up inside a step, the step's earlier tokens see their own block in 8 bits too, with a scale that the later ones had a part in (an
+infinity among those reaches them).  Fed one by one they would have seen it in 16 bits.
 
 Nothing here computes gradients, and everything runs on CUDA tensors only.
 """
@@ -235,7 +241,8 @@ def _rows(t: Tensor, tokens: int, heads: int, layer: PagedLayer, what: str) -> t
 
 def append_blocks(layer: PagedLayer, step: PagedStep, k: Tensor, v: Tensor) -> None:
     """Store the step's new keys and values ``[tokens, H, D]`` in one layer: blocks that fill up are quantized into the pool, the
-    rest goes to the open rows."""
+    rest goes to the open rows.  Once per step and layer: a block that filled up had its open rows written over by the tokens behind it,
+    so the same call again would quantize it from those."""
     _fits(layer, step)
     tokens, heads, dev = step.tokens, layer.heads, layer.device
     k, kp, kt, kh = _rows(k, tokens, heads, layer, "k")
@@ -270,7 +277,7 @@ def attend_blocks(layer: PagedLayer, step: PagedStep, q: Tensor, scale: float | 
     (the step's keys and values have been appended).  ``Hq`` is a multiple of the KV heads; default scale ``1 / sqrt(D)``.  At most
     4096 rows: longer prompts go through :meth:`PagedKVCache.prefill` (and rows times tokens of a full row of the block table stay
     below 2^35).  Rows that belong to nobody are left as they were in
-    ``out`` (``[tokens, Hq, D]``, channels adjacent, not overlapping ``q``; a new tensor if not given)."""
+    ``out`` (``[tokens, Hq, D]``, channels adjacent, not overlapping ``q``; a new tensor, with anything in those rows, if not given)."""
     call = _attend_arguments(layer, step, q, scale, out)
     return _attend(layer, step, *call)
 
@@ -313,7 +320,7 @@ def _attend(layer: PagedLayer, step: PagedStep, q: Tensor, qp: int, qt: int, qh:
 @dataclass
 class PagedKVConfig:
     """``num_blocks`` blocks of ``block_size`` (16, 32 or 64) tokens in the pool, up to ``max_requests`` requests of up to
-    ``max_seq_len`` tokens."""
+    ``max_seq_len`` tokens (to the end of the last block where the GPU alone knows the lengths)."""
 
     num_blocks: int
     block_size: int = 32
@@ -442,7 +449,8 @@ class PagedKVCache:
 
     def attend(self, layer_idx: int, step: PagedStep, q: Tensor, new_k: Tensor, new_v: Tensor, scale: float | None = None,
                out: Tensor | None = None) -> Tensor:
-        """Append the step's keys and values, then attention of its queries over the whole requests (:func:`attend_blocks`)."""
+        """Append the step's keys and values, then attention of its queries over the whole requests (:func:`attend_blocks`).  Once per
+        step and layer; a call that is refused has stored nothing."""
         layer = self.layers[layer_idx]
         call = _attend_arguments(layer, step, q, scale, out)      # first: what is refused has not been stored either
         append_blocks(layer, step, new_k, new_v)
@@ -452,7 +460,8 @@ class PagedKVCache:
         """Causal attention of prompts' queries ``[tokens, Hq, D]`` with the step's own keys and values at full precision, older
         tokens as the cache holds them, and the append (``head_dim`` 128; what ``QuantizedKVCache.prefill`` does, request by
         request on the prompt attention kernel).  The host needs the lengths: where they were given as tensors it waits for
-        them, once for a step, but in every call where the step was planned in a graph that may have been replayed since."""
+        them, once for a step of :meth:`plan`, but in every call where a graph that may have been replayed since, or
+        :func:`plan_blocks`, made it.  Rows behind the last token hold anything.  Once per step and layer; a call that is refused has stored nothing."""
         layer = self.layers[layer_idx]
         if layer.head_dim != 128:
             raise ValueError("prefill needs head_dim 128: use attend")
