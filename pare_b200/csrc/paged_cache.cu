@@ -542,9 +542,10 @@ int pare_paged_append(const void* k, const void* v, int64_t k_stride_t, int64_t 
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int bs = l->block_size;
   const bool many = (int64_t)s.n_items * 2 * l->H * 8 * bs > (int64_t)sm_count() * 8192;
-  auto go = [&](auto kern, int team) {
-    const int threads = append_threads(team), teams = threads / team;
-    const int rc = launch_pdl(kern, dim3(s.n_items, (2 * l->H + teams - 1) / teams), dim3(threads), 0, st, p);
+  auto go = [&](auto kern, int team) -> int {
+    const int threads = append_threads(team), teams = threads / team, groups = (2 * l->H + teams - 1) / teams;
+    PARE_REQUIRE(groups <= 65535, PARE_ERR_UNSUPPORTED);      // a grid's second dimension
+    const int rc = launch_pdl(kern, dim3(s.n_items, groups), dim3(threads), 0, st, p);
     return rc != PARE_OK ? rc : launch_status();
   };
   auto by_size = [&](auto tag, auto dim) {
