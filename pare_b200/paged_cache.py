@@ -16,7 +16,7 @@ Three functions work on plain tensors, and :class:`PagedKVCache` keeps those ten
 * :func:`attend_blocks` is the attention of the step's queries over the layer: one new token per request (decode) or several
   (short prompts, continuations), causal by position.
 
-A step's tokens stay: there is no way to take some of them back (drafted tokens that a check rejects, say), for a block that they
+A step's tokens stay: there is no way to take some of them back (drafted tokens that turn out wrong, say), for a block that they
 filled up has been quantized with them, and its open rows hold the tokens behind it.  And attention reads what is stored: where a block
 fills up inside a step, the step's earlier tokens see their own block in 8 bits too, with a scale that the later ones had a part in (an
 infinity among those reaches them).  Fed one by one they would have seen it in 16 bits.
