@@ -278,12 +278,11 @@ def attend_blocks(layer: PagedLayer, step: PagedStep, q: Tensor, scale: float | 
     4096 rows: longer prompts go through :meth:`PagedKVCache.prefill` (and rows times tokens of a full row of the block table stay
     below 2^35).  Rows that belong to nobody are left as they were in
     ``out`` (``[tokens, Hq, D]``, channels adjacent, not overlapping ``q``; a new tensor, with anything in those rows, if not given)."""
-    call = _attend_arguments(layer, step, q, scale, out)
-    return _attend(layer, step, *call)
+    return _attend(layer, step, q, None, None, scale, out)
 
 
-def _attend_arguments(layer: PagedLayer, step: PagedStep, q: Tensor, scale: float | None, out: Tensor | None) -> tuple:
-    """What :func:`_attend` takes, looked over and allocated: nothing is refused after this."""
+def _attend(layer: PagedLayer, step: PagedStep, q: Tensor, new_k: Tensor | None, new_v: Tensor | None, scale: float | None, out: Tensor | None) -> Tensor:
+    """:func:`attend_blocks`, where ``new_k`` is given after :func:`append_blocks`: what is refused has not been stored either."""
     _fits(layer, step)
     tokens, d, dev = step.tokens, layer.head_dim, layer.device
     hq = q.size(1) if q.dim() == 3 else 0
@@ -291,7 +290,7 @@ def _attend_arguments(layer: PagedLayer, step: PagedStep, q: Tensor, scale: floa
         raise ValueError(f"attend_blocks: q [tokens, heads, {d}] with a multiple of {layer.heads} heads, got {list(q.shape)}")
     if tokens > MAX_QUERY_TOKENS:
         raise ValueError(f"attend_blocks takes at most {MAX_QUERY_TOKENS} rows, got {tokens}")
-    if tokens * (step.block_table.shape[1] * step.block_size // 16 + 2) >= 1 << 31:
+    if tokens > 15 and tokens * (step.block_table.shape[1] * step.block_size // 16 + 2) >= 1 << 31:      # a row of the table has less than 2^31 tokens
         raise ValueError(f"attend_blocks: {tokens} rows times {step.block_table.shape[1]} blocks of {step.block_size} tokens a request are too many to count")
     q, qp, qt, qh = _rows(q, tokens, hq, layer, "q")
     if out is None:
@@ -301,16 +300,14 @@ def _attend_arguments(layer: PagedLayer, step: PagedStep, q: Tensor, scale: floa
         raise ValueError(f"out must be {q.dtype} {list(q.shape)} on {dev} with adjacent channels")
     else:
         ot, oh, _ = out.stride()
-    return q, qp, qt, qh, hq, out, ot, oh, 1.0 / math.sqrt(d) if scale is None else float(scale)
-
-
-def _attend(layer: PagedLayer, step: PagedStep, q: Tensor, qp: int, qt: int, qh: int, hq: int, out: Tensor, ot: int, oh: int, scale: float) -> Tensor:
-    dev = layer.device
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     if dev.index != _lib.current_device():
         with torch.cuda.device(dev):
-            return _attend(layer, step, q, qp, qt, qh, hq, out, ot, oh, scale)
-    stream, nbytes = _lib.current_stream(dev), _attn_workspace(layer.head_dim, dev.index)
+            return _attend(layer, step, q, new_k, new_v, scale, out)
+    stream, nbytes = _lib.current_stream(dev), _attn_workspace(d, dev.index)
     ws = _lib.scratch(dev, nbytes, stream)
+    if new_k is not None:
+        append_blocks(layer, step, new_k, new_v)
     status = _lib.lib().pare_paged_attn(qp, qt, qh, layer._c, step._c or step._tables(), hq, out.data_ptr(), ot, oh, scale, ws.data_ptr(), nbytes, stream)
     if status:
         _lib.check(status, "pare_paged_attn")
@@ -451,10 +448,9 @@ class PagedKVCache:
                out: Tensor | None = None) -> Tensor:
         """Append the step's keys and values, then attention of its queries over the whole requests (:func:`attend_blocks`).  Once per
         step and layer; a call that is refused has stored nothing."""
-        layer = self.layers[layer_idx]
-        call = _attend_arguments(layer, step, q, scale, out)      # first: what is refused has not been stored either
-        append_blocks(layer, step, new_k, new_v)
-        return _attend(layer, step, *call)
+        if new_k is None:
+            raise ValueError("attend: the step's keys and values are needed")
+        return _attend(self.layers[layer_idx], step, q, new_k, new_v, scale, out)
 
     def prefill(self, layer_idx: int, step: PagedStep, q: Tensor, new_k: Tensor, new_v: Tensor, scale: float | None = None) -> Tensor:
         """Causal attention of prompts' queries ``[tokens, Hq, D]`` with the step's own keys and values at full precision, older
